@@ -52,6 +52,13 @@ from .pytorch_runtime import (  # noqa: F401
     patch_model_tensor_parallel,
     prepare_model,
 )
+from .paged import (  # noqa: F401
+    PagedKVCache,
+    adjust_logits,
+    paged_attention,
+    paged_gather,
+    rope_paged_append,
+)
 from ._lib import check_status, reserve_workspace, validate_compressed  # noqa: F401
 
 __all__ = [n for n in dir() if not n.startswith("_")]

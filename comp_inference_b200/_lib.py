@@ -38,6 +38,28 @@ class DenseWeight(C.Structure):
                 ("N", C.c_uint32), ("tile_h", C.c_uint32), ("tile_w", C.c_uint32)]
 
 
+class PagedCache(C.Structure):
+    """struct ci_paged_cache"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("num_pages", C.c_uint32), ("page_size", C.c_uint32), ("n_kv", C.c_uint32), ("head_dim", C.c_uint32),
+                ("bits", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class PagedBatch(C.Structure):
+    """struct ci_paged_batch"""
+    _fields_ = [("block_table", C.c_void_p), ("kv_lens", C.c_void_p), ("q_starts", C.c_void_p), ("B", C.c_uint32),
+                ("max_pages", C.c_uint32), ("T", C.c_uint32), ("table_stride", C.c_uint32)]
+
+
+class LogitAdjust(C.Structure):
+    """struct ci_logit_adjust"""
+    _fields_ = [("d_in", C.c_void_p), ("d_out", C.c_void_p), ("ld_in", C.c_int64), ("ld_out", C.c_int64),
+                ("d_tokens", C.c_void_p), ("d_lens", C.c_void_p), ("d_prompt_lens", C.c_void_p), ("ld_tokens", C.c_int64),
+                ("d_repetition", C.c_void_p), ("d_presence", C.c_void_p), ("d_frequency", C.c_void_p),
+                ("d_bias_ids", C.c_void_p), ("d_bias", C.c_void_p), ("ld_bias", C.c_int64), ("d_mask", C.c_void_p),
+                ("ld_mask", C.c_int64), ("B", C.c_uint32), ("V", C.c_uint32), ("L", C.c_uint32), ("n_bias", C.c_uint32)]
+
+
 # Every entry point of the header, with its argument types.  tests check this
 # table against the header and against the symbols the library exports.
 _V, _S = C.c_void_p, C.c_void_p
@@ -106,6 +128,13 @@ SIGNATURES = {
                                       C.c_float, _V, C.c_size_t, _V, C.c_int64, _S]),
     "ci_greedy_step": (C.c_int, [_V, C.c_int64, C.c_uint32, C.c_uint32, _V, _V, _V, _V, C.c_int64, _V, _S]),
     "ci_silu_mul": (C.c_int, [_V, C.c_int64, _V, C.c_int64, C.c_uint32, C.c_uint32, _V, C.c_int64, _S]),
+    "ci_rope_paged_append": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedBatch), _V, C.c_int64, _V, C.c_int64, _V, C.c_int64,
+                                       C.c_uint32, _V, _V, C.c_uint32, _V, _S]),
+    "ci_paged_gather": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedBatch), _V, _V, _S]),
+    "ci_paged_attention_workspace_bytes": (C.c_size_t, [C.c_uint32]),
+    "ci_paged_attention": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedBatch), _V, C.c_int64, C.c_uint32, C.c_uint32,
+                                     C.c_uint32, C.c_uint32, C.c_float, _V, C.c_size_t, _V, C.c_int64, _S]),
+    "ci_adjust_logits": (C.c_int, [C.POINTER(LogitAdjust), _S]),
     "ci_allreduce_buffer_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32]),
     "ci_allreduce_counter_bytes": (C.c_size_t, []),
     "ci_linear_allreduce_counter_bytes": (C.c_size_t, []),

@@ -7,12 +7,15 @@
 // 0.47 is finding that the module's buffers are still the same; the kernel itself takes 5.6.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <mutex>
 #include <optional>
+#include <sstream>
 #include <unordered_map>
 
 #include "../../include/comp_inference_b200.h"
@@ -497,6 +500,281 @@ PyObject *linear_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return THPVariable_Wrap(linear_call(h, THPVariable_Unpack(args[4]), bias, std::nullopt, v[2], false, v[3]));
     END_HANDLE_TH_ERRORS
 }
+// ---- serving over a paged cache --------------------------------------------------------------------------
+// Shapes and types first, the device last: what is wrong with a call shows without one.
+
+void refuse(bool wrong, const std::string &what) {
+    if (wrong) throw py::value_error(what);
+}
+std::string shape_of(const Tensor &t) {
+    std::ostringstream o;
+    o << t.sizes();
+    return o.str();
+}
+void want(const Tensor &t, at::ScalarType type, const char *name) {
+    TORCH_CHECK(t.scalar_type() == type, name, " must be torch.", type, ", got torch.", t.scalar_type());
+}
+void same_device(const Tensor &t, const Tensor &like, const char *name) {
+    require_cuda(t, name);
+    TORCH_CHECK(t.device() == like.device(), name, " is on ", t.device(), ", the others on ", like.device());
+}
+bool aligned16(const Tensor &t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
+
+// Pages of one layer and their descriptor.
+struct PagedCache {
+    Tensor k, v, k_scale, v_scale;
+    ci_paged_cache c;
+
+    PagedCache(const Tensor &k_, const Tensor &v_, const OptTensor &ks, const OptTensor &vs) : k(k_), v(v_) {
+        const bool four = k.scalar_type() == at::kByte;
+        TORCH_CHECK(four || k.scalar_type() == at::kBFloat16, "pages must be bfloat16, or uint8 for codes of 4 bits, got torch.", k.scalar_type());
+        want(v, k.scalar_type(), "pages of values");
+        refuse(k.dim() != 4 || k.sizes() != v.sizes(), "pages must be two tensors [num_pages, n_kv, page_size, row], got " + shape_of(k) + " and " + shape_of(v));
+        refuse(!k.is_contiguous() || !v.is_contiguous(), "pages must be contiguous");
+        const int64_t d = k.size(3) * (four ? 2 : 1);
+        refuse(d != 64 && d != 128 && d != 256, "head dimension " + std::to_string(d) + " must be 64, 128 or 256");
+        const int64_t page = k.size(2);
+        refuse(page != 16 && page != 32 && page != 64 && page != 128, "pages of " + std::to_string(page) + " tokens; 16, 32, 64 or 128");
+        refuse(k.size(0) < 1 || k.size(0) > 0x7FFFFFFF || k.size(1) < 1 || k.size(1) > 65535, "a cache of " + shape_of(k));
+        refuse(four != (ks.has_value() && vs.has_value()) || ks.has_value() != vs.has_value(), "a cache of 4 bits, and no other, has two tensors of steps and lowest values");
+        if (four) {
+            k_scale = *ks;
+            v_scale = *vs;
+            want(k_scale, at::kBFloat16, "steps and lowest values");
+            want(v_scale, at::kBFloat16, "steps and lowest values");
+            const std::vector<int64_t> s{k.size(0), k.size(1), page, d / 64, 2};
+            refuse(k_scale.sizes() != at::IntArrayRef(s) || v_scale.sizes() != at::IntArrayRef(s) || !k_scale.is_contiguous() || !v_scale.is_contiguous(),
+                   "steps and lowest values must be contiguous [num_pages, n_kv, page_size, head_dim / 64, 2], got " + shape_of(k_scale) + " and " + shape_of(v_scale));
+        }
+        require_cuda(k, "pages");
+        same_device(v, k, "pages of values");
+        if (four) {
+            same_device(k_scale, k, "steps and lowest values");
+            same_device(v_scale, k, "steps and lowest values");
+        }
+        memset(&c, 0, sizeof c);
+        c.k = k.data_ptr();
+        c.v = v.data_ptr();
+        c.k_scale = four ? (uint32_t *)k_scale.data_ptr() : nullptr;
+        c.v_scale = four ? (uint32_t *)v_scale.data_ptr() : nullptr;
+        c.num_pages = (uint32_t)k.size(0);
+        c.page_size = (uint32_t)page;
+        c.n_kv = (uint32_t)k.size(1);
+        c.head_dim = (uint32_t)d;
+        c.bits = four ? 4 : 16;
+        for (const Tensor *t : {&k, &v, &k_scale, &v_scale}) refuse(t->defined() && !aligned16(*t), "pages must be 16-byte aligned");
+        bytes = k.nbytes();
+        scale_bytes = four ? k_scale.nbytes() : 0;
+    }
+    // A tensor may have been given other memory since (resize_, .data): the kernels go by what it has now.
+    const ci_paged_cache *now() {
+        refuse((size_t)k.nbytes() != bytes || (size_t)v.nbytes() != bytes || (k_scale.defined() && ((size_t)k_scale.nbytes() != scale_bytes || (size_t)v_scale.nbytes() != scale_bytes)),
+               "the pages have another size than when the cache was made");
+        c.k = k.data_ptr();
+        c.v = v.data_ptr();
+        if (k_scale.defined()) {
+            c.k_scale = (uint32_t *)k_scale.data_ptr();
+            c.v_scale = (uint32_t *)v_scale.data_ptr();
+        }
+        return &c;
+    }
+
+private:
+    size_t bytes, scale_bytes;
+};
+
+ci_paged_batch paged_batch(const PagedCache &cache, const Tensor &table, const Tensor &kv_lens, const OptTensor &q_starts, int64_t T) {
+    want(table, at::kInt, "block_table");
+    want(kv_lens, at::kInt, "kv_lens");
+    refuse(table.dim() != 2 || (table.size(1) > 1 && table.stride(1) != 1), "block_table must be [sequences, pages] with unit inner stride");
+    const int64_t B = table.size(0);
+    refuse(kv_lens.dim() != 1 || kv_lens.size(0) != B || (B > 1 && kv_lens.stride(0) != 1), "kv_lens must have one entry for each of " + std::to_string(B) + " sequences");
+    const int64_t stride = B > 1 ? table.stride(0) : table.size(1);
+    refuse(B > (1 << 20) || T > (1 << 30), "too many sequences or tokens");
+    refuse(stride < table.size(1) || stride > 0x7FFFFFFF || table.size(1) * (int64_t)cache.c.page_size > (1 << 30), "a block table of " + shape_of(table));
+    if (q_starts.has_value()) {
+        want(*q_starts, at::kInt, "q_starts");
+        refuse(q_starts->dim() != 1 || q_starts->size(0) != B + 1 || q_starts->stride(0) != 1, "q_starts must have " + std::to_string(B + 1) + " entries");
+    } else {
+        refuse(T != B, std::to_string(T) + " tokens for " + std::to_string(B) + " sequences: q_starts says which are whose");
+    }
+    same_device(table, cache.k, "block_table");
+    same_device(kv_lens, cache.k, "kv_lens");
+    if (q_starts.has_value()) same_device(*q_starts, cache.k, "q_starts");
+    ci_paged_batch b;
+    b.block_table = (const int32_t *)table.data_ptr();
+    b.kv_lens = (const int32_t *)kv_lens.data_ptr();
+    b.q_starts = q_starts.has_value() ? (const int32_t *)q_starts->data_ptr() : nullptr;
+    b.B = (uint32_t)B;
+    b.max_pages = (uint32_t)table.size(1);
+    b.T = (uint32_t)T;
+    b.table_stride = (uint32_t)stride;
+    return b;
+}
+
+// [T, heads, d] or [T, heads * d] with the heads side by side, as rows `ld` apart; copied where `align` asks for 16-byte rows
+// that it does not have.
+struct HeadRows {
+    Tensor keep;
+    const uint16_t *ptr;
+    int64_t T, heads, ld;
+};
+HeadRows head_rows(const Tensor &x, int64_t d, const char *name, bool align) {
+    want(x, at::kBFloat16, name);
+    refuse(x.dim() < 2 || x.dim() > 3 || (x.dim() == 3 ? x.size(2) != d : x.size(1) % d != 0),
+           std::string(name) + " must be [tokens, heads, " + std::to_string(d) + "] or [tokens, heads * " + std::to_string(d) + "], got " + shape_of(x));
+    HeadRows r;
+    r.T = x.size(0);
+    r.heads = x.dim() == 3 ? x.size(1) : x.size(1) / d;
+    refuse(r.heads < 1 || r.heads > 65535, std::string(name) + " has " + std::to_string(r.heads) + " heads");
+    const bool side_by_side = x.stride(-1) == 1 && (x.dim() == 2 || x.size(1) == 1 || x.stride(1) == d);
+    // rows that overlap (an expanded tensor) are copied too
+    const bool rows = r.T <= 1 || x.stride(0) >= r.heads * d;
+    const bool ok = side_by_side && rows && (!align || (aligned16(x) && (r.T <= 1 || x.stride(0) % 8 == 0)));
+    r.keep = ok ? x : x.contiguous();
+    if (align && !aligned16(r.keep)) r.keep = r.keep.clone();
+    r.ld = r.T > 1 ? r.keep.stride(0) : r.heads * d;
+    r.ptr = (const uint16_t *)r.keep.data_ptr();
+    return r;
+}
+
+Tensor paged_append(PagedCache &cache, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &cos, const Tensor &sin,
+                    const Tensor &table, const Tensor &kv_lens, const OptTensor &q_starts, const OptTensor &out) {
+    const int64_t d = cache.c.head_dim, n_kv = cache.c.n_kv;
+    const HeadRows rq = head_rows(q, d, "q", false), rk = head_rows(k, d, "k", false), rv = head_rows(v, d, "v", false);
+    refuse(rk.T != rq.T || rv.T != rq.T, "q, k and v have " + std::to_string(rq.T) + ", " + std::to_string(rk.T) + " and " + std::to_string(rv.T) + " tokens");
+    refuse(rk.heads != n_kv || rv.heads != n_kv, "k and v have " + std::to_string(rk.heads) + " and " + std::to_string(rv.heads) + " heads, the cache " + std::to_string(n_kv));
+    want(cos, at::kBFloat16, "cos");
+    want(sin, at::kBFloat16, "sin");
+    refuse(cos.dim() != 2 || cos.size(1) != d || cos.sizes() != sin.sizes() || !cos.is_contiguous() || !sin.is_contiguous() || cos.size(0) > 0x7FFFFFFF,
+           "cos and sin must be contiguous tables [positions, " + std::to_string(d) + "]");
+    Tensor y;
+    if (out.has_value()) {
+        y = *out;
+        want(y, at::kBFloat16, "out");
+        refuse(y.numel() != rq.T * rq.heads * d || !y.is_contiguous() || !aligned16(y), "out must be a contiguous, 16-byte aligned tensor of the size of q");
+    }
+    const ci_paged_batch b = paged_batch(cache, table, kv_lens, q_starts, rq.T);
+    for (const Tensor *t : {&q, &k, &v, &cos, &sin}) same_device(*t, cache.k, "an argument");
+    const c10::cuda::CUDAGuard guard(cache.k.device());
+    if (out.has_value()) same_device(y, cache.k, "out");
+    else y = at::empty({rq.T, rq.heads, d}, q.options());
+    if (rq.T == 0 || b.B == 0) return y;
+    check(ci_rope_paged_append(cache.now(), &b, rq.ptr, rq.ld, rk.ptr, rk.ld, rv.ptr, rv.ld, (uint32_t)rq.heads, (const uint16_t *)cos.data_ptr(),
+                               (const uint16_t *)sin.data_ptr(), (uint32_t)cos.size(0), (uint16_t *)y.data_ptr(), stream()));
+    return y;
+}
+
+py::tuple paged_gather(PagedCache &cache, const Tensor &table, const Tensor &kv_lens, const OptTensor &starts, int64_t total) {
+    refuse(total < 0, "a negative number of rows");
+    const ci_paged_batch b = paged_batch(cache, table, kv_lens, starts, total);
+    const c10::cuda::CUDAGuard guard(cache.k.device());
+    const auto options = cache.k.options().dtype(at::kBFloat16);
+    Tensor k = at::empty({total, cache.c.n_kv, cache.c.head_dim}, options), v = at::empty({total, cache.c.n_kv, cache.c.head_dim}, options);
+    if (total > 0 && b.B > 0) check(ci_paged_gather(cache.now(), &b, (uint16_t *)k.data_ptr(), (uint16_t *)v.data_ptr(), stream()));
+    return py::make_tuple(k, v);
+}
+
+Tensor paged_attention(PagedCache &cache, const Tensor &q, const Tensor &table, const Tensor &kv_lens, const OptTensor &q_starts,
+                       int64_t max_q_len, int64_t window, int64_t sinks, std::optional<double> scale, const OptTensor &out) {
+    const int64_t d = cache.c.head_dim;
+    const HeadRows r = head_rows(q, d, "q", true);
+    refuse(r.heads % cache.c.n_kv != 0, std::to_string(r.heads) + " query heads over " + std::to_string(cache.c.n_kv) + " key/value heads");
+    refuse(window < 0 || sinks < 0 || max_q_len < 0, "window, sinks and max_q_len must not be negative");
+    constexpr int64_t most = 0x7FFFFFFF;
+    refuse(r.T * r.heads > most, std::to_string(r.T) + " tokens of " + std::to_string(r.heads) + " heads");
+    Tensor y;
+    if (out.has_value()) {
+        y = *out;
+        want(y, at::kBFloat16, "out");
+        refuse(y.dim() != 2 || y.size(0) != r.T || y.size(1) != r.heads * d || (r.T && y.stride(1) != 1) || (r.T > 1 && (y.stride(0) % 8 || y.stride(0) < r.heads * d)) || !aligned16(y),
+               "out must be [tokens, heads * head_dim] with 16-byte aligned rows");
+    }
+    const ci_paged_batch b = paged_batch(cache, table, kv_lens, q_starts, r.T);
+    same_device(q, cache.k, "q");
+    const c10::cuda::CUDAGuard guard(cache.k.device());
+    if (out.has_value()) same_device(y, cache.k, "out");
+    else y = at::empty({r.T, r.heads * d}, q.options());
+    if (r.T == 0 || b.B == 0) return y;
+    // of this call: from the allocator's pool of the stream, or of the graph that is being captured
+    const Tensor ws = at::empty({(int64_t)ci_paged_attention_workspace_bytes((uint32_t)d)}, q.options().dtype(at::kByte));
+    check(ci_paged_attention(cache.now(), &b, r.ptr, r.ld, (uint32_t)r.heads, (uint32_t)std::min(max_q_len, most), (uint32_t)std::min(window, most),
+                             (uint32_t)std::min(sinks, most), (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)d)), ws.data_ptr(),
+                             ws.nbytes(), (uint16_t *)y.data_ptr(), r.T > 1 ? y.stride(0) : r.heads * d, stream()));
+    return y;
+}
+
+Tensor adjust_logits(const Tensor &logits, const OptTensor &tokens, const OptTensor &lens, const OptTensor &prompt_lens, const OptTensor &repetition,
+                     const OptTensor &presence, const OptTensor &frequency, const OptTensor &bias_ids, const OptTensor &bias,
+                     const OptTensor &mask, const OptTensor &out) {
+    want(logits, at::kBFloat16, "logits");
+    refuse(logits.dim() != 2 || logits.size(1) < 1 || logits.size(1) > 0x7FFFFFFF || logits.size(0) > 65535 || logits.stride(1) != 1 ||
+               (logits.size(0) > 1 && logits.stride(0) < logits.size(1)),
+           "logits must be [sequences, vocabulary] with unit inner stride, got " + shape_of(logits));
+    const int64_t B = logits.size(0), V = logits.size(1);
+    ci_logit_adjust a;
+    memset(&a, 0, sizeof a);
+    a.B = (uint32_t)B;
+    a.V = (uint32_t)V;
+    std::vector<std::pair<const Tensor *, const char *>> given;
+    auto rows = [&](const OptTensor &t, at::ScalarType type, int64_t cols, const char *name, int64_t &ld) -> const void * {
+        want(*t, type, name);
+        refuse(t->dim() != 2 || t->size(0) != B || (cols >= 0 && t->size(1) < cols) || (t->size(1) > 1 && t->stride(1) != 1),
+               std::string(name) + " must have a row for each of " + std::to_string(B) + " sequences" + (cols > 0 ? ", of " + std::to_string(cols) + " entries" : "") + ", got " + shape_of(*t));
+        ld = B > 1 ? t->stride(0) : t->size(1);
+        refuse(ld < t->size(1), std::string(name) + " has rows that overlap");
+        given.emplace_back(&*t, name);
+        return t->data_ptr();
+    };
+    auto each = [&](const OptTensor &t, at::ScalarType type, const char *name) -> const void * {
+        if (!t.has_value()) return nullptr;
+        want(*t, type, name);
+        refuse(t->dim() != 1 || t->size(0) != B || (B > 1 && t->stride(0) != 1), std::string(name) + " must have one entry for each of " + std::to_string(B) + " sequences");
+        given.emplace_back(&*t, name);
+        return t->data_ptr();
+    };
+    refuse(!tokens.has_value() && (lens.has_value() || prompt_lens.has_value() || repetition.has_value() || presence.has_value() || frequency.has_value()),
+           "penalties need the tokens that have been");
+    if (tokens.has_value()) {
+        refuse(!lens.has_value(), "tokens need their lengths");
+        a.d_tokens = (const int64_t *)rows(tokens, at::kLong, -1, "tokens", a.ld_tokens);
+        refuse(tokens->size(1) > 0x7FFFFFFF, "a history of " + shape_of(*tokens));
+        a.L = (uint32_t)tokens->size(1);
+        a.d_lens = (const int32_t *)each(lens, at::kInt, "lens");
+        a.d_prompt_lens = (const int32_t *)each(prompt_lens, at::kInt, "prompt_lens");
+        a.d_repetition = (const float *)each(repetition, at::kFloat, "repetition");
+        a.d_presence = (const float *)each(presence, at::kFloat, "presence");
+        a.d_frequency = (const float *)each(frequency, at::kFloat, "frequency");
+    }
+    refuse(bias_ids.has_value() != bias.has_value(), "biases need their tokens, and the tokens their biases");
+    if (bias.has_value()) {
+        int64_t ld = 0;
+        a.d_bias_ids = (const int64_t *)rows(bias_ids, at::kLong, -1, "bias_ids", a.ld_bias);
+        a.d_bias = (const float *)rows(bias, at::kFloat, -1, "bias", ld);
+        refuse(bias->sizes() != bias_ids->sizes() || (B > 1 && ld != a.ld_bias) || bias->size(1) > 0x7FFFFFFF, "bias and bias_ids must be laid out alike");
+        a.n_bias = (uint32_t)bias->size(1);
+    }
+    if (mask.has_value()) a.d_mask = (const uint32_t *)rows(mask, at::kInt, (V + 31) / 32, "mask", a.ld_mask);
+    Tensor y;
+    if (out.has_value()) {
+        y = *out;
+        want(y, at::kBFloat16, "out");
+        refuse(y.sizes() != logits.sizes() || y.stride(1) != 1 || (B > 1 && y.stride(0) < V), "out must be like logits, with unit inner stride");
+    }
+    require_cuda(logits, "logits");
+    for (const auto &g : given) same_device(*g.first, logits, g.second);
+    const c10::cuda::CUDAGuard guard(logits.device());
+    if (out.has_value()) same_device(y, logits, "out");
+    else y = at::empty({B, V}, logits.options());
+    if (B == 0) return y;
+    a.d_in = (const uint16_t *)logits.data_ptr();
+    a.d_out = (uint16_t *)y.data_ptr();
+    a.ld_in = B > 1 ? logits.stride(0) : V;
+    a.ld_out = B > 1 ? y.stride(0) : V;
+    check(ci_adjust_logits(&a, stream()));
+    return y;
+}
+
 PyMethodDef fast_calls[] = {{"linear_of", (PyCFunction)(void (*)(void))linear_of, METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace
@@ -517,5 +795,11 @@ PYBIND11_MODULE(_ci_host, m) {
              py::arg("transposed") = false, py::arg("prefill_rows") = 0)
         .def("embedding", &embedding_call, py::arg("x"), py::arg("out") = py::none())
         .def("decode", &decode_call, py::arg("bf16"));
+    py::class_<PagedCache>(m, "PagedCache", "Descriptor of one layer's pages and the tensors it points into")
+        .def(py::init<const Tensor &, const Tensor &, const OptTensor &, const OptTensor &>())
+        .def("append", &paged_append)
+        .def("gather", &paged_gather)
+        .def("attention", &paged_attention);
+    m.def("adjust_logits", &adjust_logits);
     m.def("compress", &compress, py::arg("weight"), py::arg("tile_h"), py::arg("tile_w"), py::arg("want_man_hist"));
 }

@@ -282,3 +282,8 @@ def greedy_step(logits, tok, pos, steps_done, out, ticket):
     _lib.check(_lib.load().ci_greedy_step(_lib.ptr(l2), l2.stride(0), B, V, _lib.ptr(tok), _lib.ptr(pos),
                                           _lib.ptr(steps_done), _lib.ptr(out), out.shape[1], _lib.ptr(ticket),
                                           _lib.stream()))
+
+
+# ---- the same over a paged cache, and the logits before greedy_step (csrc/paged_*.cu, csrc/logits.cu) ----
+
+from .paged import adjust_logits, paged_attention, paged_gather, rope_paged_append  # noqa: E402, F401

@@ -395,6 +395,82 @@ int ci_decode_attention(const uint16_t *d_q, const uint16_t *d_k_cache, const ui
 int ci_silu_mul(const uint16_t *d_gate, int64_t ldg, const uint16_t *d_up, int64_t ldu, uint32_t rows, uint32_t cols,
                 uint16_t *d_out, int64_t ldo, ci_stream_t stream);
 
+/* ---- serving over a paged key/value cache ------------------------------------------ */
+
+/* One layer's cache: pages of `page_size` tokens (16, 32, 64 or 128) for each key/value head, [num_pages, n_kv, page_size, row],
+ * keys and values apart.  bits = 16: a row is head_dim bf16.  bits = 4: a row is head_dim codes of 4 bits, beside it
+ * head_dim / 64 words of (step in the low half, lowest in the high one), both bf16: code c of a group of 64 channels stands for
+ * lowest + step * c.  The 32-bit word p of a row of codes belongs to group p % G (G = head_dim / 64) and holds channels
+ * 8 (p / G) .. + 7 of it, channel i of those in bits 4 (i / 2) + 16 (i % 2).  All four arrays 16-byte aligned; k_scale and
+ * v_scale are not looked at where bits = 16.  head_dim 64, 128 or 256.  No counterpart in the reference (it leaves the
+ * cache to Hugging Face's modules). */
+typedef struct ci_paged_cache {
+    void *k, *v;
+    uint32_t *k_scale, *v_scale;
+    uint32_t num_pages, page_size, n_kv, head_dim, bits, reserved;
+} ci_paged_cache;
+
+/* The sequences of a call: row b of block_table [B, max_pages] (rows table_stride
+ * entries apart) names the pages of sequence b in order, kv_lens[b] counts its
+ * tokens, the new ones among them; its new tokens are rows q_starts[b] .. q_starts[b + 1] - 1 of the call's T rows, the last ones
+ * of the sequence (q_starts [B + 1], ascending; null: row b alone).  All three are device memory and read when the kernel runs,
+ * so a captured call goes by what they hold at its replay.  An id outside the pool, or a position past the table's row, names no
+ * page: nothing is written there and no query sees it.  Rows behind the last sequence are left alone.
+ * max_pages * page_size <= 2^30, B <= 2^20. */
+typedef struct ci_paged_batch {
+    const int32_t *block_table, *kv_lens, *q_starts;
+    uint32_t B, max_pages, T, table_stride;
+} ci_paged_batch;
+
+/* Rotary embedding (rotate-half convention, bf16 tables [table_len, head_dim]) of the new tokens, and their way into the cache:
+ * q_out[t][h] = rot(q[t][h]) for n_q heads (row strides ldq / ldk / ldv in elements), rot(k) and v to the page and place of
+ * the token's position.  bits = 4: of each 64 channels (after rotation and rounding to bf16) lowest = min,
+ * step = bf16((max - min) / 15), code = round((x - lowest) / step) in [0, 15]; a NaN, or a span that is not finite, makes the
+ * group NaN.  A token whose position is negative or past the tables gets a zero row of q_out and goes nowhere. */
+int ci_rope_paged_append(const ci_paged_cache *cache, const ci_paged_batch *batch, const uint16_t *d_q, int64_t ldq,
+                         const uint16_t *d_k, int64_t ldk, const uint16_t *d_v, int64_t ldv, uint32_t n_q, const uint16_t *d_cos,
+                         const uint16_t *d_sin, uint32_t table_len, uint16_t *d_q_out, ci_stream_t stream);
+
+/* k_out[t][h], v_out[t][h] (bf16 [T, n_kv, head_dim]) = the cache's rows at the positions of the batch's tokens; zeros where
+ * there is no page. */
+int ci_paged_gather(const ci_paged_cache *cache, const ci_paged_batch *batch, uint16_t *d_k_out, uint16_t *d_v_out,
+                    ci_stream_t stream);
+
+/* out[t][h] = softmax over j of (scale * q[t][h] . K[j]) times V[j], key/value head h / (n_q / n_kv), over the positions
+ * j <= i of the token's sequence (i: the token's own position) with i - j < window or j < sinks; window = 0: all j <= i.  A
+ * token that sees nothing gets zeros.  q rows ldq elements apart, heads head_dim apart, both 16-byte aligned, and out alike
+ * with ldo.  max_q_len: no sequence has more new tokens (0: not known; it chooses kernels, and longer ones are served all
+ * the same).  d_workspace: ci_paged_attention_workspace_bytes, 16-byte aligned, its contents do not matter; calls that
+ * overlap on the GPU must not share one. */
+size_t ci_paged_attention_workspace_bytes(uint32_t head_dim);
+int ci_paged_attention(const ci_paged_cache *cache, const ci_paged_batch *batch, const uint16_t *d_q, int64_t ldq, uint32_t n_q,
+                       uint32_t max_q_len, uint32_t window, uint32_t sinks, float scale, void *d_workspace,
+                       size_t workspace_bytes, uint16_t *d_out, int64_t ldo, ci_stream_t stream);
+
+/* Logits [B, V] (bf16, rows ld_in / ld_out apart; d_out may be d_in) as a sampler adjusts them, in fp32 with one rounding:
+ *   x / r (x > 0) or x * r, r = d_repetition[b], for tokens of the history d_tokens[b][0 .. d_lens[b]);
+ *   - d_frequency[b] * count - d_presence[b] (count > 0), count over d_tokens[b][d_prompt_lens[b] .. d_lens[b]);
+ *   + the sum of d_bias[b][i] over the i with d_bias_ids[b][i] == token;
+ *   -inf for tokens whose bit (token % 32 of word token / 32 of d_mask[b]) is 0.
+ * Null d_tokens, d_repetition, d_presence, d_frequency, d_mask or n_bias = 0 leaves that step out; null d_prompt_lens: all of the
+ * history counts.  Token ids outside [0, V) are passed over.  No counterpart in the reference. */
+typedef struct ci_logit_adjust {
+    const uint16_t *d_in;
+    uint16_t *d_out;
+    int64_t ld_in, ld_out;
+    const int64_t *d_tokens;
+    const int32_t *d_lens, *d_prompt_lens;
+    int64_t ld_tokens;
+    const float *d_repetition, *d_presence, *d_frequency;
+    const int64_t *d_bias_ids;
+    const float *d_bias;
+    int64_t ld_bias;
+    const uint32_t *d_mask;
+    int64_t ld_mask;
+    uint32_t B, V, L, n_bias;
+} ci_logit_adjust;
+int ci_adjust_logits(const ci_logit_adjust *d, ci_stream_t stream);
+
 /* ---- tensor-parallel exchange ---------------------------------------------- */
 
 /* One-shot all-reduce (sum) of a small bf16 tensor over peer memory, for the outputs of row-parallel linears.
