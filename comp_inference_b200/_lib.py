@@ -134,6 +134,7 @@ SIGNATURES = {
     "ci_paged_attention_workspace_bytes": (C.c_size_t, [C.c_uint32]),
     "ci_paged_attention": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedBatch), _V, C.c_int64, C.c_uint32, C.c_uint32,
                                      C.c_uint32, C.c_uint32, C.c_float, _V, C.c_size_t, _V, C.c_int64, _S]),
+    "ci_paged_status": (C.c_int, [u32p, C.c_int, _S]),
     "ci_adjust_logits": (C.c_int, [C.POINTER(LogitAdjust), _S]),
     "ci_allreduce_buffer_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32]),
     "ci_allreduce_counter_bytes": (C.c_size_t, []),
@@ -333,6 +334,8 @@ def check_status(device=None, clear=True):
     for ws in _status_words(device):
         word = lib.ci_workspace_status_word(ptr(ws))
         check(lib.ci_status(C.c_void_p(word), None, 1 if clear else 0, stream()))
+    with torch.cuda.device(device):
+        check(lib.ci_paged_status(None, 1 if clear else 0, stream()))
 
 
 def validate_compressed(c, K=None, N=None, th=None, tw=None, max_tile_len=0):

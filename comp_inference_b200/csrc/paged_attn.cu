@@ -425,14 +425,14 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
                 } else {
 #pragma unroll
                     for (int gr = 0; gr < G; ++gr) {
-                        // v = low + step c: the step goes with the weight, and the same rounded product that the
-                        // instructions get takes the 128 off again
+                        // v = low + step c = middle + step (c - 8): the step goes with the weight; what its product loses
+                        // by rounding counts c - 8 times, and the same rounded product takes the 128 + 8 off again
                         uint32_t pb[NR][2];
 #pragma unroll
                         for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                const float step = lo_bf16(f[u].vs[j][gr]), low = hi_bf16(f[u].vs[j][gr]);
+                                const float step = lo_bf16(f[u].vs[j][gr]), low = hi_bf16(f[u].vs[j][gr]) + 8.f * step;
                                 const float x0 = pr[nr][2 * j], x1 = pr[nr][2 * j + 1];
                                 uint32_t y = pack_bf16(x0 * step, x1 * step);
                                 float c0 = x0 * low, c1 = x1 * low;
@@ -440,8 +440,8 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
                                     if (x0 == 0.f) { y &= 0xFFFF0000u; c0 = 0.f; }
                                     if (x1 == 0.f) { y &= 0x0000FFFFu; c1 = 0.f; }
                                 }
-                                corr[nr][gr][0] += c0 - 128.f * lo_bf16(y);
-                                corr[nr][gr][1] += c1 - 128.f * hi_bf16(y);
+                                corr[nr][gr][0] += c0 - 136.f * lo_bf16(y);
+                                corr[nr][gr][1] += c1 - 136.f * hi_bf16(y);
                                 pb[nr][j] = transpose8x8(y);
                             }
                         const uint32_t a01 = __byte_perm(f[u].v[0][gr], f[u].v[1][gr], 0x5410);
@@ -571,6 +571,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Page
 }
 
 constexpr uint32_t kPaMaxRows = 16;              // widest group of query rows of any variant
+constexpr uint32_t kPaRows = 64;                 // query rows of a sequence and key head up to which this kernel has them
 constexpr uint32_t kPaMaxResident = 4;           // blocks of a multiprocessor that the workspace has room for
 
 // As many blocks as fit on the device at once: a block more would start when the others have ended.
@@ -646,19 +647,23 @@ int ci_paged_attention(const ci_paged_cache *c, const ci_paged_batch *batch, con
     a.window = (int32_t)(window >= kFar ? 0 : window);
     a.sinks = (int32_t)(sinks >= kFar ? kFar : sinks);
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.max_rows = 0xFFFFFFFFu;
     a.out = d_out;
     a.ldo = ldo;
     const size_t blocks = (size_t)sm_count() * kPaMaxResident;
     a.desc = (int32_t *)d_workspace;
     a.ml = (float *)(a.desc + blocks * 8);
     a.partial = a.ml + blocks * 2 * kPaMaxRows * 2;
-    const uint32_t longest = batch->q_starts == nullptr ? 1 : max_q_len ? max_q_len : a.p.T;
-    const bool wide = (uint64_t)longest * a.group > 8;
+    const uint64_t longest = batch->q_starts == nullptr ? 1 : max_q_len && max_q_len < a.p.T ? max_q_len : a.p.T;
+    // Sequences of many new tokens go to the tensor cores' kernel, the others to this one; both look at every sequence.
+    const bool prompts = batch->q_starts != nullptr && longest * a.group > kPaRows && a.group <= 128;
+    a.max_rows = prompts ? kPaRows : 0xFFFFFFFFu;
+    const bool wide = longest * a.group > 8;
     cudaStream_t s = (cudaStream_t)stream;
-    return c->head_dim == 64    ? launch_attention_bits<64>(a, c->bits, wide, s)
-           : c->head_dim == 128 ? launch_attention_bits<128>(a, c->bits, wide, s)
-                                : launch_attention_bits<256>(a, c->bits, wide, s);
+    const int rc = c->head_dim == 64    ? launch_attention_bits<64>(a, c->bits, wide, s)
+                   : c->head_dim == 128 ? launch_attention_bits<128>(a, c->bits, wide, s)
+                                        : launch_attention_bits<256>(a, c->bits, wide, s);
+    if (rc != CI_OK || !prompts) return rc;
+    return launch_paged_prompt(c, a.p, d_q, ldq, n_q, a.window, a.sinks, a.scale_log2, kPaRows, d_out, ldo, s);
 }
 
 }  // extern "C"

@@ -1,0 +1,549 @@
+// Attention of many new tokens over a paged cache, on the tensor cores (tcgen05): the prompts, and parts of prompts, of a
+// batch.  The same result as k_paged_attention (paged_attn.cu), which has the sequences with few.
+//
+// A block has two tiles of 128 query rows (one where head_dim = 256) of one key/value head: `tt` tokens by the heads that
+// share it, side by side, so that grouped heads read their keys once.  It walks over tiles of 128 positions:
+//   S = Q . K^T        Q and K in shared memory (128-byte swizzle), S fp32 in tensor memory
+//   P = exp2(S scale - m), written back in bf16 over S by the row's own thread: no exchange between threads at all
+//   O += P . V         P from tensor memory, V as it lies (its rows are the k index: an MN-major operand), O in tensor memory
+// While one tile's threads are at their exponentials the tensor cores work for the other.  The maximum that a row's weights
+// refer to moves only when it is exceeded by 2^8 (kLazy), so O is rarely rescaled; the row's own thread does that too,
+// between two products, when nothing else touches it.  Tiles that no row sees are not visited; a page that does not exist
+// is fetched from outside the tensor, which gives zeros.
+//
+// One warp issues the products, one the TMA copies (for 4 bits, four warps turn codes into bf16); mbarriers connect them.  All
+// waits are bounded: on expiry a role sets the status word and the abort flag, and everyone leaves.
+#include "paged.cuh"
+#include "umma.cuh"
+
+namespace ci {
+
+constexpr uint32_t kKt = 128;                // positions per tile
+constexpr float kLazy = 8.f;
+__device__ uint32_t g_prompt_status;         // code of a wait that ran out
+
+struct PromptArgs {
+    PagedBatch p;
+    const uint8_t *k, *v;                    // 4 bits only
+    const uint32_t *ks, *vs;
+    uint32_t n_q, group, tt, min_rows, negate;
+    int32_t window, sinks;
+    float scale_log2;                        // not negative
+    uint16_t *out;
+    int64_t ldo;
+};
+
+template <int D, int BITS>
+struct PromptShape {
+    static constexpr uint32_t NT = D == 256 ? 1 : 2;
+    static constexpr uint32_t kTile = kKt * D * 2, kBlock = kKt * 128;       // bytes: a tile of 128 rows, its 64-channel block
+    static constexpr uint32_t NS = D == 64 ? 6 : D == 128 ? 4 : 2;           // ring of K and V tiles
+    static constexpr uint32_t PW = BITS == 16 ? 1 : 4;                       // producer warps
+    static constexpr uint32_t kMma = 4 * NT, kProd = kMma + 1, kThreads = (kProd + PW) * 32;
+    static constexpr uint32_t oQ = 0, oRing = NT * kTile, oBar = oRing + NS * kTile, kSmem = oBar + 256 + 1024;
+    // barriers
+    static constexpr uint32_t bQ = 0, bFull = 1, bEmpty = bFull + NS, bS = bEmpty + NS, bP = bS + NT, bO = bP + NT, bFix = bO + 1;
+    static constexpr uint32_t oTmem = (bFix + 1) * 8, oAbort = oTmem + 4, oItem = oTmem + 8;
+    static_assert(oItem + 16 <= 256, "barrier region");
+    static constexpr uint32_t cO = NT * kKt;                                 // first column of O
+};
+
+__device__ __forceinline__ float ex2f(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Positions that the query tiles of a block see, and the key tiles to visit.
+struct PromptSpan {
+    int32_t p0[2], p1[2], lo[2], hi[2];      // of each query tile: first and last position, visible range; p1 < p0: no tokens
+    int32_t all_lo, all_hi, t_lo, n_sink, n;
+    __device__ __forceinline__ int32_t first(int32_t i) const { return (i < n_sink ? i : t_lo + i - n_sink) * (int32_t)kKt; }
+    __device__ __forceinline__ bool active(uint32_t t, int32_t i) const {
+        const int32_t f = first(i);
+        return p1[t] >= p0[t] && f < hi[t] && (i < n_sink || f + (int32_t)kKt > lo[t]);
+    }
+};
+
+template <int D, int BITS>
+__global__ void __launch_bounds__(PromptShape<D, BITS>::kThreads, 1)
+k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+               const __grid_constant__ CUtensorMap v_map) {
+    using Sh = PromptShape<D, BITS>;
+    constexpr uint32_t NT = Sh::NT, NS = Sh::NS, NB = D / 64;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_s = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem = smem_raw + (smem_s - smem_u32(smem_raw));
+    const uint32_t warp = threadIdx.x >> 5, lane = lane_id();
+    const PagedBatch &p = a.p;
+    auto bar = [&](uint32_t i) { return smem_s + Sh::oBar + i * 8; };
+    volatile uint32_t *s_tmem = reinterpret_cast<volatile uint32_t *>(smem + Sh::oBar + Sh::oTmem);
+    volatile uint32_t *s_abort = reinterpret_cast<volatile uint32_t *>(smem + Sh::oBar + Sh::oAbort);
+    volatile uint32_t *s_item = reinterpret_cast<volatile uint32_t *>(smem + Sh::oBar + Sh::oItem);
+
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // ---- which sequence, which tokens -------------------------------------------------------------------------
+    const uint32_t kvh = blockIdx.x % p.n_kv, item = blockIdx.x / p.n_kv, per_item = NT * a.tt;
+    if (warp == 0) {
+        auto tiles_of = [&](uint32_t b) {
+            const Seq s = load_seq(p, b);
+            return (uint64_t)s.q_len * a.group <= a.min_rows ? 0u : ((uint32_t)s.q_len + per_item - 1) / per_item;
+        };
+        const uint32_t per = (p.B + 31) / 32, b0 = min(lane * per, p.B), b1 = min(b0 + per, p.B);
+        uint32_t mine = 0;
+        for (uint32_t b = b0; b < b1; ++b) mine += tiles_of(b);
+        uint32_t incl = mine;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(kFull, incl, o);
+            if (lane >= (uint32_t)o) incl += x;
+        }
+        if (lane == 0) s_item[0] = p.B;
+        __syncwarp();
+        uint32_t before = incl - mine;
+        if (before <= item && item < incl)
+            for (uint32_t b = b0; b < b1; ++b) {
+                const uint32_t n = tiles_of(b);
+                if (item < before + n) {
+                    s_item[0] = b;
+                    s_item[1] = n - 1 - (item - before);        // the longest first: they see the most
+                    break;
+                }
+                before += n;
+            }
+    }
+    __syncthreads();
+    const uint32_t b = s_item[0];
+    if (b >= p.B) return;
+    const Seq s = load_seq(p, b);
+    PromptSpan sp;
+    {
+        sp.all_lo = p.cap;
+        sp.all_hi = 0;
+#pragma unroll
+        for (uint32_t t = 0; t < NT; ++t) {
+            const int32_t i0 = (int32_t)((s_item[1] * NT + t) * a.tt), n = min(max(s.q_len - i0, 0), (int32_t)a.tt);
+            sp.p0[t] = s.kv_len - s.q_len + i0;
+            sp.p1[t] = sp.p0[t] + n - 1;
+            sp.hi[t] = n ? max(min(sp.p1[t] + 1, p.cap), 0) : 0;
+            sp.lo[t] = a.window ? min(max(sp.p0[t] - a.window + 1, 0), sp.hi[t]) : 0;
+            if (n) {
+                sp.all_lo = min(sp.all_lo, sp.lo[t]);
+                sp.all_hi = max(sp.all_hi, sp.hi[t]);
+            }
+        }
+        sp.all_lo = min(sp.all_lo, sp.all_hi);
+        sp.t_lo = sp.all_lo / (int32_t)kKt;
+        sp.n_sink = a.window ? min((min(a.sinks, sp.all_hi) + (int32_t)kKt - 1) / (int32_t)kKt, sp.t_lo) : 0;
+        sp.n = sp.n_sink + (sp.all_hi + (int32_t)kKt - 1) / (int32_t)kKt - sp.t_lo;
+    }
+    const int32_t q_row = s.q0 + (int32_t)(s_item[1] * NT * a.tt);              // first token of the block
+
+    if (threadIdx.x == 0) {
+        mbar_init(bar(Sh::bQ), 1);
+        for (uint32_t i = 0; i < NS; ++i) {
+            mbar_init(bar(Sh::bFull + i), BITS == 16 ? 1 : Sh::PW);
+            mbar_init(bar(Sh::bEmpty + i), 1);
+        }
+        for (uint32_t t = 0; t < NT; ++t) {
+            mbar_init(bar(Sh::bS + t), 1);
+            mbar_init(bar(Sh::bP + t), 4);
+        }
+        mbar_init(bar(Sh::bO), 1);
+        mbar_init(bar(Sh::bFix), 1);
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == Sh::kMma) tmem_alloc(smem_s + Sh::oBar + Sh::oTmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+    auto give_up = [&](uint32_t code) {
+        if (lane == 0) { atomicExch(&g_prompt_status, code); *s_abort = 1; }
+    };
+
+    if (warp < Sh::kMma) {
+        // =========================== softmax: one thread per query row ===============================================
+        const uint32_t t = warp >> 2, w = warp & 3, row = w * 32 + lane;
+        const uint32_t tok = row / a.group, head = row % a.group;
+        const int32_t pos = sp.p0[t] + (int32_t)tok, last = min(pos, p.cap - 1);
+        const uint32_t s_addr = tmem + ((w * 32u) << 16) + t * kKt, o_addr = tmem + ((w * 32u) << 16) + Sh::cO + t * D;
+        float m = -INFINITY, l = 0.f;
+        uint32_t done = 0;                                      // products so far
+        bool ok = true;
+        const uint32_t ids = kKt >> p.page_shift;               // pages of a tile
+        auto missing = [&](int32_t i) {                         // whether a page of tile i is not there (lanes ask for one each)
+            const int32_t at = sp.first(i) + (int32_t)(lane << p.page_shift);
+            return lane < ids && at < sp.all_hi && page_of(p, b, at) < 0;
+        };
+        bool miss = sp.n > 0 && missing(0);
+        for (int32_t i = 0; i < sp.n && ok; ++i) {
+            const uint32_t gone = __ballot_sync(kFull, miss);   // one bit per page
+            if (i + 1 < sp.n) miss = missing(i + 1);
+            if (!sp.active(t, i)) continue;
+            const int32_t f = sp.first(i);
+            if (!mbar_wait(bar(Sh::bS + t), done & 1)) { give_up(11); ok = false; }
+            ok = __all_sync(kFull, ok) && !*s_abort;
+            if (!__all_sync(kFull, ok)) { ok = false; break; }
+            tc_fence_after();
+            const bool edge = gone || f + (int32_t)kKt - 1 > min(sp.p0[t], p.cap - 1) ||
+                              (a.window && f <= sp.p1[t] - a.window && f + (int32_t)kKt > a.sinks);
+            uint32_t x[BITS == 16 ? 4 : 1][32];
+            auto hide = [&](uint32_t (&v)[32], int32_t c) {     // scores of positions that the row does not see
+                if (!edge) return;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    const int32_t at = f + c * 32 + j;
+                    const bool seen = at <= last && (!a.window || at > pos - a.window || at < a.sinks) &&
+                                      !(gone >> ((uint32_t)(c * 32 + j) >> p.page_shift) & 1);
+                    if (!seen) v[j] = 0xFF800000u;
+                }
+            };
+            float mx = -INFINITY;
+            if constexpr (BITS == 16) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32_start(s_addr + c * 32, x[c]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tmem_ld_wait(x[c]);
+                    hide(x[c], c);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(x[c][j]));
+                }
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    tmem_ld32(s_addr + c * 32, x[0]);
+                    hide(x[0], c);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(x[0][j]));
+                }
+            }
+            mx *= a.scale_log2;
+            if (!(mx == mx)) mx = -INFINITY;                    // 0 times infinity: nothing to refer to
+            const bool grow = mx > m + kLazy;
+            if (__any_sync(kFull, grow)) {
+                const float c = grow ? ex2f(m - mx) : 1.f;
+                if (grow) m = mx;
+                l *= c;
+                if (done) {
+#pragma unroll 1
+                    for (uint32_t j = 0; j < D / 32; ++j) {
+                        uint32_t o[32];
+                        tmem_ld32(o_addr + j * 32, o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * c);
+                        tmem_st32(o_addr + j * 32, o);
+                    }
+                }
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t(&v)[32] = x[BITS == 16 ? c : 0];
+                if constexpr (BITS == 4) {
+                    tmem_ld32(s_addr + c * 32, v);
+                    hide(v, c);
+                }
+                uint32_t pk[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float e0 = ex2f(__uint_as_float(v[2 * j]) * a.scale_log2 - ref);
+                    const float e1 = ex2f(__uint_as_float(v[2 * j + 1]) * a.scale_log2 - ref);
+                    l += e0 + e1;
+                    pk[j] = pack_bf16(e0, e1);
+                }
+                tmem_st16(s_addr + c * 16, pk);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(Sh::bP + t));
+            ++done;
+        }
+        // ---- the row's result ----------------------------------------------------------------------------------
+        if (ok && !mbar_wait(bar(Sh::bO), 0)) { give_up(12); ok = false; }
+        ok = __all_sync(kFull, ok) && !*s_abort;
+        if (__all_sync(kFull, ok)) {
+            tc_fence_after();
+            const bool live = tok < a.tt && sp.p0[t] + (int32_t)tok <= sp.p1[t];
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            uint16_t *dst = a.out + (int64_t)(q_row + (int32_t)(t * a.tt + tok)) * a.ldo + (size_t)(kvh * a.group + head) * D;
+#pragma unroll 1
+            for (uint32_t j = 0; j < D / 32; ++j) {
+                uint32_t o[32];
+                if (done) {
+                    tmem_ld32(o_addr + j * 32, o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                }
+                if (live) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t y[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            y[q] = pack_bf16(__uint_as_float(o[8 * e + 2 * q]) * inv, __uint_as_float(o[8 * e + 2 * q + 1]) * inv);
+                        *reinterpret_cast<uint4 *>(dst + j * 32 + e * 8) = make_uint4(y[0], y[1], y[2], y[3]);
+                    }
+                }
+            }
+        }
+    } else if (warp == Sh::kMma) {
+        // =========================== products ======================================================================
+        constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((kKt >> 3) << 17) | ((128u >> 4) << 24);
+        constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
+        const uint32_t idesc_s = kIdescS | (a.negate ? 1u << 13 : 0u);
+        uint32_t asked[2] = {0, 0};                             // score tiles issued
+        uint32_t made[2] = {0, 0};                              // products with V issued
+        auto ring = [&](uint32_t c) { return smem_s + Sh::oRing + (c % NS) * Sh::kTile; };
+        auto full = [&](uint32_t c) { return mbar_wait_warp(bar(Sh::bFull + c % NS), (c / NS) & 1); };
+        auto scores = [&](uint32_t t, int32_t i) {
+            tc_fence_after();
+            if (lane == 0) {
+#pragma unroll
+                for (uint32_t kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t o = (kk / 4) * Sh::kBlock + (kk % 4) * 32;
+                    umma_bf16(tmem + t * kKt, umma_desc_sw128(smem_s + Sh::oQ + t * Sh::kTile + o), umma_desc_sw128(ring(2 * i) + o), idesc_s, kk != 0);
+                }
+                umma_commit(bar(Sh::bS + t));
+            }
+            __syncwarp();
+            ++asked[t];
+        };
+        bool ok = sp.n == 0 || mbar_wait_warp(bar(Sh::bQ), 0);
+        if (ok && sp.n > 0) ok = full(0);
+        if (ok && sp.n > 0) {
+            for (uint32_t t = 0; t < NT; ++t)
+                if (sp.active(t, 0)) scores(t, 0);
+            if (lane == 0) umma_commit(bar(Sh::bEmpty + 0));
+            __syncwarp();
+        }
+        for (int32_t i = 0; i < sp.n && ok; ++i) {
+            for (uint32_t t = 0; t < NT && ok; ++t) {
+                if (sp.active(t, i)) {
+                    ok = full(2 * i + 1) && mbar_wait_warp(bar(Sh::bP + t), made[t] & 1) && !*s_abort;
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+#pragma unroll
+                        for (uint32_t kk = 0; kk < kKt / 16; ++kk)
+                            umma_bf16_ts(tmem + Sh::cO + t * D, tmem + t * kKt + kk * 8, umma_desc_sw128_mn(ring(2 * i + 1) + kk * 2048, Sh::kBlock),
+                                         kIdescO, made[t] != 0 || kk != 0);
+                    }
+                    __syncwarp();
+                    ++made[t];
+                }
+                if (i + 1 < sp.n && sp.active(t, i + 1)) {
+                    ok = full(2 * i + 2);
+                    if (!ok) break;
+                    scores(t, i + 1);
+                }
+            }
+            if (ok && lane == 0) {
+                umma_commit(bar(Sh::bEmpty + (2 * i + 1) % NS));
+                if (i + 1 < sp.n) umma_commit(bar(Sh::bEmpty + (2 * i + 2) % NS));
+            }
+            __syncwarp();
+        }
+        if (!ok) give_up(13);
+        if (lane == 0) umma_commit(bar(Sh::bO));
+        __syncwarp();
+        if (!mbar_wait_warp(bar(Sh::bO), 0)) give_up(14);       // tensor memory is given back behind the last product
+    } else if constexpr (BITS == 16) {
+        // =========================== TMA copies ====================================================================
+        const uint32_t ids = kKt >> p.page_shift;
+        if (lane == 0 && sp.n > 0) {
+            const uint32_t bytes = a.tt * a.group * 128;        // of a block of 64 channels
+            mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
+            for (uint32_t t = 0; t < NT; ++t)
+                for (uint32_t c = 0; c < NB; ++c)
+                    tma_load_3d(smem_s + Sh::oQ + t * Sh::kTile + c * Sh::kBlock, &q_map, (int32_t)(c * 64), (int32_t)(kvh * a.group),
+                                q_row + (int32_t)(t * a.tt), bar(Sh::bQ));
+        }
+        uint32_t issued = 0, fixes = 0;
+        bool ok = true;
+        auto row_of = [&](int32_t i) {                          // this lane's page of tile i, as a row of the pool
+            const int32_t at = sp.first(i) + (int32_t)(lane << p.page_shift);
+            const int32_t id = lane < ids && at < sp.all_hi ? page_of(p, b, at) : -1;
+            return id < 0 ? -(int32_t)kKt : (int32_t)row_index(p, id, kvh, at);
+        };
+        int32_t next = sp.n > 0 ? row_of(0) : 0;
+        for (int32_t i = 0; i < sp.n && ok; ++i) {
+            const int32_t r = next, f = sp.first(i);
+            if (i + 1 < sp.n) next = row_of(i + 1);
+            // rows of V that no query of the block sees become zeros: 0 times what lies there need not be 0
+            const bool fix = f + (int32_t)kKt > sp.all_hi || (a.window && f <= sp.all_lo - 1 && f + (int32_t)kKt > a.sinks);
+            for (uint32_t kv = 0; kv < 2; ++kv, ++issued) {
+                const uint32_t slot = issued % NS;
+                if (!mbar_wait_warp(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1) || *s_abort) { give_up(15); ok = false; break; }
+                const bool mend = kv == 1 && fix;
+                const uint32_t to = mend ? bar(Sh::bFix) : bar(Sh::bFull + slot), dst = smem_s + Sh::oRing + slot * Sh::kTile;
+                if (lane == 0) mbar_expect_tx(to, Sh::kTile);
+                __syncwarp();
+                if (lane < ids)
+#pragma unroll
+                    for (uint32_t c = 0; c < NB; ++c)
+                        tma_load_2d(dst + c * Sh::kBlock + (lane << p.page_shift) * 128, kv ? &v_map : &k_map, (int32_t)(c * 64), r, to);
+                __syncwarp();
+                if (mend) {
+                    if (!mbar_wait_warp(bar(Sh::bFix), fixes & 1)) { give_up(16); ok = false; break; }
+                    ++fixes;
+                    for (uint32_t y = 0; y < kKt; ++y) {
+                        const int32_t at = f + (int32_t)y;
+                        if (at < sp.all_hi && !(a.window && at < sp.all_lo && at >= a.sinks)) continue;
+                        for (uint32_t c = lane; c < NB * 8; c += 32)
+                            sts_v4(dst + (c / 8) * Sh::kBlock + y * 128 + (c % 8) * 16, 0, 0, 0, 0);
+                    }
+                    fence_async_proxy();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(Sh::bFull + slot));
+                }
+            }
+        }
+        if (!ok)                                                // copies under way end before the block does
+            for (uint32_t c = issued > NS ? issued - NS : 0; c < issued; ++c) (void)mbar_wait_warp(bar(Sh::bFull + c % NS), (c / NS) & 1);
+        if (!ok && sp.n > 0) (void)mbar_wait_warp(bar(Sh::bQ), 0);
+    } else {
+        // =========================== codes to bf16: one thread per position ==========================================
+        constexpr uint32_t G = D / 64;
+        const uint32_t y = threadIdx.x - Sh::kProd * 32;        // position inside the tile
+        if (y == 0 && sp.n > 0) {
+            const uint32_t bytes = a.tt * a.group * 128;
+            mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
+            for (uint32_t t = 0; t < NT; ++t)
+                for (uint32_t c = 0; c < NB; ++c)
+                    tma_load_3d(smem_s + Sh::oQ + t * Sh::kTile + c * Sh::kBlock, &q_map, (int32_t)(c * 64), (int32_t)(kvh * a.group),
+                                q_row + (int32_t)(t * a.tt), bar(Sh::bQ));
+        }
+        uint32_t issued = 0;
+        bool ok = true;
+        for (int32_t i = 0; i < sp.n && ok; ++i) {
+            const int32_t at = sp.first(i) + (int32_t)y;
+            const bool wanted = at < sp.all_hi && !(a.window && at < sp.all_lo && at >= a.sinks);
+            const int32_t id = wanted ? page_of(p, b, at) : -1;
+            const size_t r = id < 0 ? 0 : row_index(p, id, kvh, at);
+            for (uint32_t kv = 0; kv < 2; ++kv, ++issued) {
+                uint4 code[D / 32];
+                uint32_t sc[G];
+                if (id >= 0) {
+                    const uint4 *src = reinterpret_cast<const uint4 *>((kv ? a.v : a.k) + r * (D / 2));
+#pragma unroll
+                    for (uint32_t c = 0; c < D / 32; ++c) code[c] = __ldg(src + c);
+#pragma unroll
+                    for (uint32_t g = 0; g < G; ++g) sc[g] = __ldg((kv ? a.vs : a.ks) + r * G + g);
+                }
+                const uint32_t slot = issued % NS, dst = smem_s + Sh::oRing + slot * Sh::kTile;
+                if (!mbar_wait_warp(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1) || *s_abort) { give_up(17); ok = false; break; }
+                const uint32_t *words = &code[0].x;
+#pragma unroll
+                for (uint32_t q = 0; q < D / 8; ++q) {          // word q: eight channels of group q % G
+                    const uint32_t g = q % G, c8 = q / G;
+                    uint32_t o[4] = {0, 0, 0, 0};
+                    if (id >= 0) {
+                        const float step = lo_bf16(sc[g]), low = hi_bf16(sc[g]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t w = words[q] >> 4 * j;
+                            o[j] = pack_bf16(step * (float)(w & 15u) + low, step * (float)(w >> 16 & 15u) + low);
+                        }
+                    }
+                    sts_v4(dst + g * Sh::kBlock + y * 128 + ((c8 ^ (y & 7)) << 4), o[0], o[1], o[2], o[3]);
+                }
+                fence_async_proxy();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(Sh::bFull + slot));
+            }
+        }
+        if (!ok && sp.n > 0) (void)mbar_wait_warp(bar(Sh::bQ), 0);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == Sh::kMma) tmem_dealloc(tmem, 512);
+}
+
+template <int D, int BITS>
+static int launch_prompt(const PromptArgs &a, const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t s) {
+    using Sh = PromptShape<D, BITS>;
+    static SmemLimit lim = {};
+    if (int rc = ensure_smem_limit(lim, (const void *)k_paged_prompt<D, BITS>, Sh::kSmem)) return rc;
+    const uint64_t items = (uint64_t)a.p.T / (Sh::NT * a.tt) + a.p.B, blocks = items * a.p.n_kv;
+    CI_REQUIRE(blocks <= 0x7FFFFFFFu, "too many blocks");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(Sh::kThreads);
+    cfg.dynamicSmemBytes = Sh::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    CI_CUDA(cudaLaunchKernelEx(&cfg, k_paged_prompt<D, BITS>, a, qm, km, vm));
+    return CI_OK;
+}
+
+static int pool_map(CUtensorMap *m, const ci_paged_cache *c, void *base) {
+    const cuuint64_t dims[2] = {c->head_dim, (cuuint64_t)c->num_pages * c->n_kv * c->page_size};
+    const cuuint64_t strides[1] = {(cuuint64_t)c->head_dim * 2};
+    const cuuint32_t box[2] = {64, c->page_size}, one[2] = {1, 1};
+    const CUresult r = encode_tiled_fn()(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed with code %d", (int)r);
+        return CI_E_CUDA;
+    }
+    return CI_OK;
+}
+
+// Sequences with more than min_rows query rows per key/value head.  Needs group <= 128.
+int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const uint16_t *q, int64_t ldq, uint32_t n_q, int32_t window,
+                        int32_t sinks, float scale_log2, uint32_t min_rows, uint16_t *out, int64_t ldo, cudaStream_t s) {
+    CI_REQUIRE(encode_tiled_fn() != nullptr, "the driver has no cuTensorMapEncodeTiled");
+    CI_REQUIRE(c->bits == 4 || (uint64_t)c->num_pages * c->n_kv * c->page_size <= 0x7FFFFFFFu, "a pool of more than 2^31 rows");
+    PromptArgs a;
+    a.p = p;
+    a.k = (const uint8_t *)c->k; a.v = (const uint8_t *)c->v; a.ks = c->k_scale; a.vs = c->v_scale;
+    a.n_q = n_q;
+    a.group = n_q / c->n_kv;
+    a.tt = 128 / a.group;
+    a.min_rows = min_rows;
+    a.negate = scale_log2 < 0.f;
+    a.window = window; a.sinks = sinks;
+    a.scale_log2 = fmaxf(fabsf(scale_log2), 1e-30f);            // not 0: hidden scores are -inf before they are scaled
+    a.out = out; a.ldo = ldo;
+    CUtensorMap qm, km, vm;
+    memset(&km, 0, sizeof km);
+    memset(&vm, 0, sizeof vm);
+    const cuuint64_t dims[3] = {c->head_dim, n_q, p.T};
+    const cuuint64_t strides[2] = {(cuuint64_t)c->head_dim * 2, (cuuint64_t)ldq * 2};
+    const cuuint32_t box[3] = {64, a.group, a.tt}, one[3] = {1, 1, 1};
+    const CUresult r = encode_tiled_fn()(&qm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t *>(q), dims, strides, box, one,
+                                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed with code %d", (int)r);
+        return CI_E_CUDA;
+    }
+    if (c->bits == 16) {
+        if (int rc = pool_map(&km, c, c->k)) return rc;
+        if (int rc = pool_map(&vm, c, c->v)) return rc;
+        return c->head_dim == 64 ? launch_prompt<64, 16>(a, qm, km, vm, s) : c->head_dim == 128 ? launch_prompt<128, 16>(a, qm, km, vm, s)
+                                                                                             : launch_prompt<256, 16>(a, qm, km, vm, s);
+    }
+    return c->head_dim == 64 ? launch_prompt<64, 4>(a, qm, km, vm, s) : c->head_dim == 128 ? launch_prompt<128, 4>(a, qm, km, vm, s)
+                                                                                         : launch_prompt<256, 4>(a, qm, km, vm, s);
+}
+
+}  // namespace ci
+
+using namespace ci;
+
+extern "C" int ci_paged_status(uint32_t *code, int clear, ci_stream_t stream) {
+    void *word = nullptr;
+    CI_CUDA(cudaGetSymbolAddress(&word, g_prompt_status));
+    return ci_status((uint32_t *)word, code, clear, stream);
+}

@@ -446,6 +446,9 @@ size_t ci_paged_attention_workspace_bytes(uint32_t head_dim);
 int ci_paged_attention(const ci_paged_cache *cache, const ci_paged_batch *batch, const uint16_t *d_q, int64_t ldq, uint32_t n_q,
                        uint32_t max_q_len, uint32_t window, uint32_t sinks, float scale, void *d_workspace,
                        size_t workspace_bytes, uint16_t *d_out, int64_t ldo, ci_stream_t stream);
+/* ci_status for the waits inside ci_paged_attention on the current device: a wait that runs out ends the call with wrong
+ * outputs and leaves its code here.  Waits for `stream`; the first call on a device outside any stream capture. */
+int ci_paged_status(uint32_t *code, int clear, ci_stream_t stream);
 
 /* Logits [B, V] (bf16, rows ld_in / ld_out apart; d_out may be d_in) as a sampler adjusts them, in fp32 with one rounding:
  *   x / r (x > 0) or x * r, r = d_repetition[b], for tokens of the history d_tokens[b][0 .. d_lens[b]);

@@ -73,12 +73,13 @@ def sequence(cache, table, b, n):
     return out[0], out[1], there
 
 
-def attention(q, cache, table, kv_lens, q_starts=None, window=0, sinks=0, scale=None):
+def attention(q, cache, table, kv_lens, q_starts=None, window=0, sinks=0, scale=None, few=64):
     """(result, bound) float64 [T, n_q, d]: the result, and how far one that rounds each weight (4 bits: times its step) and
-    the result to bf16 may be from it.  Half a step of bf16 is 2^-8 relative: 2^-8 (sum of p |v| + |o|), |v - lowest| in the
-    place of |v| for 4 bits, where the lowest values are not rounded with the weights; a sixty-fourth more for
-    products of roundings; and for sums in float32 2^-18 of the sum of p times the largest thing added up, |v| or (4 bits)
-    step * 143 and |lowest|."""
+    the result to bf16 may be from it.  Half a step of bf16 is 2^-8 relative: 2^-8 (sum of p |v| + |o|); for 4 bits
+    |v - middle| in the place of |v|, the middle of a group being code 8, where the few new tokens' kernel rounds the weights'
+    products with steps alone, and 2 |v| and the change of p by keys that are rounded too, 2^-8 scale sum |q k|, where the
+    prompts' kernel makes bf16 of codes (`prompt`); a sixty-fourth more for products of roundings; and for sums in float32
+    2^-18 of the sum of p times the largest thing added up, |v| or (4 bits) step * 143 and |lowest|."""
     T, n_q, d = q.shape
     scale = d ** -0.5 if scale is None else scale
     out = torch.zeros(T, n_q, d, dtype=torch.float64, device=q.device)
@@ -116,7 +117,10 @@ def attention(q, cache, table, kv_lens, q_starts=None, window=0, sinks=0, scale=
             if cache.bits == 16:
                 a, big = p @ v[:, g].abs(), p @ v[:, g].abs()
             else:
-                a, big = p @ (v[:, g] - lowv[:, g]).abs(), p @ (143 * stepv[:, g] + lowv[:, g].abs())
+                a, big = p @ (v[:, g] - lowv[:, g] - 8 * stepv[:, g]).abs(), p @ (143 * stepv[:, g] + lowv[:, g].abs())
+                if q_starts is not None and (int(q_starts[b + 1]) - int(q_starts[b])) * (n_q // cache.n_kv) > few:
+                    ds = scale * (k[:, g].abs() @ q[t, h].double().abs())       # p_j changes by at most (e^(2 max ds) - 1) p_j
+                    a = 2 * (p @ v[:, g].abs()) + (p * 2 * ds.max()) @ (v[:, g] - out[t, h]).abs()
             bound[t, h] = 2.0 ** -8 * (a + out[t, h].abs()) * (1 + 2.0 ** -6) + 2.0 ** -18 * big
     return out, bound
 
