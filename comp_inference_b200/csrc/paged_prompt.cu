@@ -6,13 +6,15 @@
 //   S = Q . K^T        Q and K in shared memory (128-byte swizzle), S fp32 in tensor memory
 //   P = exp2(S scale - m), written back in bf16 over S by the row's own thread: no exchange between threads at all
 //   O += P . V         P from tensor memory, V as it lies (its rows are the k index: an MN-major operand), O in tensor memory
-// While one tile's threads are at their exponentials the tensor cores work for the other.  The maximum that a row's weights
-// refer to moves only when it is exceeded by 2^8 (kLazy), so O is rarely rescaled; the row's own thread does that too,
-// between two products, when nothing else touches it.  Tiles that no row sees are not visited; a page that does not exist
+// While one tile's threads are at their exponentials the tensor cores work for the other; the weights are handed over in two
+// halves.  The maximum that a row's weights refer to moves only when it is exceeded by 2^8 (kLazy), so O is rarely rescaled; the
+// row's own thread does that too, between two products, when nothing else touches it.  Tiles that no row sees are not visited; a page that does not exist
 // is fetched from outside the tensor, which gives zeros.
 //
-// One warp issues the products, one the TMA copies (for 4 bits, four warps turn codes into bf16); mbarriers connect them.  All
-// waits are bounded: on expiry a role sets the status word and the abort flag, and everyone leaves.
+// One warp per query tile issues the products, one the TMA copies (for 4 bits, four warps turn codes into bf16); mbarriers
+// connect them.  All waits are bounded: on expiry a role sets the status word and the abort flag, and everyone leaves.
+#include <type_traits>
+
 #include "paged.cuh"
 #include "umma.cuh"
 
@@ -39,11 +41,15 @@ struct PromptShape {
     static constexpr uint32_t kTile = kKt * D * 2, kBlock = kKt * 128;       // bytes: a tile of 128 rows, its 64-channel block
     static constexpr uint32_t NS = D == 64 ? 6 : D == 128 ? 4 : 2;           // ring of K and V tiles
     static constexpr uint32_t PW = BITS == 16 ? 1 : 4;                       // producer warps
-    static constexpr uint32_t kMma = 4 * NT, kProd = kMma + 1, kThreads = (kProd + PW) * 32;
+    static constexpr uint32_t kProd = 4 * NT, kMma = kProd + PW;
+    // Two query tiles: whole warpgroups, so that registers can go where the scores are held.
+    static constexpr uint32_t kWarps = NT == 2 ? (kMma + NT + 3) / 4 * 4 : kMma + NT, kThreads = kWarps * 32;
+    static constexpr uint32_t kSoftRegs = BITS == 16 ? 200 : 184, kProdRegs = 104, kMmaRegs = BITS == 16 ? kProdRegs : 40;
+    static_assert(NT == 1 || 256 * kSoftRegs + 128 * kProdRegs + (BITS == 16 ? 0 : 128 * kMmaRegs) <= kThreads * (65536 / kThreads / 8 * 8), "registers");
     static constexpr uint32_t oQ = 0, oRing = NT * kTile, oBar = oRing + NS * kTile, kSmem = oBar + 256 + 1024;
     // barriers
-    static constexpr uint32_t bQ = 0, bFull = 1, bEmpty = bFull + NS, bS = bEmpty + NS, bP = bS + NT, bO = bP + NT, bFix = bO + 1;
-    static constexpr uint32_t oTmem = (bFix + 1) * 8, oAbort = oTmem + 4, oItem = oTmem + 8;
+    static constexpr uint32_t bQ = 0, bFull = 1, bEmpty = bFull + NS, bS = bEmpty + NS, bP = bS + NT, bO = bP + 2 * NT, bFix = bO + 1, bTurn = bFix + 1;
+    static constexpr uint32_t oTmem = (bTurn + 2) * 8, oAbort = oTmem + 4, oItem = oTmem + 8;
     static_assert(oItem + 16 <= 256, "barrier region");
     static constexpr uint32_t cO = NT * kKt;                                 // first column of O
 };
@@ -54,16 +60,64 @@ __device__ __forceinline__ float ex2f(float x) {
     return y;
 }
 
-// Positions that the query tiles of a block see, and the key tiles to visit.
-struct PromptSpan {
-    int32_t p0[2], p1[2], lo[2], hi[2];      // of each query tile: first and last position, visible range; p1 < p0: no tokens
-    int32_t all_lo, all_hi, t_lo, n_sink, n;
+// A query tile: positions of its first and last token (p1 < p0: it has none) and the range that they see.
+struct QueryTile {
+    int32_t p0, p1, lo, hi;
+};
+// The key tiles that a block visits: tile i of n starts at first(i).
+struct KeyTiles {
+    int32_t lo, hi, t_lo, n_sink, n;
     __device__ __forceinline__ int32_t first(int32_t i) const { return (i < n_sink ? i : t_lo + i - n_sink) * (int32_t)kKt; }
-    __device__ __forceinline__ bool active(uint32_t t, int32_t i) const {
+    __device__ __forceinline__ bool seen_by(const QueryTile &q, int32_t i) const {
         const int32_t f = first(i);
-        return p1[t] >= p0[t] && f < hi[t] && (i < n_sink || f + (int32_t)kKt > lo[t]);
+        return q.p1 >= q.p0 && f < q.hi && (i < n_sink || f + (int32_t)kKt > q.lo);
     }
 };
+
+// The same in every lane: said to the compiler, which then forms what depends on it in uniform registers.
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __shfl_sync(kFull, v, 0); }
+
+// Bits 0 .. n - 1, for any n.
+__device__ __forceinline__ uint32_t low_bits(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
+
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void split(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// 2^x of two values, x <= 2^6, in the fused multiply-add units: the integer next to x goes into the exponent field, 2^f for the rest
+// in [-1/2, 1/2] is a polynomial of degree 3 fitted for the smallest largest relative error, 7.5e-5, a fiftieth of what rounding to
+// bf16 loses.  The special-function unit makes four results per cycle and scheduler; a quarter of the weights comes from here
+// (4096 tokens, 32 heads of 128 over 8: 160.6 us; none of them 167.6, half 181.8).  For x of
+// -126 and less it gives 2^-126, not 0: not for tiles with hidden scores.
+constexpr float kExp0 = 0.99992812f, kExp1 = 0.69326097f, kExp2 = 0.24261075f, kExp3 = 0.05517141f;
+__device__ __forceinline__ void ex2_poly(uint64_t x, float &r0, float &r1) {
+    float x0, x1;
+    split(x, x0, x1);
+    x = pair(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+    const uint64_t magic = pair(12582912.f, 12582912.f), t = add2(x, magic);
+    const uint64_t f = add2(x, fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), 0));
+    uint64_t y = fma2(f, pair(kExp3, kExp3), pair(kExp2, kExp2));
+    y = fma2(f, y, pair(kExp1, kExp1));
+    y = fma2(f, y, pair(kExp0, kExp0));
+    float y0, y1, t0, t1;
+    split(y, y0, y1);
+    split(t, t0, t1);
+    r0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
+    r1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
+}
 
 template <int D, int BITS>
 __global__ void __launch_bounds__(PromptShape<D, BITS>::kThreads, 1)
@@ -74,7 +128,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_s = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem = smem_raw + (smem_s - smem_u32(smem_raw));
-    const uint32_t warp = threadIdx.x >> 5, lane = lane_id();
+    const uint32_t warp = uniform(threadIdx.x >> 5), lane = lane_id();
     const PagedBatch &p = a.p;
     auto bar = [&](uint32_t i) { return smem_s + Sh::oBar + i * 8; };
     volatile uint32_t *s_tmem = reinterpret_cast<volatile uint32_t *>(smem + Sh::oBar + Sh::oTmem);
@@ -117,41 +171,50 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     const uint32_t b = s_item[0];
     if (b >= p.B) return;
     const Seq s = load_seq(p, b);
-    PromptSpan sp;
-    {
-        sp.all_lo = p.cap;
-        sp.all_hi = 0;
+    QueryTile qt[NT];
+    KeyTiles kt;
+    kt.lo = p.cap;
+    kt.hi = 0;
 #pragma unroll
-        for (uint32_t t = 0; t < NT; ++t) {
-            const int32_t i0 = (int32_t)((s_item[1] * NT + t) * a.tt), n = min(max(s.q_len - i0, 0), (int32_t)a.tt);
-            sp.p0[t] = s.kv_len - s.q_len + i0;
-            sp.p1[t] = sp.p0[t] + n - 1;
-            sp.hi[t] = n ? max(min(sp.p1[t] + 1, p.cap), 0) : 0;
-            sp.lo[t] = a.window ? min(max(sp.p0[t] - a.window + 1, 0), sp.hi[t]) : 0;
-            if (n) {
-                sp.all_lo = min(sp.all_lo, sp.lo[t]);
-                sp.all_hi = max(sp.all_hi, sp.hi[t]);
-            }
+    for (uint32_t t = 0; t < NT; ++t) {
+        const int32_t i0 = (int32_t)((s_item[1] * NT + t) * a.tt), n = min(max(s.q_len - i0, 0), (int32_t)a.tt);
+        qt[t].p0 = s.kv_len - s.q_len + i0;
+        qt[t].p1 = qt[t].p0 + n - 1;
+        qt[t].hi = n ? max(min(qt[t].p1 + 1, p.cap), 0) : 0;
+        qt[t].lo = a.window ? min(max(qt[t].p0 - a.window + 1, 0), qt[t].hi) : 0;
+        if (n) {
+            kt.lo = min(kt.lo, qt[t].lo);
+            kt.hi = max(kt.hi, qt[t].hi);
         }
-        sp.all_lo = min(sp.all_lo, sp.all_hi);
-        sp.t_lo = sp.all_lo / (int32_t)kKt;
-        sp.n_sink = a.window ? min((min(a.sinks, sp.all_hi) + (int32_t)kKt - 1) / (int32_t)kKt, sp.t_lo) : 0;
-        sp.n = sp.n_sink + (sp.all_hi + (int32_t)kKt - 1) / (int32_t)kKt - sp.t_lo;
     }
+    kt.lo = min(kt.lo, kt.hi);
+    kt.t_lo = kt.lo / (int32_t)kKt;
+    kt.n_sink = a.window ? min((min(a.sinks, kt.hi) + (int32_t)kKt - 1) / (int32_t)kKt, kt.t_lo) : 0;
+    kt.n = kt.n_sink + (kt.hi + (int32_t)kKt - 1) / (int32_t)kKt - kt.t_lo;
+    kt.lo = uniform(kt.lo);
+    kt.hi = uniform(kt.hi);
+    kt.t_lo = uniform(kt.t_lo);
+    kt.n_sink = uniform(kt.n_sink);
+    kt.n = uniform(kt.n);
+#pragma unroll
+    for (uint32_t t = 0; t < NT; ++t) qt[t] = {uniform(qt[t].p0), uniform(qt[t].p1), uniform(qt[t].lo), uniform(qt[t].hi)};
     const int32_t q_row = s.q0 + (int32_t)(s_item[1] * NT * a.tt);              // first token of the block
 
     if (threadIdx.x == 0) {
         mbar_init(bar(Sh::bQ), 1);
         for (uint32_t i = 0; i < NS; ++i) {
             mbar_init(bar(Sh::bFull + i), BITS == 16 ? 1 : Sh::PW);
-            mbar_init(bar(Sh::bEmpty + i), 1);
+            mbar_init(bar(Sh::bEmpty + i), NT);
         }
         for (uint32_t t = 0; t < NT; ++t) {
             mbar_init(bar(Sh::bS + t), 1);
-            mbar_init(bar(Sh::bP + t), 4);
+            mbar_init(bar(Sh::bP + 2 * t), 4);
+            mbar_init(bar(Sh::bP + 2 * t + 1), 4);
         }
-        mbar_init(bar(Sh::bO), 1);
+        mbar_init(bar(Sh::bO), NT);
         mbar_init(bar(Sh::bFix), 1);
+        mbar_init(bar(Sh::bTurn), 1);
+        mbar_init(bar(Sh::bTurn + 1), 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -159,75 +222,81 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *s_tmem;
+    const uint32_t tmem = uniform(*s_tmem);
     auto give_up = [&](uint32_t code) {
         if (lane == 0) { atomicExch(&g_prompt_status, code); *s_abort = 1; }
     };
 
-    if (warp < Sh::kMma) {
+    if (warp < 4 * NT) {
+        if (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::kSoftRegs));
         // =========================== softmax: one thread per query row ===============================================
         const uint32_t t = warp >> 2, w = warp & 3, row = w * 32 + lane;
         const uint32_t tok = row / a.group, head = row % a.group;
-        const int32_t pos = sp.p0[t] + (int32_t)tok, last = min(pos, p.cap - 1);
+        QueryTile q = qt[0];
+        if (NT == 2 && t == 1) q = qt[NT - 1];
+        const int32_t pos = q.p0 + (int32_t)tok, last = min(pos, p.cap - 1);
         const uint32_t s_addr = tmem + ((w * 32u) << 16) + t * kKt, o_addr = tmem + ((w * 32u) << 16) + Sh::cO + t * D;
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY;
+        uint64_t l2[4] = {0, 0, 0, 0};                          // sums of weights, eight at once
         uint32_t done = 0;                                      // products so far
         bool ok = true;
         const uint32_t ids = kKt >> p.page_shift;               // pages of a tile
-        auto missing = [&](int32_t i) {                         // whether a page of tile i is not there (lanes ask for one each)
-            const int32_t at = sp.first(i) + (int32_t)(lane << p.page_shift);
-            return lane < ids && at < sp.all_hi && page_of(p, b, at) < 0;
+        auto page_id = [&](int32_t i) {                         // of tile i, one per lane; 0 where there is none to ask for
+            const int32_t at = kt.first(i) + (int32_t)(lane << p.page_shift);
+            return i < kt.n && lane < ids && at < kt.hi ? __ldg(p.table + (size_t)b * p.table_stride + ((uint32_t)at >> p.page_shift)) : 0;
         };
-        bool miss = sp.n > 0 && missing(0);
-        for (int32_t i = 0; i < sp.n && ok; ++i) {
-            const uint32_t gone = __ballot_sync(kFull, miss);   // one bit per page
-            if (i + 1 < sp.n) miss = missing(i + 1);
-            if (!sp.active(t, i)) continue;
-            const int32_t f = sp.first(i);
-            if (!mbar_wait(bar(Sh::bS + t), done & 1)) { give_up(11); ok = false; }
-            ok = __all_sync(kFull, ok) && !*s_abort;
-            if (!__all_sync(kFull, ok)) { ok = false; break; }
-            tc_fence_after();
-            const bool edge = gone || f + (int32_t)kKt - 1 > min(sp.p0[t], p.cap - 1) ||
-                              (a.window && f <= sp.p1[t] - a.window && f + (int32_t)kKt > a.sinks);
-            uint32_t x[BITS == 16 ? 4 : 1][32];
-            auto hide = [&](uint32_t (&v)[32], int32_t c) {     // scores of positions that the row does not see
-                if (!edge) return;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const int32_t at = f + c * 32 + j;
-                    const bool seen = at <= last && (!a.window || at > pos - a.window || at < a.sinks) &&
-                                      !(gone >> ((uint32_t)(c * 32 + j) >> p.page_shift) & 1);
-                    if (!seen) v[j] = 0xFF800000u;
-                }
-            };
-            float mx = -INFINITY;
-            if constexpr (BITS == 16) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32_start(s_addr + c * 32, x[c]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tmem_ld_wait(x[c]);
-                    hide(x[c], c);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(x[c][j]));
-                }
-            } else {
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    tmem_ld32(s_addr + c * 32, x[0]);
-                    hide(x[0], c);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(x[0][j]));
-                }
+        int32_t id = page_id(0);
+        const uint64_t scale2 = pair(a.scale_log2, a.scale_log2);
+        for (int32_t i = 0; i < kt.n; ++i) {
+            const uint32_t gone = __ballot_sync(kFull, (uint32_t)id >= p.num_pages);    // one bit per page that does not exist
+            id = page_id(i + 1);
+            if (!kt.seen_by(q, i)) continue;
+            const int32_t f = kt.first(i);
+            const bool edge = gone || f + (int32_t)kKt - 1 > min(q.p0, p.cap - 1) ||
+                              (a.window && f <= q.p1 - a.window && f + (int32_t)kKt > a.sinks);
+            if (!__all_sync(kFull, mbar_wait(bar(Sh::bS + t), done & 1))) {
+                give_up(11);
+                ok = false;
+                break;
             }
-            mx *= a.scale_log2;
-            if (!(mx == mx)) mx = -INFINITY;                    // 0 times infinity: nothing to refer to
+            tc_fence_after();
+            uint32_t x[4][32];
+            auto hide = [&](uint32_t (&v)[32], int32_t c) {     // scores of positions that the row does not see
+                const int32_t f32 = f + c * 32;
+                uint32_t seen = low_bits(last + 1 - f32);
+                if (a.window) seen &= ~low_bits(pos - a.window + 1 - f32) | low_bits(a.sinks - f32);
+                if (gone)
+#pragma unroll
+                    for (int j = 0; j < 32; j += 16)
+                        if (gone >> ((uint32_t)(c * 32 + j) >> p.page_shift) & 1) seen &= ~(0xFFFFu << j);
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (!(seen & (1u << j))) v[j] = 0xFF800000u;
+            };
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto largest = [&](const uint32_t (&v)[32]) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        mx4[e] = fmaxf(fmaxf(mx4[e], __uint_as_float(v[j + e])), __uint_as_float(v[j + 4 + e]));
+            };
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32_start(s_addr + c * 32, x[c]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld_wait(x[c]);
+            if (edge)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) hide(x[c], c);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) largest(x[c]);
+            float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
             const bool grow = mx > m + kLazy;
             if (__any_sync(kFull, grow)) {
                 const float c = grow ? ex2f(m - mx) : 1.f;
                 if (grow) m = mx;
-                l *= c;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) l2[e] = fma2(l2[e], pair(c, c), 0);
                 if (done) {
 #pragma unroll 1
                     for (uint32_t j = 0; j < D / 32; ++j) {
@@ -239,37 +308,54 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     }
                 }
             }
-            const float ref = m == -INFINITY ? 0.f : m;
+            const float ref = m == -INFINITY ? 0.f : -m;
+            const uint64_t ref2 = pair(ref, ref);
+            auto weights = [&](auto whole) {                    // whole: no score of the tile is hidden
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t(&v)[32] = x[BITS == 16 ? c : 0];
-                if constexpr (BITS == 4) {
-                    tmem_ld32(s_addr + c * 32, v);
-                    hide(v, c);
-                }
-                uint32_t pk[16];
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t(&v)[32] = x[c];
+                    uint32_t pk[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float e0 = ex2f(__uint_as_float(v[2 * j]) * a.scale_log2 - ref);
-                    const float e1 = ex2f(__uint_as_float(v[2 * j + 1]) * a.scale_log2 - ref);
-                    l += e0 + e1;
-                    pk[j] = pack_bf16(e0, e1);
+                    for (int j = 0; j < 16; ++j) {
+                        const uint64_t y = fma2(pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), scale2, ref2);
+                        float e0, e1;
+                        if (decltype(whole)::value && j % 4 == 3) {
+                            ex2_poly(y, e0, e1);
+                        } else {
+                            split(y, e0, e1);
+                            e0 = ex2f(e0);
+                            e1 = ex2f(e1);
+                        }
+                        l2[j % 4] = add2(l2[j % 4], pair(e0, e1));
+                        pk[j] = pack_bf16(e0, e1);
+                    }
+                    tmem_st16(s_addr + c * 16, pk);
+                    if (c % 2) {                                    // half of the weights are there
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar(Sh::bP + 2 * t + c / 2));
+                    }
                 }
-                tmem_st16(s_addr + c * 16, pk);
-            }
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(Sh::bP + t));
+            };
+            if (edge) weights(std::false_type());
+            else weights(std::true_type());
             ++done;
+        }
+        float l = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float l0, l1;
+            split(l2[e], l0, l1);
+            l += l0 + l1;
         }
         // ---- the row's result ----------------------------------------------------------------------------------
         if (ok && !mbar_wait(bar(Sh::bO), 0)) { give_up(12); ok = false; }
         ok = __all_sync(kFull, ok) && !*s_abort;
         if (__all_sync(kFull, ok)) {
             tc_fence_after();
-            const bool live = tok < a.tt && sp.p0[t] + (int32_t)tok <= sp.p1[t];
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const bool live = tok < a.tt && pos <= q.p1;
+            const float inv = m == -INFINITY ? 0.f : 1.f / l;            // (nothing seen: zeros)
             uint16_t *dst = a.out + (int64_t)(q_row + (int32_t)(t * a.tt + tok)) * a.ldo + (size_t)(kvh * a.group + head) * D;
 #pragma unroll 1
             for (uint32_t j = 0; j < D / 32; ++j) {
@@ -285,78 +371,99 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     for (int e = 0; e < 4; ++e) {
                         uint32_t y[4];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            y[q] = pack_bf16(__uint_as_float(o[8 * e + 2 * q]) * inv, __uint_as_float(o[8 * e + 2 * q + 1]) * inv);
+                        for (int h = 0; h < 4; ++h)
+                            y[h] = pack_bf16(__uint_as_float(o[8 * e + 2 * h]) * inv, __uint_as_float(o[8 * e + 2 * h + 1]) * inv);
                         *reinterpret_cast<uint4 *>(dst + j * 32 + e * 8) = make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 }
             }
         }
-    } else if (warp == Sh::kMma) {
+    } else {
+        if (NT == 2) {                                          // by warpgroups: 4 bits have one of producers, one for the products
+            if (BITS == 4 && warp >= 12) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kMmaRegs));
+            else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kProdRegs));
+        }
+    if (warp >= Sh::kMma && warp < Sh::kMma + NT) {
         // =========================== products ======================================================================
         constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((kKt >> 3) << 17) | ((128u >> 4) << 24);
         constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
-        const uint32_t idesc_s = kIdescS | (a.negate ? 1u << 13 : 0u);
-        uint32_t asked[2] = {0, 0};                             // score tiles issued
-        uint32_t made[2] = {0, 0};                              // products with V issued
-        auto ring = [&](uint32_t c) { return smem_s + Sh::oRing + (c % NS) * Sh::kTile; };
-        auto full = [&](uint32_t c) { return mbar_wait_warp(bar(Sh::bFull + c % NS), (c / NS) & 1); };
-        auto scores = [&](uint32_t t, int32_t i) {
+        // One warp per query tile, in turns: while one tile's products run, the other's rows are at their exponentials.  Without
+        // turns both come to do the same at the same time (4250 cycles for a pair of query tiles and a key tile instead of 2800).
+        const uint32_t t = warp - Sh::kMma, idesc_s = kIdescS | (a.negate ? 1u << 13 : 0u);
+        QueryTile q = qt[0];
+        if (NT == 2 && t == 1) q = qt[NT - 1];
+        uint32_t made = 0;                                      // products with V issued
+        const uint64_t q_desc = umma_desc_sw128(smem_s + Sh::oQ + t * Sh::kTile), k_desc = umma_desc_sw128(smem_s + Sh::oRing);
+        const uint64_t v_desc = umma_desc_sw128_mn(smem_s + Sh::oRing, Sh::kBlock);
+        const uint32_t s_col = tmem + t * kKt, o_col = tmem + Sh::cO + t * D;
+        auto full = [&](uint32_t c) { return mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1); };
+        auto scores = [&](int32_t i) {
             tc_fence_after();
-            if (lane == 0) {
+            const uint64_t kd = k_desc + ((2 * i) % NS) * (Sh::kTile >> 4);
+            if (elect_one()) {
 #pragma unroll
                 for (uint32_t kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t o = (kk / 4) * Sh::kBlock + (kk % 4) * 32;
-                    umma_bf16(tmem + t * kKt, umma_desc_sw128(smem_s + Sh::oQ + t * Sh::kTile + o), umma_desc_sw128(ring(2 * i) + o), idesc_s, kk != 0);
+                    const uint32_t o = (kk / 4) * (Sh::kBlock >> 4) + (kk % 4) * (32 >> 4);
+                    umma_bf16(s_col, q_desc + o, kd + o, idesc_s, kk != 0);
                 }
                 umma_commit(bar(Sh::bS + t));
             }
             __syncwarp();
-            ++asked[t];
         };
-        bool ok = sp.n == 0 || mbar_wait_warp(bar(Sh::bQ), 0);
-        if (ok && sp.n > 0) ok = full(0);
-        if (ok && sp.n > 0) {
-            for (uint32_t t = 0; t < NT; ++t)
-                if (sp.active(t, 0)) scores(t, 0);
-            if (lane == 0) umma_commit(bar(Sh::bEmpty + 0));
+        auto release = [&](uint32_t c) {                        // the slot is free once this warp's products so far are done
+            if (elect_one()) umma_commit(bar(Sh::bEmpty + c % NS));
             __syncwarp();
+        };
+        bool ok = kt.n == 0 || __all_sync(kFull, mbar_wait(bar(Sh::bQ), 0) && full(0));
+        if (ok && kt.n > 0) {
+            if (kt.seen_by(q, 0)) scores(0);
+            release(0);
         }
-        for (int32_t i = 0; i < sp.n && ok; ++i) {
-            for (uint32_t t = 0; t < NT && ok; ++t) {
-                if (sp.active(t, i)) {
-                    ok = full(2 * i + 1) && mbar_wait_warp(bar(Sh::bP + t), made[t] & 1) && !*s_abort;
+        for (int32_t i = 0; i < kt.n && ok; ++i) {
+            if (NT == 2 && (t == 1 || i > 0)) {
+                ok = __all_sync(kFull, mbar_wait(bar(Sh::bTurn + t), (t == 1 ? i : i - 1) & 1));
+                if (!ok) break;
+            }
+            if (kt.seen_by(q, i)) {
+                const uint64_t vd = v_desc + ((2 * i + 1) % NS) * (Sh::kTile >> 4);
+                ok = __all_sync(kFull, full(2 * i + 1));
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {              // the weights come in two halves
+                    ok = ok && __all_sync(kFull, mbar_wait(bar(Sh::bP + 2 * t + h), made & 1));
                     if (!ok) break;
                     tc_fence_after();
-                    if (lane == 0) {
+                    if (elect_one()) {
 #pragma unroll
-                        for (uint32_t kk = 0; kk < kKt / 16; ++kk)
-                            umma_bf16_ts(tmem + Sh::cO + t * D, tmem + t * kKt + kk * 8, umma_desc_sw128_mn(ring(2 * i + 1) + kk * 2048, Sh::kBlock),
-                                         kIdescO, made[t] != 0 || kk != 0);
+                        for (uint32_t kk = h * (kKt / 32); kk < (h + 1) * (kKt / 32); ++kk)
+                            umma_ts(o_col, s_col + kk * 8, vd + kk * (2048 >> 4), kIdescO, made != 0 || kk != 0);
                     }
                     __syncwarp();
-                    ++made[t];
                 }
-                if (i + 1 < sp.n && sp.active(t, i + 1)) {
-                    ok = full(2 * i + 2);
+                if (!ok) break;
+                ++made;
+            }
+            release(2 * i + 1);
+            if (i + 1 < kt.n) {
+                if (kt.seen_by(q, i + 1)) {
+                    ok = __all_sync(kFull, full(2 * i + 2));
                     if (!ok) break;
-                    scores(t, i + 1);
+                    scores(i + 1);
                 }
+                release(2 * i + 2);
             }
-            if (ok && lane == 0) {
-                umma_commit(bar(Sh::bEmpty + (2 * i + 1) % NS));
-                if (i + 1 < sp.n) umma_commit(bar(Sh::bEmpty + (2 * i + 2) % NS));
-            }
+            if (NT == 2 && lane == 0) mbar_arrive(bar(Sh::bTurn + (t ^ 1)));
             __syncwarp();
         }
         if (!ok) give_up(13);
-        if (lane == 0) umma_commit(bar(Sh::bO));
+        if (elect_one()) umma_commit(bar(Sh::bO));
         __syncwarp();
-        if (!mbar_wait_warp(bar(Sh::bO), 0)) give_up(14);       // tensor memory is given back behind the last product
+        if (!__all_sync(kFull, mbar_wait(bar(Sh::bO), 0))) give_up(14);       // tensor memory is given back behind the last product
+    } else if (warp >= Sh::kMma + NT) {
+        // (warps that fill a warpgroup)
     } else if constexpr (BITS == 16) {
         // =========================== TMA copies ====================================================================
         const uint32_t ids = kKt >> p.page_shift;
-        if (lane == 0 && sp.n > 0) {
+        if (lane == 0 && kt.n > 0) {
             const uint32_t bytes = a.tt * a.group * 128;        // of a block of 64 channels
             mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
             for (uint32_t t = 0; t < NT; ++t)
@@ -367,16 +474,16 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         uint32_t issued = 0, fixes = 0;
         bool ok = true;
         auto row_of = [&](int32_t i) {                          // this lane's page of tile i, as a row of the pool
-            const int32_t at = sp.first(i) + (int32_t)(lane << p.page_shift);
-            const int32_t id = lane < ids && at < sp.all_hi ? page_of(p, b, at) : -1;
+            const int32_t at = kt.first(i) + (int32_t)(lane << p.page_shift);
+            const int32_t id = lane < ids && at < kt.hi ? page_of(p, b, at) : -1;
             return id < 0 ? -(int32_t)kKt : (int32_t)row_index(p, id, kvh, at);
         };
-        int32_t next = sp.n > 0 ? row_of(0) : 0;
-        for (int32_t i = 0; i < sp.n && ok; ++i) {
-            const int32_t r = next, f = sp.first(i);
-            if (i + 1 < sp.n) next = row_of(i + 1);
+        int32_t next = kt.n > 0 ? row_of(0) : 0;
+        for (int32_t i = 0; i < kt.n && ok; ++i) {
+            const int32_t r = next, f = kt.first(i);
+            if (i + 1 < kt.n) next = row_of(i + 1);
             // rows of V that no query of the block sees become zeros: 0 times what lies there need not be 0
-            const bool fix = f + (int32_t)kKt > sp.all_hi || (a.window && f <= sp.all_lo - 1 && f + (int32_t)kKt > a.sinks);
+            const bool fix = f + (int32_t)kKt > kt.hi || (a.window && f <= kt.lo - 1 && f + (int32_t)kKt > a.sinks);
             for (uint32_t kv = 0; kv < 2; ++kv, ++issued) {
                 const uint32_t slot = issued % NS;
                 if (!mbar_wait_warp(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1) || *s_abort) { give_up(15); ok = false; break; }
@@ -394,7 +501,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     ++fixes;
                     for (uint32_t y = 0; y < kKt; ++y) {
                         const int32_t at = f + (int32_t)y;
-                        if (at < sp.all_hi && !(a.window && at < sp.all_lo && at >= a.sinks)) continue;
+                        if (at < kt.hi && !(a.window && at < kt.lo && at >= a.sinks)) continue;
                         for (uint32_t c = lane; c < NB * 8; c += 32)
                             sts_v4(dst + (c / 8) * Sh::kBlock + y * 128 + (c % 8) * 16, 0, 0, 0, 0);
                     }
@@ -406,12 +513,12 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         }
         if (!ok)                                                // copies under way end before the block does
             for (uint32_t c = issued > NS ? issued - NS : 0; c < issued; ++c) (void)mbar_wait_warp(bar(Sh::bFull + c % NS), (c / NS) & 1);
-        if (!ok && sp.n > 0) (void)mbar_wait_warp(bar(Sh::bQ), 0);
+        if (!ok && kt.n > 0) (void)mbar_wait_warp(bar(Sh::bQ), 0);
     } else {
         // =========================== codes to bf16: one thread per position ==========================================
         constexpr uint32_t G = D / 64;
         const uint32_t y = threadIdx.x - Sh::kProd * 32;        // position inside the tile
-        if (y == 0 && sp.n > 0) {
+        if (y == 0 && kt.n > 0) {
             const uint32_t bytes = a.tt * a.group * 128;
             mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
             for (uint32_t t = 0; t < NT; ++t)
@@ -421,9 +528,9 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         }
         uint32_t issued = 0;
         bool ok = true;
-        for (int32_t i = 0; i < sp.n && ok; ++i) {
-            const int32_t at = sp.first(i) + (int32_t)y;
-            const bool wanted = at < sp.all_hi && !(a.window && at < sp.all_lo && at >= a.sinks);
+        for (int32_t i = 0; i < kt.n && ok; ++i) {
+            const int32_t at = kt.first(i) + (int32_t)y;
+            const bool wanted = at < kt.hi && !(a.window && at < kt.lo && at >= a.sinks);
             const int32_t id = wanted ? page_of(p, b, at) : -1;
             const size_t r = id < 0 ? 0 : row_index(p, id, kvh, at);
             for (uint32_t kv = 0; kv < 2; ++kv, ++issued) {
@@ -458,7 +565,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 if (lane == 0) mbar_arrive(bar(Sh::bFull + slot));
             }
         }
-        if (!ok && sp.n > 0) (void)mbar_wait_warp(bar(Sh::bQ), 0);
+        if (!ok && kt.n > 0) (void)mbar_wait_warp(bar(Sh::bQ), 0);
+    }
     }
     tc_fence_before();
     __syncthreads();
