@@ -11,8 +11,14 @@
 // row's own thread does that too, between two products, when nothing else touches it.  Tiles that no row sees are not visited; a page that does not exist
 // is fetched from outside the tensor, which gives zeros.
 //
-// One warp per query tile issues the products, one the TMA copies (for 4 bits, four warps turn codes into bf16); mbarriers
-// connect them.  All waits are bounded: on expiry a role sets the status word and the abort flag, and everyone leaves.
+// A cache of 4 bits is turned into fp16 on its way into shared memory by four warps, so that what codes stand for, and the
+// weights, are rounded by 2^-12 and not 2^-9 (error of a prompt's outputs against 64 bits 0.0017 instead of 0.0034; bf16's own
+// rounding of the result is 0.0016).  fp16 has no range for that by itself: every key tile is scaled by the power of two that
+// its largest value asks for, the values by one that only grows, O following it, and a query row by its own.
+//
+// One warp per query tile issues the products, one the TMA copies; mbarriers connect them.  All waits are bounded: on expiry a role sets the status word and the abort flag, and everyone leaves.
+#include <cuda_fp16.h>
+
 #include <type_traits>
 
 #include "paged.cuh"
@@ -43,14 +49,19 @@ struct PromptShape {
     static constexpr uint32_t PW = BITS == 16 ? 1 : 4;                       // producer warps
     static constexpr uint32_t kProd = 4 * NT, kMma = kProd + PW;
     // Two query tiles: whole warpgroups, so that registers can go where the scores are held.
-    static constexpr uint32_t kWarps = NT == 2 ? (kMma + NT + 3) / 4 * 4 : kMma + NT, kThreads = kWarps * 32;
-    static constexpr uint32_t kSoftRegs = BITS == 16 ? 200 : 184, kProdRegs = 104, kMmaRegs = BITS == 16 ? kProdRegs : 40;
-    static_assert(NT == 1 || 256 * kSoftRegs + 128 * kProdRegs + (BITS == 16 ? 0 : 128 * kMmaRegs) <= kThreads * (65536 / kThreads / 8 * 8), "registers");
-    static constexpr uint32_t oQ = 0, oRing = NT * kTile, oBar = oRing + NS * kTile, kSmem = oBar + 256 + 1024;
+    static constexpr bool kMove = NT == 2;
+    static constexpr uint32_t kWarps = kMove ? (kMma + NT + 3) / 4 * 4 : kMma + NT, kThreads = kWarps * 32;
+    static constexpr uint32_t kLaunchRegs = 65536 / kThreads / 8 * 8;        // setmaxnreg: up from here, or down, within their sum
+    static constexpr uint32_t kSoftRegs = BITS == 16 ? 200 : 160, kProdRegs = BITS == 16 ? 104 : 120, kMmaRegs = BITS == 16 ? kProdRegs : 72;
+    static_assert(!kMove || (kSoftRegs >= kLaunchRegs && kProdRegs <= kLaunchRegs && kMmaRegs <= kLaunchRegs &&
+                             256 * kSoftRegs + 128 * kProdRegs + (BITS == 16 ? 0 : 128 * kMmaRegs) <= kThreads * kLaunchRegs), "registers");
+    static constexpr uint32_t oQ = 0, oRing = NT * kTile, oBar = oRing + NS * kTile, kSmem = oBar + 384 + 1024;
     // barriers
-    static constexpr uint32_t bQ = 0, bFull = 1, bEmpty = bFull + NS, bS = bEmpty + NS, bP = bS + NT, bO = bP + 2 * NT, bFix = bO + 1, bTurn = bFix + 1;
-    static constexpr uint32_t oTmem = (bTurn + 2) * 8, oAbort = oTmem + 4, oItem = oTmem + 8;
-    static_assert(oItem + 16 <= 256, "barrier region");
+    static constexpr uint32_t bQ = 0, bFull = 1, bEmpty = bFull + NS, bS = bEmpty + NS, bP = bS + NT, bO = bP + 2 * NT, bFix = bO + 1, bTurn = bFix + 1, bQh = bTurn + 2;
+    static constexpr uint32_t oTmem = (bQh + 1) * 8, oAbort = oTmem + 4, oItem = oTmem + 8;
+    static constexpr uint32_t oScale = oItem + 8, oLargest = oScale + 64;    // 4 bits: exponents of eight tiles' K and V; of warps
+    static_assert(oLargest + 32 <= 384, "barrier region");
+    static constexpr int kHeld = BITS == 16 ? 4 : 2;                         // groups of 32 scores that a row's thread holds
     static constexpr uint32_t cO = NT * kKt;                                 // first column of O
 };
 
@@ -118,6 +129,30 @@ __device__ __forceinline__ void ex2_poly(uint64_t x, float &r0, float &r1) {
     r0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
     r1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
 }
+
+template <int G>
+__device__ __forceinline__ void load_group_words(uint32_t (&w)[G], const uint32_t *p) {
+    if constexpr (G == 1) {
+        w[0] = __ldg(p);
+    } else if constexpr (G == 2) {
+        const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
+        w[0] = x.x; w[1] = x.y;
+    } else {
+        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+    }
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// The smallest e with x < 2^e, for x >= 0 that is finite; others do not ask for a scale.
+__device__ __forceinline__ int32_t exponent_of(float x) {
+    const uint32_t e = __float_as_uint(x) >> 23 & 0xFFu;
+    return e == 255 ? -126 : (int32_t)e - 126;
+}
+__device__ __forceinline__ float power_of_2(int32_t n) { return __uint_as_float((uint32_t)(min(max(n, -126), 127) + 127) << 23); }
 
 template <int D, int BITS>
 __global__ void __launch_bounds__(PromptShape<D, BITS>::kThreads, 1)
@@ -215,6 +250,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         mbar_init(bar(Sh::bFix), 1);
         mbar_init(bar(Sh::bTurn), 1);
         mbar_init(bar(Sh::bTurn + 1), 1);
+        mbar_init(bar(Sh::bQh), 4 * NT);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -228,7 +264,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     };
 
     if (warp < 4 * NT) {
-        if (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::kSoftRegs));
+        if (Sh::kMove) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::kSoftRegs));
         // =========================== softmax: one thread per query row ===============================================
         const uint32_t t = warp >> 2, w = warp & 3, row = w * 32 + lane;
         const uint32_t tok = row / a.group, head = row % a.group;
@@ -246,8 +282,42 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             return i < kt.n && lane < ids && at < kt.hi ? __ldg(p.table + (size_t)b * p.table_stride + ((uint32_t)at >> p.page_shift)) : 0;
         };
         int32_t id = page_id(0);
-        const uint64_t scale2 = pair(a.scale_log2, a.scale_log2);
-        for (int32_t i = 0; i < kt.n; ++i) {
+        float scale = a.scale_log2;
+        volatile const int32_t *s_scale = reinterpret_cast<volatile const int32_t *>(smem + Sh::oBar + Sh::oScale);
+        int32_t v_exp = 0;                                      // O stands for O 2^v_exp
+        if (BITS == 4 && kt.n > 0) {                            // this row of Q to fp16, its largest value below 2^15
+            ok = __all_sync(kFull, mbar_wait(bar(Sh::bQ), 0));
+            if (!ok) give_up(18);
+            const uint32_t q_s = smem_s + Sh::oQ + t * Sh::kTile + row * 128;
+            auto chunk = [&](uint32_t c) { return q_s + (c / 8) * Sh::kBlock + ((c % 8 ^ (row & 7)) << 4); };
+            float big = 0.f;
+#pragma unroll 4
+            for (uint32_t c = 0; c < D / 8; ++c) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    const uint32_t x = lds_u32(chunk(c) + 4 * e);
+                    big = fmaxf(big, fmaxf(fabsf(lo_bf16(x)), fabsf(hi_bf16(x))));
+                }
+            }
+            const int32_t e = exponent_of(big) - 15;
+            const float up = power_of_2(-e / 2), up2 = power_of_2(-e - -e / 2);
+#pragma unroll 4
+            for (uint32_t c = 0; c < D / 8; ++c) {
+                uint32_t y[4];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const uint32_t x = lds_u32(chunk(c) + 4 * j);
+                    y[j] = pack_f16(lo_bf16(x) * up * up2, hi_bf16(x) * up * up2);
+                }
+                sts_v4(chunk(c), y[0], y[1], y[2], y[3]);
+            }
+            scale *= power_of_2(e / 2) * power_of_2(e - e / 2);
+            fence_async_proxy();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(Sh::bQh));
+        }
+        const float row_scale = scale;
+        for (int32_t i = 0; i < kt.n && ok; ++i) {
             const uint32_t gone = __ballot_sync(kFull, (uint32_t)id >= p.num_pages);    // one bit per page that does not exist
             id = page_id(i + 1);
             if (!kt.seen_by(q, i)) continue;
@@ -260,7 +330,22 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 break;
             }
             tc_fence_after();
-            uint32_t x[4][32];
+            float v_down = 1.f;                                 // what O is to be multiplied by for the scale of this tile's V
+            if (BITS == 4) {
+                // The tile of V cannot be replaced before this row's weights are out, so its barrier can be waited on here; the
+                // exponents of the tile were written before it.
+                if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + (2 * i + 1) % NS), ((2 * i + 1) / NS) & 1))) {
+                    give_up(19);
+                    ok = false;
+                    break;
+                }
+                const int32_t ke = s_scale[i % 8], ve = s_scale[8 + i % 8];
+                scale = fmaxf(row_scale * power_of_2(ke / 2) * power_of_2(ke - ke / 2), 1.2e-38f);
+                v_down = done ? power_of_2(v_exp - ve) : 1.f;
+                v_exp = ve;
+            }
+            const uint64_t scale2 = pair(scale, scale);
+            uint32_t x[Sh::kHeld][32];
             auto hide = [&](uint32_t (&v)[32], int32_t c) {     // scores of positions that the row does not see
                 const int32_t f32 = f + c * 32;
                 uint32_t seen = low_bits(last + 1 - f32);
@@ -281,22 +366,29 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     for (int e = 0; e < 4; ++e)
                         mx4[e] = fmaxf(fmaxf(mx4[e], __uint_as_float(v[j + e])), __uint_as_float(v[j + 4 + e]));
             };
+            auto load = [&](int first) {                        // kHeld groups of 32 scores
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32_start(s_addr + c * 32, x[c]);
+                for (int c = 0; c < Sh::kHeld; ++c) tmem_ld32_start(s_addr + (first + c) * 32, x[c]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld_wait(x[c]);
-            if (edge)
+                for (int c = 0; c < Sh::kHeld; ++c) tmem_ld_wait(x[c]);
+                if (edge)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) hide(x[c], c);
+                    for (int c = 0; c < Sh::kHeld; ++c) hide(x[c], first + c);
+            };
 #pragma unroll
-            for (int c = 0; c < 4; ++c) largest(x[c]);
-            float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
+            for (int first = 4 - Sh::kHeld; first >= 0; first -= Sh::kHeld) {
+                load(first);
+#pragma unroll
+                for (int c = 0; c < Sh::kHeld; ++c) largest(x[c]);
+            }
+            float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;
             const bool grow = mx > m + kLazy;
-            if (__any_sync(kFull, grow)) {
-                const float c = grow ? ex2f(m - mx) : 1.f;
+            if (__any_sync(kFull, grow || v_down != 1.f)) {
+                float c = grow ? ex2f(m - mx) : 1.f;
                 if (grow) m = mx;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) l2[e] = fma2(l2[e], pair(c, c), 0);
+                c *= v_down;
                 if (done) {
 #pragma unroll 1
                     for (uint32_t j = 0; j < D / 32; ++j) {
@@ -313,13 +405,14 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             auto weights = [&](auto whole) {                    // whole: no score of the tile is hidden
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const uint32_t(&v)[32] = x[c];
+                    if (c && c % Sh::kHeld == 0) load(c);
+                    const uint32_t(&v)[32] = x[c % Sh::kHeld];
                     uint32_t pk[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         const uint64_t y = fma2(pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), scale2, ref2);
                         float e0, e1;
-                        if (decltype(whole)::value && j % 4 == 3) {
+                        if (decltype(whole)::value && BITS == 16 && j % 4 == 3) {
                             ex2_poly(y, e0, e1);
                         } else {
                             split(y, e0, e1);
@@ -327,7 +420,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                             e1 = ex2f(e1);
                         }
                         l2[j % 4] = add2(l2[j % 4], pair(e0, e1));
-                        pk[j] = pack_bf16(e0, e1);
+                        pk[j] = BITS == 16 ? pack_bf16(e0, e1) : pack_f16(e0, e1);
                     }
                     tmem_st16(s_addr + c * 16, pk);
                     if (c % 2) {                                    // half of the weights are there
@@ -355,7 +448,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         if (__all_sync(kFull, ok)) {
             tc_fence_after();
             const bool live = tok < a.tt && pos <= q.p1;
-            const float inv = m == -INFINITY ? 0.f : 1.f / l;            // (nothing seen: zeros)
+            const float inv = m == -INFINITY ? 0.f : 1.f / l;     // (nothing seen: zeros)
+            const float up = BITS == 4 ? power_of_2(v_exp / 2) : 1.f, up2 = BITS == 4 ? power_of_2(v_exp - v_exp / 2) : 1.f;
             uint16_t *dst = a.out + (int64_t)(q_row + (int32_t)(t * a.tt + tok)) * a.ldo + (size_t)(kvh * a.group + head) * D;
 #pragma unroll 1
             for (uint32_t j = 0; j < D / 32; ++j) {
@@ -372,21 +466,22 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                         uint32_t y[4];
 #pragma unroll
                         for (int h = 0; h < 4; ++h)
-                            y[h] = pack_bf16(__uint_as_float(o[8 * e + 2 * h]) * inv, __uint_as_float(o[8 * e + 2 * h + 1]) * inv);
+                            y[h] = pack_bf16(__uint_as_float(o[8 * e + 2 * h]) * inv * up * up2, __uint_as_float(o[8 * e + 2 * h + 1]) * inv * up * up2);
                         *reinterpret_cast<uint4 *>(dst + j * 32 + e * 8) = make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 }
             }
         }
     } else {
-        if (NT == 2) {                                          // by warpgroups: 4 bits have one of producers, one for the products
-            if (BITS == 4 && warp >= 12) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kMmaRegs));
+        if (Sh::kMove) {                                        // by warpgroups: 4 bits have one of producers, one for the products
+            if (BITS == 4 && warp >= Sh::kMma) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kMmaRegs));
             else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kProdRegs));
         }
     if (warp >= Sh::kMma && warp < Sh::kMma + NT) {
         // =========================== products ======================================================================
-        constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((kKt >> 3) << 17) | ((128u >> 4) << 24);
-        constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
+        constexpr uint32_t kTypes = BITS == 16 ? (1u << 7) | (1u << 10) : 0u;       // both bf16, or both fp16
+        constexpr uint32_t kIdescS = (1u << 4) | kTypes | ((kKt >> 3) << 17) | ((128u >> 4) << 24);
+        constexpr uint32_t kIdescO = (1u << 4) | kTypes | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
         // One warp per query tile, in turns: while one tile's products run, the other's rows are at their exponentials.  Without
         // turns both come to do the same at the same time (4250 cycles for a pair of query tiles and a key tile instead of 2800).
         const uint32_t t = warp - Sh::kMma, idesc_s = kIdescS | (a.negate ? 1u << 13 : 0u);
@@ -414,7 +509,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             if (elect_one()) umma_commit(bar(Sh::bEmpty + c % NS));
             __syncwarp();
         };
-        bool ok = kt.n == 0 || __all_sync(kFull, mbar_wait(bar(Sh::bQ), 0) && full(0));
+        bool ok = kt.n == 0 || __all_sync(kFull, mbar_wait(bar(BITS == 16 ? Sh::bQ : Sh::bQh), 0) && full(0));
         if (ok && kt.n > 0) {
             if (kt.seen_by(q, 0)) scores(0);
             release(0);
@@ -515,9 +610,11 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             for (uint32_t c = issued > NS ? issued - NS : 0; c < issued; ++c) (void)mbar_wait_warp(bar(Sh::bFull + c % NS), (c / NS) & 1);
         if (!ok && kt.n > 0) (void)mbar_wait_warp(bar(Sh::bQ), 0);
     } else {
-        // =========================== codes to bf16: one thread per position ==========================================
+        // =========================== codes to fp16: one thread per position ==========================================
         constexpr uint32_t G = D / 64;
         const uint32_t y = threadIdx.x - Sh::kProd * 32;        // position inside the tile
+        volatile int32_t *s_scale = reinterpret_cast<volatile int32_t *>(smem + Sh::oBar + Sh::oScale);
+        volatile uint32_t *s_largest = reinterpret_cast<volatile uint32_t *>(smem + Sh::oBar + Sh::oLargest);
         if (y == 0 && kt.n > 0) {
             const uint32_t bytes = a.tt * a.group * 128;
             mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
@@ -527,43 +624,92 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                                 q_row + (int32_t)(t * a.tt), bar(Sh::bQ));
         }
         uint32_t issued = 0;
+        int32_t v_exp = -1000;                                  // (no tile of V yet)
         bool ok = true;
-        for (int32_t i = 0; i < kt.n && ok; ++i) {
+        // What this thread's position of a tile holds, fetched while the tile before is turned.
+        struct Codes {
+            uint4 code[D / 32];
+            uint32_t sc[G];
+        };
+        auto page_at = [&](int32_t i) {                         // -1: no page, or nobody sees the position
+            if (i >= kt.n) return -1;
             const int32_t at = kt.first(i) + (int32_t)y;
-            const bool wanted = at < kt.hi && !(a.window && at < kt.lo && at >= a.sinks);
-            const int32_t id = wanted ? page_of(p, b, at) : -1;
-            const size_t r = id < 0 ? 0 : row_index(p, id, kvh, at);
-            for (uint32_t kv = 0; kv < 2; ++kv, ++issued) {
-                uint4 code[D / 32];
-                uint32_t sc[G];
-                if (id >= 0) {
-                    const uint4 *src = reinterpret_cast<const uint4 *>((kv ? a.v : a.k) + r * (D / 2));
+            return at < kt.hi && !(a.window && at < kt.lo && at >= a.sinks) ? page_of(p, b, at) : -1;
+        };
+        auto fetch = [&](Codes &f, int32_t id, int32_t i, uint32_t kv) {
+            if (id < 0) return;
+            const size_t r = row_index(p, id, kvh, kt.first(i) + (int32_t)y);
+            load_group_words(f.sc, (kv ? a.vs : a.ks) + r * G);
+            const uint4 *src = reinterpret_cast<const uint4 *>((kv ? a.v : a.k) + r * (D / 2));
 #pragma unroll
-                    for (uint32_t c = 0; c < D / 32; ++c) code[c] = __ldg(src + c);
+            for (uint32_t c = 0; c < D / 32; ++c) f.code[c] = __ldg(src + c);
+        };
+        // (to the end in any case: the four warps meet at a barrier)
+        auto turn = [&](const Codes &f, int32_t id, int32_t i, uint32_t kv) {
+            const uint32_t(&sc)[G] = f.sc;
+            float big = 0.f;
+            if (id >= 0)
 #pragma unroll
-                    for (uint32_t g = 0; g < G; ++g) sc[g] = __ldg((kv ? a.vs : a.ks) + r * G + g);
+                for (uint32_t g = 0; g < G; ++g) {
+                    const float step = lo_bf16(sc[g]), low = hi_bf16(sc[g]);
+                    big = fmaxf(big, fmaxf(fabsf(low), fabsf(low + 15.f * step)));
                 }
-                const uint32_t slot = issued % NS, dst = smem_s + Sh::oRing + slot * Sh::kTile;
-                if (!mbar_wait_warp(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1) || *s_abort) { give_up(17); ok = false; break; }
-                const uint32_t *words = &code[0].x;
+            // the tile's largest exponent
+            const uint32_t most = __reduce_max_sync(kFull, (uint32_t)(exponent_of(big) + 200));
+            if (lane == 0) s_largest[(issued & 1) * 4 + (y >> 5)] = most;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            int32_t e = 0;
 #pragma unroll
-                for (uint32_t q = 0; q < D / 8; ++q) {          // word q: eight channels of group q % G
-                    const uint32_t g = q % G, c8 = q / G;
+            for (uint32_t w = 0; w < 4; ++w) e = max(e, (int32_t)s_largest[(issued & 1) * 4 + w]);
+            e -= 200;
+            if (kv == 0) e -= 14;                           // below 2^14
+            else if (e - v_exp > 15) e = v_exp = e - 12;    // below 2^15; where it has to grow, below 2^12 again
+            else e = v_exp;
+            const float down = power_of_2(-e / 2), down2 = power_of_2(-e - -e / 2);
+            const uint32_t slot = issued % NS, dst = smem_s + Sh::oRing + slot * Sh::kTile + y * 128;
+            if (ok && (!mbar_wait_warp(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1) || *s_abort)) {
+                give_up(17);
+                ok = false;
+            }
+            if (!ok) return;
+            if (y == 0) s_scale[kv * 8 + i % 8] = e;
+            const uint32_t *words = &f.code[0].x;
+#pragma unroll
+            for (uint32_t g = 0; g < G; ++g) {
+                const float step = lo_bf16(sc[g]) * down * down2, low = hi_bf16(sc[g]) * down * down2;
+                const __half2 step2 = __float2half2_rn(step), low2 = __float2half2_rn(low), base = __float2half2_rn(1024.f);
+#pragma unroll
+                for (uint32_t c8 = 0; c8 < 8; ++c8) {       // word c8 of the group: eight channels
                     uint32_t o[4] = {0, 0, 0, 0};
                     if (id >= 0) {
-                        const float step = lo_bf16(sc[g]), low = hi_bf16(sc[g]);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const uint32_t w = words[q] >> 4 * j;
-                            o[j] = pack_bf16(step * (float)(w & 15u) + low, step * (float)(w >> 16 & 15u) + low);
+                            // fp16 of 1024 + code, the code, and one rounding for what it stands for
+                            const uint32_t w = (words[c8 * G + g] >> 4 * j & 0x000F000Fu) | 0x64006400u;
+                            const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2 *>(&w), base), step2, low2);
+                            o[j] = *reinterpret_cast<const uint32_t *>(&v);
                         }
                     }
-                    sts_v4(dst + g * Sh::kBlock + y * 128 + ((c8 ^ (y & 7)) << 4), o[0], o[1], o[2], o[3]);
+                    sts_v4(dst + g * Sh::kBlock + ((c8 ^ (y & 7)) << 4), o[0], o[1], o[2], o[3]);
                 }
-                fence_async_proxy();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(Sh::bFull + slot));
             }
+            fence_async_proxy();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(Sh::bFull + slot));
+        };
+        Codes f0, f1;
+        int32_t id = page_at(0), id_next = page_at(1);
+        if (kt.n > 0) fetch(f0, id, 0, 0);
+        for (int32_t i = 0; i < kt.n; ++i) {
+            fetch(f1, id, i, 1);
+            turn(f0, id, i, 0);
+            ++issued;
+            const int32_t id_here = id;
+            id = id_next;
+            if (i + 1 < kt.n) fetch(f0, id, i + 1, 0);
+            id_next = page_at(i + 2);
+            turn(f1, id_here, i, 1);
+            ++issued;
         }
         if (!ok && kt.n > 0) (void)mbar_wait_warp(bar(Sh::bQ), 0);
     }

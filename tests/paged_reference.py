@@ -77,8 +77,9 @@ def attention(q, cache, table, kv_lens, q_starts=None, window=0, sinks=0, scale=
     """(result, bound) float64 [T, n_q, d]: the result, and how far one that rounds each weight (4 bits: times its step) and
     the result to bf16 may be from it.  Half a step of bf16 is 2^-8 relative: 2^-8 (sum of p |v| + |o|); for 4 bits
     |v - middle| in the place of |v|, the middle of a group being code 8, where the few new tokens' kernel rounds the weights'
-    products with steps alone, and 2 |v| and the change of p by keys that are rounded too, 2^-8 scale sum |q k|, where the
-    prompts' kernel makes bf16 of codes (`prompt`); a sixty-fourth more for products of roundings; and for sums in float32
+    products with steps alone; the prompts' kernel (more than `few` query rows of a sequence and key head) has weights, values
+    and keys of 4 bits in fp16, half a step 2^-11: 2 |v| for the first two and the change of p by the third, whose scores are
+    off by 2^-11 scale sum |q k|; a sixty-fourth more for products of roundings; and for sums in float32
     2^-18 of the sum of p times the largest thing added up, |v| or (4 bits) step * 143 and |lowest|."""
     T, n_q, d = q.shape
     scale = d ** -0.5 if scale is None else scale
@@ -120,7 +121,7 @@ def attention(q, cache, table, kv_lens, q_starts=None, window=0, sinks=0, scale=
                 a, big = p @ (v[:, g] - lowv[:, g] - 8 * stepv[:, g]).abs(), p @ (143 * stepv[:, g] + lowv[:, g].abs())
                 if q_starts is not None and (int(q_starts[b + 1]) - int(q_starts[b])) * (n_q // cache.n_kv) > few:
                     ds = scale * (k[:, g].abs() @ q[t, h].double().abs())       # p_j changes by at most (e^(2 max ds) - 1) p_j
-                    a = 2 * (p @ v[:, g].abs()) + (p * 2 * ds.max()) @ (v[:, g] - out[t, h]).abs()
+                    a = (2 * (p @ v[:, g].abs()) + (p * 2 * ds.max()) @ (v[:, g] - out[t, h]).abs()) / 8
             bound[t, h] = 2.0 ** -8 * (a + out[t, h].abs()) * (1 + 2.0 ** -6) + 2.0 ** -18 * big
     return out, bound
 

@@ -323,6 +323,25 @@ def test_positions_without_a_page(new, bits):
     check_attention(q, cache, table, [30, 20], new, window=5)
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("new", [None, [150]])
+def test_values_far_from_1(new, bits):
+    """Keys, queries and values of 1e-6 and of 1e6, and values that grow along the sequence by 2^40."""
+    g = gen(19)
+    kv, d = [400], 128
+    T = new[0] if new else 1
+    table = make_table(g, kv, 32, 14)
+    for kq, kk, kv_ in ((1e-6, 1e6, 1.0), (1e3, 1e-3, 1e6), (1.0, 1.0, 1e-6), (1.0, 1.0, None)):
+        cache = ci().PagedKVCache(14, 32, 1, d, bits, DEV)
+        pos = torch.arange(kv[0], dtype=torch.float64)
+        grow = (2.0 ** (pos / 10.0 - 20.0))[:, None] if kv_ is None else kv_
+        k, v = (kk * rnd(g, kv[0], d)).to(torch.bfloat16).to(DEV), (grow * rnd(g, kv[0], d)).to(torch.bfloat16).to(DEV)
+        one, none = torch.ones(400, d, dtype=torch.bfloat16, device=DEV), torch.zeros(400, d, dtype=torch.bfloat16, device=DEV)
+        ci().rope_paged_append(k, k, v, one, none, cache, table.to(DEV), i32(kv), i32([0, 400]))
+        q = (kq * rnd(g, T, 4, d)).to(torch.bfloat16).to(DEV)
+        check_attention(q, cache, table, kv, new)
+
+
 def test_strides_scale_and_out():
     g = gen(15)
     kv, d = [100, 37, 5], 128
