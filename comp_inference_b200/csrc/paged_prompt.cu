@@ -11,7 +11,7 @@
 // row's own thread does that too, between two products, when nothing else touches it.  Tiles that no row sees are not visited; a page that does not exist
 // is fetched from outside the tensor, which gives zeros.
 //
-// A cache of 4 bits is turned into fp16 on its way into shared memory by four warps, so that what codes stand for, and the
+// A cache of 4 bits is turned into fp16 on its way into shared memory by four or eight warps, so that what codes stand for, and the
 // weights, are rounded by 2^-12 and not 2^-9 (error of a prompt's outputs against 64 bits 0.0017 instead of 0.0034; bf16's own
 // rounding of the result is 0.0016).  fp16 has no range for that by itself: every key tile is scaled by the power of two that
 // its largest value asks for, the values by one that only grows, O following it, and a query row by its own.
@@ -46,21 +46,25 @@ struct PromptShape {
     static constexpr uint32_t NT = D == 256 ? 1 : 2;
     static constexpr uint32_t kTile = kKt * D * 2, kBlock = kKt * 128;       // bytes: a tile of 128 rows, its 64-channel block
     static constexpr uint32_t NS = D == 64 ? 6 : D == 128 ? 4 : 2;           // ring of K and V tiles
-    static constexpr uint32_t PW = BITS == 16 ? 1 : 4;                       // producer warps
+    static constexpr uint32_t SPLIT = BITS == 4 && D > 64 ? 2 : 1;           // threads that share a position's codes
+    static constexpr uint32_t PW = BITS == 16 ? 1 : 4 * SPLIT;               // producer warps
     static constexpr uint32_t kProd = 4 * NT, kMma = kProd + PW;
-    // Two query tiles: whole warpgroups, so that registers can go where the scores are held.
-    static constexpr bool kMove = NT == 2;
+    // Whole warpgroups (but where nothing is gained), so that registers can go where the scores are held: setmaxnreg takes them
+    // up or down from what the block is launched with, within its sum.
+    static constexpr bool kMove = NT == 2 || BITS == 4;
     static constexpr uint32_t kWarps = kMove ? (kMma + NT + 3) / 4 * 4 : kMma + NT, kThreads = kWarps * 32;
-    static constexpr uint32_t kLaunchRegs = 65536 / kThreads / 8 * 8;        // setmaxnreg: up from here, or down, within their sum
-    static constexpr uint32_t kSoftRegs = BITS == 16 ? 200 : 160, kProdRegs = BITS == 16 ? 104 : 120, kMmaRegs = BITS == 16 ? kProdRegs : 72;
+    static constexpr uint32_t kLaunchRegs = 65536 / kThreads / 8 * 8;
+    static constexpr uint32_t kSoftRegs = BITS == 16 ? 200 : D == 64 ? 160 : D == 128 ? 152 : 176;
+    static constexpr uint32_t kProdRegs = BITS == 16 ? 104 : D == 64 ? 120 : D == 128 ? 64 : 104;
+    static constexpr uint32_t kMmaRegs = BITS == 16 ? kProdRegs : D == 64 ? 72 : D == 128 ? 48 : 112;
     static_assert(!kMove || (kSoftRegs >= kLaunchRegs && kProdRegs <= kLaunchRegs && kMmaRegs <= kLaunchRegs &&
-                             256 * kSoftRegs + 128 * kProdRegs + (BITS == 16 ? 0 : 128 * kMmaRegs) <= kThreads * kLaunchRegs), "registers");
+                             NT * 128 * kSoftRegs + (BITS == 16 ? 128 * kProdRegs : PW * 32 * kProdRegs + 128 * kMmaRegs) <= kThreads * kLaunchRegs), "registers");
     static constexpr uint32_t oQ = 0, oRing = NT * kTile, oBar = oRing + NS * kTile, kSmem = oBar + 384 + 1024;
     // barriers
     static constexpr uint32_t bQ = 0, bFull = 1, bEmpty = bFull + NS, bS = bEmpty + NS, bP = bS + NT, bO = bP + 2 * NT, bFix = bO + 1, bTurn = bFix + 1, bQh = bTurn + 2;
     static constexpr uint32_t oTmem = (bQh + 1) * 8, oAbort = oTmem + 4, oItem = oTmem + 8;
     static constexpr uint32_t oScale = oItem + 8, oLargest = oScale + 64;    // 4 bits: exponents of eight tiles' K and V; of warps
-    static_assert(oLargest + 32 <= 384, "barrier region");
+    static_assert(oLargest + 64 <= 384, "barrier region");
     static constexpr int kHeld = BITS == 16 ? 4 : 2;                         // groups of 32 scores that a row's thread holds
     static constexpr uint32_t cO = NT * kKt;                                 // first column of O
 };
@@ -130,16 +134,19 @@ __device__ __forceinline__ void ex2_poly(uint64_t x, float &r0, float &r1) {
     r1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
 }
 
-template <int G>
-__device__ __forceinline__ void load_group_words(uint32_t (&w)[G], const uint32_t *p) {
-    if constexpr (G == 1) {
-        w[0] = __ldg(p);
-    } else if constexpr (G == 2) {
-        const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
-        w[0] = x.x; w[1] = x.y;
+// Words that are asked for here and not where they are used: the compiler moves ordinary loads down to there.
+template <int N>
+__device__ __forceinline__ void ask_words(uint32_t (&w)[N], const uint32_t *p) {
+    if constexpr (N == 1) {
+        asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+    } else if constexpr (N == 2) {
+        asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
     } else {
-        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
-        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
+                         : "l"(p + i));
     }
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -610,12 +617,14 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             for (uint32_t c = issued > NS ? issued - NS : 0; c < issued; ++c) (void)mbar_wait_warp(bar(Sh::bFull + c % NS), (c / NS) & 1);
         if (!ok && kt.n > 0) (void)mbar_wait_warp(bar(Sh::bQ), 0);
     } else {
-        // =========================== codes to fp16: one thread per position ==========================================
+        // =========================== codes to fp16: a thread, or two, per position ==========================================
         constexpr uint32_t G = D / 64;
-        const uint32_t y = threadIdx.x - Sh::kProd * 32;        // position inside the tile
+        constexpr uint32_t PW = Sh::PW, NW = D / 8 / Sh::SPLIT;  // warps; words of a thread
+        const uint32_t y = (threadIdx.x - Sh::kProd * 32) % kKt, part = (threadIdx.x - Sh::kProd * 32) / kKt;   // position inside the tile
+        const bool first_thread = threadIdx.x == Sh::kProd * 32;
         volatile int32_t *s_scale = reinterpret_cast<volatile int32_t *>(smem + Sh::oBar + Sh::oScale);
         volatile uint32_t *s_largest = reinterpret_cast<volatile uint32_t *>(smem + Sh::oBar + Sh::oLargest);
-        if (y == 0 && kt.n > 0) {
+        if (first_thread && kt.n > 0) {
             const uint32_t bytes = a.tt * a.group * 128;
             mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
             for (uint32_t t = 0; t < NT; ++t)
@@ -628,27 +637,27 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         bool ok = true;
         // What this thread's position of a tile holds, fetched while the tile before is turned.
         struct Codes {
-            uint4 code[D / 32];
-            uint32_t sc[G];
+            uint32_t code[NW], sc[G];
         };
-        auto page_at = [&](int32_t i) {                         // -1: no page, or nobody sees the position
+        // Its page as the table has it (looked at when it is there, not when it is asked for); -1 where nobody sees the position.
+        auto page_at = [&](int32_t i) {
             if (i >= kt.n) return -1;
             const int32_t at = kt.first(i) + (int32_t)y;
-            return at < kt.hi && !(a.window && at < kt.lo && at >= a.sinks) ? page_of(p, b, at) : -1;
+            return at < kt.hi && !(a.window && at < kt.lo && at >= a.sinks)
+                       ? __ldg(p.table + (size_t)b * p.table_stride + ((uint32_t)at >> p.page_shift)) : -1;
         };
         auto fetch = [&](Codes &f, int32_t id, int32_t i, uint32_t kv) {
-            if (id < 0) return;
+            if ((uint32_t)id >= p.num_pages) return;
             const size_t r = row_index(p, id, kvh, kt.first(i) + (int32_t)y);
-            load_group_words(f.sc, (kv ? a.vs : a.ks) + r * G);
-            const uint4 *src = reinterpret_cast<const uint4 *>((kv ? a.v : a.k) + r * (D / 2));
-#pragma unroll
-            for (uint32_t c = 0; c < D / 32; ++c) f.code[c] = __ldg(src + c);
+            ask_words(f.sc, (kv ? a.vs : a.ks) + r * G);
+            ask_words(f.code, reinterpret_cast<const uint32_t *>(kv ? a.v : a.k) + r * (D / 8) + part * NW);
         };
-        // (to the end in any case: the four warps meet at a barrier)
+        // (to the end in any case: the warps meet at a barrier)
         auto turn = [&](const Codes &f, int32_t id, int32_t i, uint32_t kv) {
             const uint32_t(&sc)[G] = f.sc;
+            const bool there = (uint32_t)id < p.num_pages;
             float big = 0.f;
-            if (id >= 0)
+            if (there)
 #pragma unroll
                 for (uint32_t g = 0; g < G; ++g) {
                     const float step = lo_bf16(sc[g]), low = hi_bf16(sc[g]);
@@ -656,41 +665,40 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 }
             // the tile's largest exponent
             const uint32_t most = __reduce_max_sync(kFull, (uint32_t)(exponent_of(big) + 200));
-            if (lane == 0) s_largest[(issued & 1) * 4 + (y >> 5)] = most;
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (lane == 0) s_largest[(issued & 1) * 8 + (warp - Sh::kProd)] = most;
+            asm volatile("bar.sync 1, %0;" ::"n"(PW * 32) : "memory");
             int32_t e = 0;
 #pragma unroll
-            for (uint32_t w = 0; w < 4; ++w) e = max(e, (int32_t)s_largest[(issued & 1) * 4 + w]);
+            for (uint32_t w = 0; w < PW; ++w) e = max(e, (int32_t)s_largest[(issued & 1) * 8 + w]);
             e -= 200;
             if (kv == 0) e -= 14;                           // below 2^14
             else if (e - v_exp > 15) e = v_exp = e - 12;    // below 2^15; where it has to grow, below 2^12 again
             else e = v_exp;
             const float down = power_of_2(-e / 2), down2 = power_of_2(-e - -e / 2);
             const uint32_t slot = issued % NS, dst = smem_s + Sh::oRing + slot * Sh::kTile + y * 128;
-            if (ok && (!mbar_wait_warp(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1) || *s_abort)) {
+            if (ok && !__all_sync(kFull, mbar_wait(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1))) {
                 give_up(17);
                 ok = false;
             }
             if (!ok) return;
-            if (y == 0) s_scale[kv * 8 + i % 8] = e;
-            const uint32_t *words = &f.code[0].x;
+            if (first_thread) s_scale[kv * 8 + i % 8] = e;
 #pragma unroll
             for (uint32_t g = 0; g < G; ++g) {
                 const float step = lo_bf16(sc[g]) * down * down2, low = hi_bf16(sc[g]) * down * down2;
                 const __half2 step2 = __float2half2_rn(step), low2 = __float2half2_rn(low), base = __float2half2_rn(1024.f);
 #pragma unroll
-                for (uint32_t c8 = 0; c8 < 8; ++c8) {       // word c8 of the group: eight channels
+                for (uint32_t c8 = 0; c8 < NW / G; ++c8) {  // a word of the group: eight channels
                     uint32_t o[4] = {0, 0, 0, 0};
-                    if (id >= 0) {
+                    if (there) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             // fp16 of 1024 + code, the code, and one rounding for what it stands for
-                            const uint32_t w = (words[c8 * G + g] >> 4 * j & 0x000F000Fu) | 0x64006400u;
+                            const uint32_t w = (f.code[c8 * G + g] >> 4 * j & 0x000F000Fu) | 0x64006400u;
                             const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2 *>(&w), base), step2, low2);
                             o[j] = *reinterpret_cast<const uint32_t *>(&v);
                         }
                     }
-                    sts_v4(dst + g * Sh::kBlock + ((c8 ^ (y & 7)) << 4), o[0], o[1], o[2], o[3]);
+                    sts_v4(dst + g * Sh::kBlock + ((part * (NW / G) + c8 ^ (y & 7)) << 4), o[0], o[1], o[2], o[3]);
                 }
             }
             fence_async_proxy();
