@@ -738,7 +738,7 @@ Tensor adjust_logits(const Tensor &logits, const OptTensor &tokens, const OptTen
     if (tokens.has_value()) {
         refuse(!lens.has_value(), "tokens need their lengths");
         a.d_tokens = (const int64_t *)rows(tokens, at::kLong, -1, "tokens", a.ld_tokens);
-        refuse(tokens->size(1) > 0x7FFFFFFF, "a history of " + shape_of(*tokens));
+        refuse(tokens->size(1) >= (1 << 30), "a history of " + shape_of(*tokens));
         a.L = (uint32_t)tokens->size(1);
         a.d_lens = (const int32_t *)each(lens, at::kInt, "lens");
         a.d_prompt_lens = (const int32_t *)each(prompt_lens, at::kInt, "prompt_lens");

@@ -5,13 +5,16 @@
 //   x -> x - f * count - p * (count > 0), count over the generated part
 //   x -> x + the sum of the token's biases;  -inf where its mask bit is 0
 //
-// A block has kChunk tokens of one row: it counts the history's tokens of that range in shared memory (bit 31: seen),
-// adds up the biases there, and then reads, changes and writes the logits, eight to a load.
+// A block has kChunk tokens of one row: it asks for its logits, counts the history's tokens of that range in shared memory
+// meanwhile (bit 31: seen, bit 30: has a bias), and then changes and writes the logits, eight to a load.  Tokens in neither are
+// most: one word in shared memory says so.  64 rows of 131072 with histories up to 4096 tokens, 32 biases and a mask: ZZZZ.
 #include "paged.cuh"
 
 namespace ci {
 
-constexpr uint32_t kChunk = 4096;
+constexpr uint32_t kChunk = 8192, kLogitThreads = 512, kLogitLoads = kChunk / (kLogitThreads * 8);
+constexpr uint32_t kBiases = 512;
+constexpr uint32_t kSeen = 1u << 31, kBiased = 1u << 30;
 
 struct LogitArgs {
     const uint16_t *in;
@@ -24,62 +27,95 @@ struct LogitArgs {
     const uint32_t *mask;
 };
 
-__global__ void __launch_bounds__(256) k_adjust_logits(const __grid_constant__ LogitArgs a) {
-    __shared__ uint32_t s_count[kChunk];
-    __shared__ float s_bias[kChunk];
+__global__ void __launch_bounds__(kLogitThreads) k_adjust_logits(const __grid_constant__ LogitArgs a) {
+    __shared__ __align__(16) uint32_t s_count[kChunk];
+    __shared__ int32_t s_at[kBiases];            // places of the biases in this range, -1: elsewhere
+    __shared__ float s_bias[kBiases];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t b = blockIdx.y, v0 = blockIdx.x * kChunk, n = min(kChunk, a.V - v0);
-    const bool history = a.tokens != nullptr, biases = a.n_bias != 0;
-    for (uint32_t i = threadIdx.x; i < kChunk; i += 256) {
-        s_count[i] = 0;
-        s_bias[i] = 0.f;
-    }
-    __syncthreads();
-    if (history) {
-        const uint32_t len = (uint32_t)min(max(a.lens[b], 0), (int32_t)a.L);
-        const uint32_t prompt = a.prompt_lens ? (uint32_t)min(max(a.prompt_lens[b], 0), (int32_t)len) : 0;
-        const int64_t *tok = a.tokens + (int64_t)b * a.ld_tokens;
-        for (uint32_t i = threadIdx.x; i < len; i += 256) {
-            const uint64_t at = (uint64_t)__ldg(tok + i) - v0;
-            if (at >= n) continue;
-            if (i >= prompt) atomicAdd(&s_count[at], 1u);
-            atomicOr(&s_count[at], 0x80000000u);
-        }
-    }
-    if (biases && threadIdx.x == 0) {                           // in order: the same sum every time
-        for (uint32_t i = 0; i < a.n_bias; ++i) {
-            const uint64_t at = (uint64_t)a.bias_ids[(int64_t)b * a.ld_bias + i] - v0;
-            if (at < n) s_bias[at] += a.bias[(int64_t)b * a.ld_bias + i];
-        }
-    }
-    __syncthreads();
-    const float r = a.repetition ? a.repetition[b] : 1.f, f = a.frequency ? a.frequency[b] : 0.f, p = a.presence ? a.presence[b] : 0.f;
     const uint16_t *in = a.in + (int64_t)b * a.ldi + v0;
     uint16_t *out = a.out + (int64_t)b * a.ldo + v0;
-    auto one = [&](float x, uint32_t i, uint32_t allowed) {
-        const uint32_t c = s_count[i], count = c & 0x7FFFFFFFu;
-        if (c) {
-            if (a.repetition) x = x > 0.f ? __fdiv_rn(x, r) : x * r;
-            if (count) x = x - f * (float)count - p;
-        }
-        if (biases) x += s_bias[i];
-        return allowed ? x : -INFINITY;
-    };
     const uint32_t *mask = a.mask ? a.mask + (int64_t)b * a.ld_mask + v0 / 32 : nullptr;
-    if (a.vec) {
-        for (uint32_t i = threadIdx.x * 8; i < n; i += 2048) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(in + i);
-            const uint32_t bits = mask ? __ldg(mask + i / 32) >> (i % 32) : 0xFFu;
-            const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-            uint32_t y[4];
+    uint4 x[kLogitLoads];
+    uint32_t bits[kLogitLoads];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                y[j] = pack_bf16(one(lo_bf16(x[j]), i + 2 * j, bits >> 2 * j & 1), one(hi_bf16(x[j]), i + 2 * j + 1, bits >> (2 * j + 1) & 1));
+    for (uint32_t k = 0; k < kLogitLoads; ++k) {
+        const uint32_t i = (k * kLogitThreads + threadIdx.x) * 8;
+        x[k] = make_uint4(0, 0, 0, 0);
+        bits[k] = 0xFFu;
+        if (a.vec && i < n) {
+            x[k] = *reinterpret_cast<const uint4 *>(in + i);
+            if (mask) bits[k] = __ldg(mask + i / 32) >> (i % 32);
+        }
+    }
+    const bool history = a.tokens != nullptr;
+    const float r = a.repetition ? __ldg(a.repetition + b) : 1.f, f = a.frequency ? __ldg(a.frequency + b) : 0.f;
+    const float p = a.presence ? __ldg(a.presence + b) : 0.f;
+    for (uint32_t i = threadIdx.x; i < kChunk / 4; i += kLogitThreads) reinterpret_cast<uint4 *>(s_count)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    if (history) {
+        const uint32_t len = (uint32_t)min(max(__ldg(a.lens + b), 0), (int32_t)a.L);
+        const uint32_t prompt = a.prompt_lens ? (uint32_t)min(max(__ldg(a.prompt_lens + b), 0), (int32_t)len) : 0;
+        const int64_t *tok = a.tokens + (int64_t)b * a.ld_tokens;
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x; i < len; i += kLogitThreads) {
+            const uint64_t at = (uint64_t)__ldg(tok + i) - v0;
+            if (at < n) {
+                atomicOr(&s_count[at], kSeen);
+                if (i >= prompt) atomicAdd(&s_count[at], 1u);
+            }
+        }
+    }
+    const uint32_t n_bias = min(a.n_bias, kBiases);             // kept in shared memory; more than that are read again
+    for (uint32_t i = threadIdx.x; i < a.n_bias; i += kLogitThreads) {
+        const uint64_t at = (uint64_t)__ldg(a.bias_ids + (int64_t)b * a.ld_bias + i) - v0;
+        if (at < n) atomicOr(&s_count[at], kBiased);
+        if (i < kBiases) {
+            s_at[i] = at < n ? (int32_t)at : -1;
+            s_bias[i] = __ldg(a.bias + (int64_t)b * a.ld_bias + i);
+        }
+    }
+    __syncthreads();
+    auto one = [&](float y, uint32_t i, uint32_t allowed) {
+        const uint32_t c = s_count[i], count = c & (kBiased - 1);
+        if (c) {
+            if (a.repetition && (c & kSeen)) y = y > 0.f ? __fdiv_rn(y, r) : y * r;
+            if (count) y = y - f * (float)count - p;
+            if (c & kBiased) {                                  // in order: the same sum every time
+                float sum = 0.f;
+                for (uint32_t k = 0; k < n_bias; ++k)
+                    if (s_at[k] == (int32_t)i) sum += s_bias[k];
+                for (uint32_t k = kBiases; k < a.n_bias; ++k)
+                    if ((uint64_t)__ldg(a.bias_ids + (int64_t)b * a.ld_bias + k) - v0 == i) sum += __ldg(a.bias + (int64_t)b * a.ld_bias + k);
+                y += sum;
+            }
+        }
+        return allowed ? y : -INFINITY;
+    };
+    if (a.vec) {
+#pragma unroll
+        for (uint32_t k = 0; k < kLogitLoads; ++k) {
+            const uint32_t i = (k * kLogitThreads + threadIdx.x) * 8;
+            if (i >= n) continue;
+            const uint4 c0 = *reinterpret_cast<const uint4 *>(s_count + i), c1 = *reinterpret_cast<const uint4 *>(s_count + i + 4);
+            const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+            uint32_t y[4] = {w[0], w[1], w[2], w[3]};
+            if (c0.x | c0.y | c0.z | c0.w | c1.x | c1.y | c1.z | c1.w) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = pack_bf16(one(lo_bf16(w[j]), i + 2 * j, 1), one(hi_bf16(w[j]), i + 2 * j + 1, 1));
+            }
+            if (mask) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (!(bits[k] >> 2 * j & 1)) y[j] = (y[j] & 0xFFFF0000u) | 0xFF80u;
+                    if (!(bits[k] >> (2 * j + 1) & 1)) y[j] = (y[j] & 0x0000FFFFu) | 0xFF800000u;
+                }
+            }
             *reinterpret_cast<uint4 *>(out + i) = make_uint4(y[0], y[1], y[2], y[3]);
         }
     } else {
-        for (uint32_t i = threadIdx.x; i < n; i += 256)
+        for (uint32_t i = threadIdx.x; i < n; i += kLogitThreads)
             out[i] = float_to_bf16_bits(one(lo_bf16(in[i]), i, mask ? __ldg(mask + i / 32) >> (i % 32) & 1 : 1));
     }
 }
@@ -93,7 +129,7 @@ extern "C" int ci_adjust_logits(const ci_logit_adjust *d, ci_stream_t stream) {
     CI_REQUIRE(d->V > 0 && d->V <= 0x7FFFFFFFu && d->ld_in >= (int64_t)d->V && d->ld_out >= (int64_t)d->V, "row stride smaller than the vocabulary");
     CI_REQUIRE(d->B <= 65535, "%u rows of logits", d->B);
     CI_REQUIRE(d->L == 0 || d->d_tokens == nullptr || (d->d_lens && d->ld_tokens >= (int64_t)d->L), "a history needs its lengths");
-    CI_REQUIRE(d->L <= 0x7FFFFFFFu, "a history of %u tokens", d->L);
+    CI_REQUIRE(d->L < kBiased, "a history of %u tokens", d->L);
     CI_REQUIRE(d->n_bias == 0 || (d->d_bias_ids && d->d_bias && d->ld_bias >= (int64_t)d->n_bias), "biases need their tokens and values");
     CI_REQUIRE(d->d_mask == nullptr || d->ld_mask >= ((int64_t)d->V + 31) / 32, "mask rows shorter than the vocabulary");
     if (d->B == 0) return CI_OK;
@@ -109,7 +145,7 @@ extern "C" int ci_adjust_logits(const ci_logit_adjust *d, ci_stream_t stream) {
             ((reinterpret_cast<uintptr_t>(d->d_in) | reinterpret_cast<uintptr_t>(d->d_out)) & 15u) == 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((d->V + kChunk - 1) / kChunk, d->B);
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(kLogitThreads);
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -66,10 +66,16 @@ struct Span {
     __device__ __forceinline__ int32_t first(int32_t i) const { return (i < n_sink ? i : t_lo + i - n_sink) * TILE; }
 };
 
-// Tiles that a sequence's groups of rows are given, and the number of those groups.  One group: its own count; several:
-// no fewer than any of them has.
+// What starting on a group of rows and putting its result together costs, in tiles: lengths, queries, page ids, first keys, one
+// after the other.  Without it the blocks that get the short sequences of a batch end last (32 sequences of 1 to 16000 tokens, 251 MB:
+// 81.6 us with 0, 57.1 with 1, 51.5 with 3, 52.2 with 6).
+constexpr uint32_t kItemCost = 3;
+
+// Units of work of a sequence's groups of rows, and the number of those groups.  One group: its own tiles; several: no
+// fewer than any of them has.
 template <int RT, int TILE>
-__device__ __forceinline__ void seq_work(const PagedAttnArgs &a, const Seq &s, uint32_t &groups, uint32_t &tiles) {
+__device__ __forceinline__ void seq_work(const PagedAttnArgs &a, const Seq &s, uint32_t &groups, uint32_t &units) {
+    uint32_t tiles;
     const uint64_t rows = (uint64_t)s.q_len * a.group;
     groups = rows == 0 || rows > a.max_rows ? 0 : (uint32_t)((rows + RT - 1) / RT);
     tiles = 1;
@@ -80,6 +86,7 @@ __device__ __forceinline__ void seq_work(const PagedAttnArgs &a, const Seq &s, u
         if (a.window) n = min(n, (a.sinks + TILE - 1) / TILE + (a.window + (int32_t)((RT - 1) / a.group)) / TILE + 2);
         tiles = (uint32_t)max(n, 1);
     }
+    units = tiles + kItemCost;
 }
 
 // What a lane holds of 16 tokens: two rows of keys (tokens g and g + 8), four of values (2t, 2t+1, 2t+8, 2t+9).
@@ -109,8 +116,17 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint32_t *p) 
 
 constexpr uint32_t kNibbles = 0x000F000Fu, kBase = 0x43004300u;  // bf16 of 128 + c: the code lies in the last four mantissa bits
 
+// Two codes less 8 in bf16.  Values are summed over a whole sequence, where 128 times the sum of the weights would swamp what is
+// left of fp32 (outputs of 32000 tokens off by 0.0044 instead of 0.002); the scores' sums are short.
+__device__ __forceinline__ uint32_t centred(uint32_t w) {
+    const uint32_t x = (w & kNibbles) | kBase;
+    uint32_t y;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x43084308u));
+    return y;
+}
+
 template <int D, int BITS, int NR, int U>
-__global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR == 1 ? 3 : 2) k_paged_attention(const __grid_constant__ PagedAttnArgs a) {
     constexpr int RT = 8 * NR, SU = 16 * U, TILE = SU * kPaWarps, G = D / 64, NB = D / 64;
     __shared__ uint64_t s_scan[kPaWarps];
     __shared__ uint64_t s_base;
@@ -126,9 +142,9 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
     const uint32_t per = (p.B + kPaThreads - 1) / kPaThreads, b0 = min(threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
     uint64_t mine = 0;
     for (uint32_t b = b0; b < b1; ++b) {
-        uint32_t groups, tiles;
-        seq_work<RT, TILE>(a, load_seq(p, b), groups, tiles);
-        mine += (uint64_t)groups * tiles * p.n_kv;
+        uint32_t groups, units;
+        seq_work<RT, TILE>(a, load_seq(p, b), groups, units);
+        mine += (uint64_t)groups * units * p.n_kv;
     }
     uint64_t incl = mine;
     for (int o = 1; o < 32; o <<= 1) {
@@ -149,9 +165,9 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
     const uint64_t w0 = total * blockIdx.x / blocks, w1 = total * (blockIdx.x + 1) / blocks;
     if (before <= w0 && w0 < before + mine) {
         for (uint32_t b = b0; b < b1; ++b) {
-            uint32_t groups, tiles;
-            seq_work<RT, TILE>(a, load_seq(p, b), groups, tiles);
-            const uint64_t n = (uint64_t)groups * tiles * p.n_kv;
+            uint32_t groups, units;
+            seq_work<RT, TILE>(a, load_seq(p, b), groups, units);
+            const uint64_t n = (uint64_t)groups * units * p.n_kv;
             if (w0 < before + n) { s_b = b; s_base = before; break; }
             before += n;
         }
@@ -161,20 +177,20 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
     uint64_t base = s_base;                                     // where sequence b begins in the line
 
     for (uint64_t w = w0; w < w1;) {
-        uint32_t groups, tiles;
+        uint32_t groups, units;
         const Seq s = load_seq(p, b);
-        seq_work<RT, TILE>(a, s, groups, tiles);
-        const uint64_t seq_n = (uint64_t)groups * tiles * p.n_kv;
+        seq_work<RT, TILE>(a, s, groups, units);
+        const uint64_t seq_n = (uint64_t)groups * units * p.n_kv;
         if (w >= base + seq_n) {
             base += seq_n;
             ++b;
             continue;
         }
-        const uint32_t item = (uint32_t)((w - base) / tiles), i0 = (uint32_t)((w - base) % tiles);
-        const uint32_t i1 = (uint32_t)min((uint64_t)tiles, i0 + (w1 - w));
+        const uint32_t item = (uint32_t)((w - base) / units), u0 = (uint32_t)((w - base) % units);
+        const uint32_t u1 = (uint32_t)min((uint64_t)units, u0 + (w1 - w));
         const uint32_t kvh = item % p.n_kv, rt = item / p.n_kv, rows = (uint32_t)s.q_len * a.group;
         const Span<RT, TILE> sp(a, s, rt);
-        const int32_t n_tiles = min((int32_t)i1, sp.count);
+        const int32_t i0 = max((int32_t)u0 - (int32_t)kItemCost, 0), n_tiles = min((int32_t)u1 - (int32_t)kItemCost, sp.count);
 
         // ---- queries: the lane's channels of row 8 nr + g --------------------------------------------------------
         uint32_t qf[NR][D / 8];
@@ -225,61 +241,68 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
         }
 
         Frag<D, BITS> f[U];
-        int32_t id[U];
         auto first = [&](int32_t i) { return sp.first(i) + (int32_t)(warp * SU); };
-        auto find_pages = [&](int32_t i) {
+        // Pages of 32 tiles at once, one tile to a lane, and of the 32 after them: no tile waits for its page id.
+        auto ask_pages = [&](int32_t i, int32_t (&id)[U]) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int32_t tok = i < n_tiles ? first(i) + 16 * u : sp.hi;
-                id[u] = tok < sp.hi ? page_of(p, b, tok) : -1;
+                const int32_t mine = i + (int32_t)lane, tok = mine < n_tiles ? first(mine) + 16 * u : sp.hi;
+                id[u] = tok < sp.hi ? __ldg(p.table + (size_t)b * p.table_stride + ((uint32_t)tok >> p.page_shift)) : -1;
             }
         };
-        auto load_k = [&](int32_t i) {
+        int32_t ids[U], ids_next[U], here[U], page_base = i0;
+        uint32_t row[U];                                        // row of the pool of a tile's first token
+        auto enter = [&](int32_t i) {                           // tile i is the next to be asked for
+            if (i - page_base == 32) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) ids[u] = ids_next[u];
+                page_base = i;
+                ask_pages(i + 32, ids_next);
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const size_t row = id[u] < 0 ? 0 : row_index(p, id[u], kvh, first(i) + 16 * u);
+                const uint32_t id = (uint32_t)__shfl_sync(kFull, ids[u], i - page_base);
+                here[u] = id < p.num_pages ? 0 : -1;
+                row[u] = here[u] ? 0u : ((id * p.n_kv + kvh) << p.page_shift) + ((uint32_t)(first(i) + 16 * u) & (p.page - 1));
+            }
+        };
+        auto load_k = [&]() {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const size_t rj = row + g + 8 * j;
+                    const size_t r = (size_t)row[u] + g;
                     if constexpr (BITS == 16) {
 #pragma unroll
                         for (int x = 0; x < D / 32; ++x)
-                            f[u].k[j][x] = id[u] < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4 *>(a.k + rj * D * 2) + x * 4 + t);
-                    } else if (id[u] >= 0) {
-                        load_words(f[u].k[j], reinterpret_cast<const uint32_t *>(a.k) + rj * (D / 8) + t * 2 * G);
-                        load_words(f[u].ks[j], a.ks + rj * G);
+                            f[u].k[j][x] = __ldg(reinterpret_cast<const uint4 *>(a.k + r * D * 2) + j * D + x * 4 + t);      // (8 rows: D chunks)
+                    } else {
+                        load_words(f[u].k[j], reinterpret_cast<const uint32_t *>(a.k) + r * (D / 8) + t * 2 * G + j * D);
+                        load_words(f[u].ks[j], a.ks + r * G + j * 8 * G);
                     }
                 }
-            }
         };
-        auto load_v = [&](int32_t i) {
+        auto load_v = [&]() {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const size_t row = id[u] < 0 ? 0 : row_index(p, id[u], kvh, first(i) + 16 * u);
+                const size_t r = (size_t)row[u] + 2 * t;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const size_t rj = row + 2 * t + (j & 1) + 8 * (j >> 1);
+                    const uint32_t far = (j & 1) + 8 * (j >> 1);
                     if constexpr (BITS == 16) {
 #pragma unroll
                         for (int x = 0; x < NB; ++x)
-                            f[u].v[j][x] = id[u] < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4 *>(a.v + rj * D * 2) + x * 8 + g);
-                    } else if (id[u] >= 0) {
-                        load_words(f[u].v[j], reinterpret_cast<const uint32_t *>(a.v) + rj * (D / 8) + g * G);
-                        if (j < 2) load_words(f[u].vs[j], a.vs + (row + g + 8 * j) * G);
+                            f[u].v[j][x] = __ldg(reinterpret_cast<const uint4 *>(a.v + r * D * 2) + far * (D / 8) + x * 8 + g);
+                    } else {
+                        load_words(f[u].v[j], reinterpret_cast<const uint32_t *>(a.v) + r * (D / 8) + g * G + far * (D / 8));
+                        if (j < 2) load_words(f[u].vs[j], a.vs + ((size_t)row[u] + g + 8 * j) * G);
                     }
                 }
             }
         };
-
-        find_pages((int32_t)i0);
-        if ((int32_t)i0 < n_tiles) load_k((int32_t)i0);
-        for (int32_t i = (int32_t)i0; i < n_tiles; ++i) {
+        // One tile; all: every row sees all of it, and all of its pages are there.  Pages that are not there were read as page 0.
+        auto tile = [&](int32_t i, const bool kAll, const int32_t (&now)[U]) __attribute__((always_inline)) {
             const int32_t tok = first(i);
-            int32_t now[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) now[u] = id[u];
-            load_v(i);
-            find_pages(i + 1);                                  // the next tile's, while this one's scores are made
             // ---- scores ------------------------------------------------------------------------------------------
             float sc[U][NR][4];
 #pragma unroll
@@ -327,11 +350,8 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
                     }
                 }
             }
-            if (i + 1 < n_tiles) load_k(i + 1);
+            if (i + 1 < n_tiles) load_k();
             // ---- what is not seen, and the running maximum -------------------------------------------------------
-            bool all = tok + SU - 1 <= sp.p0 && (!a.window || tok > sp.p1 - a.window || tok + SU <= a.sinks);
-#pragma unroll
-            for (int u = 0; u < U; ++u) all &= now[u] >= 0;
             float mx[NR][2];
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) mx[nr][0] = mx[nr][1] = kNone;
@@ -342,26 +362,24 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float x = sc[u][nr][e] * a.scale_log2;
-                        if (!all) {
+                        if (!kAll) {
                             const int32_t j = tok + 16 * u + (int32_t)g + 8 * (e >> 1), i_pos = pos[nr][e & 1];
-                            const bool seen = now[u] >= 0 && j <= i_pos && (!a.window || j > i_pos - a.window || j < a.sinks);
+                            const bool seen = now[u] == 0 && j <= i_pos && j < sp.hi && (!a.window || j > i_pos - a.window || j < a.sinks);
                             x = seen ? x : kNone;
                         }
                         sc[u][nr][e] = x;
                         mx[nr][e & 1] = fmaxf(mx[nr][e & 1], x);
                     }
-            if constexpr (BITS == 16) {
-                if (!all) {                                     // 0 times what lies behind a sequence's end need not be 0
+            if constexpr (BITS == 16) if (!kAll) {                // 0 times what lies behind a sequence's end need not be 0
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int32_t at = tok + 16 * u + 2 * (int32_t)t + (j & 1) + 8 * (j >> 1);
-                            if (at >= sp.hi || (a.window && at <= sp.p0 - a.window && at >= a.sinks))
+                    for (int j = 0; j < 4; ++j) {
+                        const int32_t at = tok + 16 * u + 2 * (int32_t)t + (j & 1) + 8 * (j >> 1);
+                        if (now[u] != 0 || at >= sp.hi || (a.window && at <= sp.p0 - a.window && at >= a.sinks))
 #pragma unroll
-                                for (int x = 0; x < NB; ++x) f[u].v[j][x] = make_uint4(0, 0, 0, 0);
-                        }
-                }
+                            for (int x = 0; x < NB; ++x) f[u].v[j][x] = make_uint4(0, 0, 0, 0);
+                    }
             }
             bool grown = false;
 #pragma unroll
@@ -393,6 +411,11 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
                     }
             }
             // ---- weights and values ------------------------------------------------------------------------------
+            float ref[NR][2];
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) ref[nr][j] = !kAll && m[nr][j] == kNone ? 0.f : m[nr][j];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float pr[NR][4];
@@ -400,8 +423,7 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
                 for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float mm = m[nr][e & 1] == kNone ? 0.f : m[nr][e & 1];
-                        pr[nr][e] = ex2(sc[u][nr][e] - mm);
+                        pr[nr][e] = ex2(sc[u][nr][e] - ref[nr][e & 1]);
                         l[nr][e & 1] += pr[nr][e];
                     }
                 if constexpr (BITS == 16) {
@@ -425,39 +447,62 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
                 } else {
 #pragma unroll
                     for (int gr = 0; gr < G; ++gr) {
-                        // v = low + step c = middle + step (c - 8): the step goes with the weight; what its product loses
-                        // by rounding counts c - 8 times, and the same rounded product takes the 128 + 8 off again
+                        // v = low + step c = middle + step (c - 8): the step goes with the weight, and what its product loses by
+                        // rounding counts c - 8 times
                         uint32_t pb[NR][2];
 #pragma unroll
-                        for (int nr = 0; nr < NR; ++nr)
+                        for (int j = 0; j < 2; ++j) {
+                            const float step = lo_bf16(f[u].vs[j][gr]), middle = hi_bf16(f[u].vs[j][gr]) + 8.f * step;
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const float step = lo_bf16(f[u].vs[j][gr]), low = hi_bf16(f[u].vs[j][gr]) + 8.f * step;
+                            for (int nr = 0; nr < NR; ++nr) {
                                 const float x0 = pr[nr][2 * j], x1 = pr[nr][2 * j + 1];
                                 uint32_t y = pack_bf16(x0 * step, x1 * step);
-                                float c0 = x0 * low, c1 = x1 * low;
-                                if (!all) {                     // steps that nobody wrote: 0 times them need not be 0
-                                    if (x0 == 0.f) { y &= 0xFFFF0000u; c0 = 0.f; }
-                                    if (x1 == 0.f) { y &= 0x0000FFFFu; c1 = 0.f; }
+                                if (kAll) {
+                                    corr[nr][gr][0] += x0 * middle;
+                                    corr[nr][gr][1] += x1 * middle;
+                                } else {                        // steps that nobody wrote: 0 times them need not be 0
+                                    if (x0 == 0.f) y &= 0xFFFF0000u;
+                                    if (x1 == 0.f) y &= 0x0000FFFFu;
+                                    corr[nr][gr][0] += x0 == 0.f ? 0.f : x0 * middle;
+                                    corr[nr][gr][1] += x1 == 0.f ? 0.f : x1 * middle;
                                 }
-                                corr[nr][gr][0] += c0 - 136.f * lo_bf16(y);
-                                corr[nr][gr][1] += c1 - 136.f * hi_bf16(y);
                                 pb[nr][j] = transpose8x8(y);
                             }
+                        }
                         const uint32_t a01 = __byte_perm(f[u].v[0][gr], f[u].v[1][gr], 0x5410);
                         const uint32_t b01 = __byte_perm(f[u].v[0][gr], f[u].v[1][gr], 0x7632);
                         const uint32_t a23 = __byte_perm(f[u].v[2][gr], f[u].v[3][gr], 0x5410);
                         const uint32_t b23 = __byte_perm(f[u].v[2][gr], f[u].v[3][gr], 0x7632);
 #pragma unroll
                         for (int mm = 0; mm < 4; ++mm) {
-                            const uint32_t fa[4] = {(a01 >> 4 * mm & kNibbles) | kBase, (b01 >> 4 * mm & kNibbles) | kBase,
-                                                    (a23 >> 4 * mm & kNibbles) | kBase, (b23 >> 4 * mm & kNibbles) | kBase};
+                            const uint32_t fa[4] = {centred(a01 >> 4 * mm), centred(b01 >> 4 * mm), centred(a23 >> 4 * mm), centred(b23 >> 4 * mm)};
 #pragma unroll
                             for (int nr = 0; nr < NR; ++nr) mma_bf16(o[nr][gr][mm], fa, pb[nr][0], pb[nr][1]);
                         }
                     }
                 }
             }
+        };
+
+        if (i0 < n_tiles) {
+            ask_pages(i0, ids);
+            ask_pages(i0 + 32, ids_next);
+            enter(i0);
+            load_k();
+        }
+        for (int32_t i = i0; i < n_tiles; ++i) {
+            const int32_t tok = first(i);
+            int32_t now[U];
+            bool all = tok + SU - 1 <= sp.p0 && (!a.window || tok > sp.p1 - a.window || tok + SU <= a.sinks);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                now[u] = here[u];
+                all &= here[u] == 0;
+            }
+            load_v();
+            if (i + 1 < n_tiles) enter(i + 1);
+            if (all) tile(i, true, now);
+            else tile(i, false, now);
         }
 
         // ---- the warps' results together -------------------------------------------------------------------------
@@ -496,8 +541,8 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
                             make_float2(o[nr][x][mm][j], o[nr][x][mm][2 + j]);
             }
         __syncthreads();
-        const bool whole = i0 == 0 && i1 == tiles;
-        const uint32_t slot = blockIdx.x * 2 + (i0 == 0 ? 1 : 0);   // the part that begins an item, or one that goes on with it
+        const bool whole = u0 == 0 && u1 == units;
+        const uint32_t slot = blockIdx.x * 2 + (u0 == 0 ? 1 : 0);   // the part that begins an item, or one that goes on with it
         for (uint32_t x = threadIdx.x; x < RT * D / 4; x += kPaThreads) {
             const uint32_t r = x / (D / 4), c = x % (D / 4) * 4, row = rt * RT + r;
             float M = kNone, L = 0.f;
@@ -524,8 +569,8 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
                 if (c == 0) *reinterpret_cast<float2 *>(a.ml + ((size_t)slot * RT + r) * 2) = make_float2(M, L);
             }
         }
-        if (i0 == 0 && !whole && threadIdx.x == 0) {            // this block begins an item that others end
-            const uint64_t last = base + (uint64_t)(item + 1) * tiles - 1;
+        if (u0 == 0 && !whole && threadIdx.x == 0) {            // this block begins an item that others end
+            const uint64_t last = base + (uint64_t)(item + 1) * units - 1;
             const uint64_t owner = ((last + 1) * blocks - 1) / total;
             int32_t *d = a.desc + blockIdx.x * 8;
             d[0] = (int32_t)(owner - blockIdx.x + 1);
@@ -534,37 +579,52 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attention(const __grid_con
             d[3] = (int32_t)(rt * RT);
             d[4] = (int32_t)kvh;
         }
-        w += i1 - i0;
+        w += u1 - u0;
     }
 }
 
-// Joins the parts of an item that several blocks had: block c has the item that block c of the attention began.
+// Joins the parts of an item that several blocks had: block c has the item that block c of the attention began.  In order: the same
+// sum every time.
 template <int D, int RT>
 __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ PagedAttnArgs a) {
+    constexpr uint32_t kPer = 256 / RT;                         // threads that look for a row's maximum
+    __shared__ float s_m[RT], s_inv[RT];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int32_t *d = a.desc + blockIdx.x * 8;
-    const int32_t parts = __ldcg(d);
+    const int4 head = __ldcg(reinterpret_cast<const int4 *>(d));
+    const int32_t parts = head.x, q0 = head.y, rows = head.z, r0 = head.w;
     if (parts == 0) return;
-    const int32_t q0 = __ldcg(d + 1), rows = __ldcg(d + 2), r0 = __ldcg(d + 3), kvh = __ldcg(d + 4);
+    const int32_t kvh = __ldcg(d + 4);
+    auto slot = [&](int32_t i) { return (size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0); };
+    {
+        const uint32_t r = threadIdx.x / kPer;
+        float M = kNone, L = 0.f;
+        for (int32_t i = threadIdx.x % kPer; i < parts; i += kPer) M = fmaxf(M, __ldcg(a.ml + (slot(i) * RT + r) * 2));
+        for (uint32_t o = kPer / 2; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
+        for (int32_t i = threadIdx.x % kPer; i < parts; i += kPer) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.ml + (slot(i) * RT + r) * 2));
+            L += ml.x == kNone ? 0.f : ex2(ml.x - M) * ml.y;
+        }
+        for (uint32_t o = kPer / 2; o; o >>= 1) L += __shfl_xor_sync(kFull, L, o);
+        if (threadIdx.x % kPer == 0) {
+            s_m[r] = M == kNone ? 0.f : M;
+            s_inv[r] = M == kNone ? 0.f : 1.f / L;
+        }
+    }
+    __syncthreads();
     for (uint32_t x = threadIdx.x; x < RT * D / 4; x += 256) {
         const uint32_t r = x / (D / 4), c = x % (D / 4) * 4, row = (uint32_t)r0 + r;
         if ((int32_t)row >= rows) continue;
-        auto slot = [&](int32_t i) { return (size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0); };
-        float M = kNone;
-        for (int32_t i = 0; i < parts; ++i) M = fmaxf(M, __ldcg(a.ml + (slot(i) * RT + r) * 2));
-        const float safe = M == kNone ? 0.f : M;
-        float L = 0.f;
+        const float M = s_m[r], inv = s_inv[r];
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int32_t i = 0; i < parts; ++i) {                   // in order: the same sum every time
-            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.ml + (slot(i) * RT + r) * 2));
+#pragma unroll 8
+        for (int32_t i = 0; i < parts; ++i) {
+            const float m = __ldcg(a.ml + (slot(i) * RT + r) * 2);
             const float4 z = __ldcg(reinterpret_cast<const float4 *>(a.partial + (slot(i) * RT + r) * D + c));
-            const float e = ml.x == kNone ? 0.f : ex2(ml.x - safe);
-            L += e * ml.y;
+            const float e = m == kNone ? 0.f : ex2(m - M);
             y.x += e * z.x; y.y += e * z.y; y.z += e * z.z; y.w += e * z.w;
         }
-        const float inv = M == kNone ? 0.f : 1.f / L;
         *reinterpret_cast<uint2 *>(a.out + (int64_t)(q0 + row / a.group) * a.ldo + (size_t)(kvh * a.group + row % a.group) * D + c) =
             make_uint2(pack_bf16(y.x * inv, y.y * inv), pack_bf16(y.z * inv, y.w * inv));
     }

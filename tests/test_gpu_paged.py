@@ -458,7 +458,7 @@ def bf16_close(got, want):
 
 
 LOGITS = [(1, 1000, 5, 0, False), (3, 4097, 40, 7, True), (2, 8192, 0, 3, True), (5, 32, 100, 1, False), (2, 31, 9, 2, True),
-          (1, 1, 3, 1, True), (4, 12000, 3000, 300, True)]
+          (1, 1, 3, 1, True), (4, 12000, 3000, 300, True), (2, 16400, 50, 1100, False)]
 
 
 @pytest.mark.parametrize("B,V,L,n_bias,masked", LOGITS)
