@@ -131,7 +131,7 @@ SIGNATURES = {
     "ci_rope_paged_append": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedBatch), _V, C.c_int64, _V, C.c_int64, _V, C.c_int64,
                                        C.c_uint32, _V, _V, C.c_uint32, _V, _S]),
     "ci_paged_gather": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedBatch), _V, _V, _S]),
-    "ci_paged_attention_workspace_bytes": (C.c_size_t, [C.c_uint32]),
+    "ci_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.c_uint32, C.c_uint32]),
     "ci_paged_attention": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedBatch), _V, C.c_int64, C.c_uint32, C.c_uint32,
                                      C.c_uint32, C.c_uint32, C.c_float, _V, C.c_size_t, _V, C.c_int64, _S]),
     "ci_paged_status": (C.c_int, [u32p, C.c_int, _S]),

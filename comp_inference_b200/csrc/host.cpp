@@ -697,8 +697,10 @@ Tensor paged_attention(PagedCache &cache, const Tensor &q, const Tensor &table, 
     else y = at::empty({r.T, r.heads * d}, q.options());
     if (r.T == 0 || b.B == 0) return y;
     // of this call: from the allocator's pool of the stream, or of the graph that is being captured
-    const Tensor ws = at::empty({(int64_t)ci_paged_attention_workspace_bytes((uint32_t)d)}, q.options().dtype(at::kByte));
-    check(ci_paged_attention(cache.now(), &b, r.ptr, r.ld, (uint32_t)r.heads, (uint32_t)std::min(max_q_len, most), (uint32_t)std::min(window, most),
+    const ci_paged_cache *c = cache.now();
+    const uint32_t longest = (uint32_t)std::min(max_q_len, most);
+    const Tensor ws = at::empty({(int64_t)ci_paged_attention_workspace_bytes(c, &b, (uint32_t)r.heads, longest)}, q.options().dtype(at::kByte));
+    check(ci_paged_attention(c, &b, r.ptr, r.ld, (uint32_t)r.heads, longest, (uint32_t)std::min(window, most),
                              (uint32_t)std::min(sinks, most), (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)d)), ws.data_ptr(),
                              ws.nbytes(), (uint16_t *)y.data_ptr(), r.T > 1 ? y.stride(0) : r.heads * d, stream()));
     return y;
@@ -738,7 +740,7 @@ Tensor adjust_logits(const Tensor &logits, const OptTensor &tokens, const OptTen
     if (tokens.has_value()) {
         refuse(!lens.has_value(), "tokens need their lengths");
         a.d_tokens = (const int64_t *)rows(tokens, at::kLong, -1, "tokens", a.ld_tokens);
-        refuse(tokens->size(1) >= (1 << 30), "a history of " + shape_of(*tokens));
+        refuse(tokens->size(1) >= (1 << 20), "a history of " + shape_of(*tokens));
         a.L = (uint32_t)tokens->size(1);
         a.d_lens = (const int32_t *)each(lens, at::kInt, "lens");
         a.d_prompt_lens = (const int32_t *)each(prompt_lens, at::kInt, "prompt_lens");

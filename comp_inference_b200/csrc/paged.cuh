@@ -21,6 +21,21 @@ struct PagedBatch {
     int32_t cap;                                 // positions that a row of the table can name
 };
 
+// How the prompts' kernel (paged_prompt.cu) shares its work, made on the device by k_paged_join, which runs before it.  An item is
+// per_item tokens of a sequence for one key/value head, a block's work.  Where items are few, those with more key tiles than a
+// multiprocessor's share of all of them are cut into pieces no shorter than the share: as many pieces as there are
+// multiprocessors at most, all at once.  (Pieces no longer than the share would be up to one more for every item, and a second
+// round of blocks.)  Not shorter than kFewest either: a piece begins with queries and first keys one after the other and ends
+// with k_prompt_join.  32 tokens behind 8000 others, eight sequences of it: XXXX us, uncut YYYY.
+constexpr uint32_t kKt = 128;                // positions per key tile
+constexpr uint32_t kFewest = 4;
+struct PromptPlan {
+    uint32_t group, per_item, min_rows, sms, count, may_cut;     // min_rows: sequences with as many query rows or fewer are not in it
+    int32_t window, sinks;
+    int4 *pieces;                            // [count][2]: sequence (B: none), item, piece, pieces; slot of the item's first, q0, q_len, kv_len
+    int4 *cuts;                              // [0].x: items in several pieces (of each head); [1 + i][2]: the i-th's first piece
+};
+
 #ifdef __CUDACC__
 
 struct Seq {
@@ -67,6 +82,75 @@ __device__ __forceinline__ uint32_t seq_of(const int32_t *starts, uint32_t B, ui
     return __ldg(starts + lo) <= (int32_t)t ? lo : B;
 }
 
+// Pieces of the prompts' work into l.pieces (all l.count entries), items in several pieces into l.cuts, by `warps` whole warps of which
+// this is the first + 0, 1, ...  Lane i of each looks at the i-th share of the sequences.
+__device__ __forceinline__ void plan_prompts(const PagedBatch &p, const PromptPlan &l, uint32_t first, uint32_t warps) {
+    if (first >= l.count) return;
+    const uint32_t B = p.B, lane = lane_id(), per = (B + 31) / 32, b0 = min(lane * per, B), b1 = min(b0 + per, B);
+    // items of a sequence and the key tiles of the longest of them, or a few more
+    Seq s;
+    uint32_t items, tiles, at_b = B;
+    auto at = [&](uint32_t b) {
+        if (b == at_b) return;
+        at_b = b;
+        s = load_seq(p, b);
+        items = (uint64_t)s.q_len * l.group <= l.min_rows ? 0u : ((uint32_t)s.q_len + l.per_item - 1) / l.per_item;
+        uint32_t n = ((uint32_t)min(s.kv_len, p.cap) + kKt - 1) / kKt;
+        if (l.window) n = min(n, ((uint32_t)l.sinks + kKt - 1) / kKt + ((uint32_t)l.window + l.per_item) / kKt + 2);    // (below 2^31 each)
+        tiles = max(n, 1u);
+    };
+    float all = 0.f;
+    for (uint32_t b = b0; b < b1; ++b) {
+        at(b);
+        all += (float)items * (float)tiles;
+    }
+    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(kFull, all, o);
+    // one more than the share: sums in fp32 may be short of it by less, where anything is cut (fewer than 2^23 tiles)
+    const uint32_t most = max((uint32_t)fminf(all * (float)p.n_kv / (float)l.sms, 1e9f) + 1, kFewest);
+    uint32_t mine = 0, cut = 0;                                  // pieces; slots, and in the upper half cut items
+    for (uint32_t b = b0; b < b1; ++b) {
+        at(b);
+        const uint32_t n = max(tiles / most, 1u);
+        mine += items * n;
+        if (n > 1) cut += items * n + (items << 16);
+    }
+    uint32_t end = mine, end_cut = cut;
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(kFull, end, o), y = __shfl_up_sync(kFull, end_cut, o);
+        if (lane >= (uint32_t)o) {
+            end += x;
+            end_cut += y;
+        }
+    }
+    if (first == 0 && lane == 31) l.cuts[0] = make_int4((int32_t)(end_cut >> 16), 0, 0, 0);
+    for (uint32_t v = first; v < l.count; v += warps) {
+        const bool here = end - mine <= v && v < end;
+        if (here) {
+            uint32_t before = end - mine, slot = end_cut - cut;
+            for (uint32_t b = b0; b < b1; ++b) {
+                at(b);
+                const uint32_t n = max(tiles / most, 1u);
+                if (v < before + items * n) {
+                    const uint32_t i = (v - before) / n, piece = (v - before) % n;
+                    const int4 w0 = make_int4((int32_t)b, (int32_t)(items - 1 - i), (int32_t)piece, (int32_t)n);       // the longest first: they see the most
+                    const int4 w1 = make_int4((int32_t)((slot & 0xFFFFu) + i * n), s.q0, s.q_len, s.kv_len);
+                    l.pieces[(size_t)v * 2] = w0;
+                    l.pieces[(size_t)v * 2 + 1] = w1;
+                    if (n > 1 && piece == 0) {
+                        int4 *d = l.cuts + (1 + (size_t)(slot >> 16) + i) * 2;
+                        d[0] = w0;
+                        d[1] = w1;
+                    }
+                    break;
+                }
+                before += items * n;
+                if (n > 1) slot += items * n + (items << 16);
+            }
+        }
+        if (!__any_sync(kFull, here) && lane == 0) l.pieces[(size_t)v * 2] = make_int4((int32_t)B, 0, 0, 0);
+    }
+}
+
 __device__ __forceinline__ float lo_bf16(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_bf16(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -78,7 +162,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 #endif  // __CUDACC__
 
 int check_paged(const ci_paged_cache *c, const ci_paged_batch *b, PagedBatch &out);
-int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const uint16_t *q, int64_t ldq, uint32_t n_q, int32_t window,
-                        int32_t sinks, float scale_log2, uint32_t min_rows, uint16_t *out, int64_t ldo, cudaStream_t s);
+PromptPlan prompt_plan(uint32_t head_dim, uint32_t page_size, uint32_t n_kv, const ci_paged_batch *b, uint32_t group, int32_t window,
+                       int32_t sinks, uint32_t min_rows, void *workspace);
+size_t prompt_workspace_bytes(uint32_t head_dim, const PromptPlan &l);
+int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const PromptPlan &l, const uint16_t *q, int64_t ldq, uint32_t n_q,
+                        float scale_log2, uint16_t *out, int64_t ldo, cudaStream_t s);
 
 }  // namespace ci

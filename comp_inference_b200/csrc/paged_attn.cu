@@ -583,50 +583,106 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
     }
 }
 
-// Joins the parts of an item that several blocks had: block c has the item that block c of the attention began.  In order: the same
-// sum every time.
+// Joins the parts of an item that several blocks had: block c has the item that block c of the attention began, all rows at once, if
+// that has few parts.  Items of many parts are few, and the blocks share their rows: a block per row, its threads over the
+// parts (5 items of 59 parts, heads of 256: the join's 55 us become XXXX).  Everything in a fixed order: the same sum every time.
+constexpr int32_t kFewParts = 16;
+
 template <int D, int RT>
-__global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PromptPlan plan) {
     constexpr uint32_t kPer = 256 / RT;                         // threads that look for a row's maximum
+    constexpr uint32_t kLanes = D / 4, kShares = 256 / kLanes;  // threads of a row, and such rows of threads
     __shared__ float s_m[RT], s_inv[RT];
+    __shared__ __align__(16) float4 s_y[kShares][kLanes];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    auto slot = [&](uint32_t c, int32_t i) { return (size_t)(c + i) * 2 + (i == 0 ? 1 : 0); };
+    auto store = [&](const int4 &head, int32_t kvh, uint32_t row, uint32_t c, const float4 &y, float inv) {
+        *reinterpret_cast<uint2 *>(a.out + (int64_t)(head.y + (int32_t)(row / a.group)) * a.ldo + (size_t)(kvh * a.group + row % a.group) * D + c) =
+            make_uint2(pack_bf16(y.x * inv, y.y * inv), pack_bf16(y.z * inv, y.w * inv));
+    };
+    uint32_t rows_here = 0;                                     // of items of many parts: a bit per row
+    {
+        int32_t n[RT];
+#pragma unroll
+        for (uint32_t k = 0; k < RT; ++k) n[k] = __ldcg(a.desc + (blockIdx.x + k * gridDim.x) / RT * 8);
+#pragma unroll
+        for (uint32_t k = 0; k < RT; ++k) rows_here |= n[k] > kFewParts ? 1u << k : 0u;
+    }
+    if (plan.count) plan_prompts(a.p, plan, blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8);
     const int32_t *d = a.desc + blockIdx.x * 8;
     const int4 head = __ldcg(reinterpret_cast<const int4 *>(d));
-    const int32_t parts = head.x, q0 = head.y, rows = head.z, r0 = head.w;
-    if (parts == 0) return;
-    const int32_t kvh = __ldcg(d + 4);
-    auto slot = [&](int32_t i) { return (size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0); };
-    {
-        const uint32_t r = threadIdx.x / kPer;
-        float M = kNone, L = 0.f;
-        for (int32_t i = threadIdx.x % kPer; i < parts; i += kPer) M = fmaxf(M, __ldcg(a.ml + (slot(i) * RT + r) * 2));
-        for (uint32_t o = kPer / 2; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
-        for (int32_t i = threadIdx.x % kPer; i < parts; i += kPer) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.ml + (slot(i) * RT + r) * 2));
-            L += ml.x == kNone ? 0.f : ex2(ml.x - M) * ml.y;
+    if (head.x > 0 && head.x <= kFewParts) {
+        const int32_t parts = head.x, kvh = __ldcg(d + 4);
+        {
+            const uint32_t r = threadIdx.x / kPer;
+            float M = kNone, L = 0.f;
+            for (int32_t i = threadIdx.x % kPer; i < parts; i += kPer) M = fmaxf(M, __ldcg(a.ml + (slot(blockIdx.x, i) * RT + r) * 2));
+            for (uint32_t o = kPer / 2; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
+            for (int32_t i = threadIdx.x % kPer; i < parts; i += kPer) {
+                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.ml + (slot(blockIdx.x, i) * RT + r) * 2));
+                L += ml.x == kNone ? 0.f : ex2(ml.x - M) * ml.y;
+            }
+            for (uint32_t o = kPer / 2; o; o >>= 1) L += __shfl_xor_sync(kFull, L, o);
+            if (threadIdx.x % kPer == 0) {
+                s_m[r] = M == kNone ? 0.f : M;
+                s_inv[r] = M == kNone ? 0.f : 1.f / L;
+            }
         }
-        for (uint32_t o = kPer / 2; o; o >>= 1) L += __shfl_xor_sync(kFull, L, o);
-        if (threadIdx.x % kPer == 0) {
-            s_m[r] = M == kNone ? 0.f : M;
-            s_inv[r] = M == kNone ? 0.f : 1.f / L;
+        __syncthreads();
+        for (uint32_t x = threadIdx.x; x < RT * D / 4; x += 256) {
+            const uint32_t r = x / (D / 4), c = x % (D / 4) * 4, row = (uint32_t)head.w + r;
+            if ((int32_t)row >= head.z) continue;
+            const float M = s_m[r];
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int32_t i = 0; i < parts; ++i) {
+                const float m = __ldcg(a.ml + (slot(blockIdx.x, i) * RT + r) * 2);
+                const float4 z = __ldcg(reinterpret_cast<const float4 *>(a.partial + (slot(blockIdx.x, i) * RT + r) * D + c));
+                const float e = m == kNone ? 0.f : ex2(m - M);
+                y.x += e * z.x; y.y += e * z.y; y.z += e * z.z; y.w += e * z.w;
+            }
+            store(head, kvh, row, c, y, s_inv[r]);
         }
     }
-    __syncthreads();
-    for (uint32_t x = threadIdx.x; x < RT * D / 4; x += 256) {
-        const uint32_t r = x / (D / 4), c = x % (D / 4) * 4, row = (uint32_t)r0 + r;
-        if ((int32_t)row >= rows) continue;
-        const float M = s_m[r], inv = s_inv[r];
+    for (; rows_here; rows_here &= rows_here - 1) {
+        const uint32_t u = blockIdx.x + (__ffs(rows_here) - 1) * gridDim.x, c = u / RT, r = u % RT;
+        const int4 h = __ldcg(reinterpret_cast<const int4 *>(a.desc + c * 8));
+        const uint32_t row = (uint32_t)h.w + r;
+        if ((int32_t)row >= h.z) continue;
+        const int32_t parts = h.x, kvh = __ldcg(a.desc + c * 8 + 4);
+        const uint32_t lane = lane_id();
+        float M = kNone, L = 0.f;                               // in every warp
+#pragma unroll 4
+        for (int32_t i = lane; i < parts; i += 32) M = fmaxf(M, __ldcg(a.ml + (slot(c, i) * RT + r) * 2));
+        for (uint32_t o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
+        const float safe = M == kNone ? 0.f : M;
+#pragma unroll 4
+        for (int32_t i = lane; i < parts; i += 32) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.ml + (slot(c, i) * RT + r) * 2));
+            L += ml.x == kNone ? 0.f : ex2(ml.x - safe) * ml.y;
+        }
+        for (uint32_t o = 16; o; o >>= 1) L += __shfl_xor_sync(kFull, L, o);
+        const uint32_t at = threadIdx.x % kLanes, share = threadIdx.x / kLanes;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-        for (int32_t i = 0; i < parts; ++i) {
-            const float m = __ldcg(a.ml + (slot(i) * RT + r) * 2);
-            const float4 z = __ldcg(reinterpret_cast<const float4 *>(a.partial + (slot(i) * RT + r) * D + c));
-            const float e = m == kNone ? 0.f : ex2(m - M);
+        for (int32_t i = share; i < parts; i += kShares) {
+            const float m = __ldcg(a.ml + (slot(c, i) * RT + r) * 2);
+            const float4 z = __ldcg(reinterpret_cast<const float4 *>(a.partial + (slot(c, i) * RT + r) * D + at * 4));
+            const float e = m == kNone ? 0.f : ex2(m - safe);
             y.x += e * z.x; y.y += e * z.y; y.z += e * z.z; y.w += e * z.w;
         }
-        *reinterpret_cast<uint2 *>(a.out + (int64_t)(q0 + row / a.group) * a.ldo + (size_t)(kvh * a.group + row % a.group) * D + c) =
-            make_uint2(pack_bf16(y.x * inv, y.y * inv), pack_bf16(y.z * inv, y.w * inv));
+        __syncthreads();                                        // (the last row's are read)
+        s_y[share][at] = y;
+        __syncthreads();
+        if (threadIdx.x < kLanes) {
+#pragma unroll
+            for (uint32_t j = 1; j < kShares; ++j) {
+                const float4 z = s_y[j][at];
+                y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+            }
+            store(h, kvh, row, at * 4, y, M == kNone ? 0.f : 1.f / L);
+        }
     }
 }
 
@@ -643,7 +699,7 @@ static int resident_blocks(const void *kernel, uint32_t &blocks) {
 }
 
 template <int D, int BITS, int NR>
-static int launch_attention(const PagedAttnArgs &a, cudaStream_t s) {
+static int launch_attention(const PagedAttnArgs &a, const PromptPlan &plan, cudaStream_t s) {
     constexpr int U = BITS == 4 ? 2 : 1;
     static uint32_t resident = 0;
     if (resident == 0)
@@ -659,16 +715,28 @@ static int launch_attention(const PagedAttnArgs &a, cudaStream_t s) {
     cfg.numAttrs = 1;
     CI_CUDA(cudaLaunchKernelEx(&cfg, k_paged_attention<D, BITS, NR, U>, a));
     cfg.blockDim = dim3(256);
-    CI_CUDA(cudaLaunchKernelEx(&cfg, k_paged_join<D, 8 * NR>, a));
+    CI_CUDA(cudaLaunchKernelEx(&cfg, k_paged_join<D, 8 * NR>, a, plan));
     return CI_OK;
 }
 
 template <int D>
-static int launch_attention_bits(const PagedAttnArgs &a, uint32_t bits, bool wide, cudaStream_t s) {
+static int launch_attention_bits(const PagedAttnArgs &a, const PromptPlan &plan, uint32_t bits, bool wide, cudaStream_t s) {
     if constexpr (D <= 128) {
-        if (wide) return bits == 16 ? launch_attention<D, 16, 2>(a, s) : launch_attention<D, 4, 2>(a, s);
+        if (wide) return bits == 16 ? launch_attention<D, 16, 2>(a, plan, s) : launch_attention<D, 4, 2>(a, plan, s);
     }
-    return bits == 16 ? launch_attention<D, 16, 1>(a, s) : launch_attention<D, 4, 1>(a, s);
+    return bits == 16 ? launch_attention<D, 16, 1>(a, plan, s) : launch_attention<D, 4, 1>(a, plan, s);
+}
+
+static size_t few_bytes(uint32_t head_dim) {
+    const size_t blocks = (size_t)sm_count() * kPaMaxResident;
+    return blocks * 8 * sizeof(int32_t) + blocks * 2 * kPaMaxRows * (2 + (size_t)head_dim) * sizeof(float);
+}
+static uint64_t longest_of(const ci_paged_batch *b, uint32_t max_q_len) {
+    return b->q_starts == nullptr ? 1 : max_q_len && max_q_len < b->T ? max_q_len : b->T;
+}
+// Sequences of many new tokens go to the tensor cores' kernel, the others to this one; both look at every sequence.
+static bool has_prompts(const ci_paged_batch *b, uint32_t group, uint32_t max_q_len) {
+    return b->q_starts != nullptr && longest_of(b, max_q_len) * group > kPaRows && group <= 128;
 }
 
 }  // namespace ci
@@ -677,9 +745,12 @@ using namespace ci;
 
 extern "C" {
 
-size_t ci_paged_attention_workspace_bytes(uint32_t head_dim) {
-    const size_t blocks = (size_t)sm_count() * kPaMaxResident;
-    return blocks * 8 * sizeof(int32_t) + blocks * 2 * kPaMaxRows * (2 + (size_t)head_dim) * sizeof(float);
+size_t ci_paged_attention_workspace_bytes(const ci_paged_cache *c, const ci_paged_batch *batch, uint32_t n_q, uint32_t max_q_len) {
+    if (c == nullptr || batch == nullptr || c->n_kv == 0) return 0;
+    const size_t few = few_bytes(c->head_dim);
+    const uint32_t group = n_q / c->n_kv;
+    if (group == 0 || !has_prompts(batch, group, max_q_len)) return few;
+    return few + prompt_workspace_bytes(c->head_dim, prompt_plan(c->head_dim, c->page_size, c->n_kv, batch, group, 0, 0, kPaRows, nullptr));
 }
 
 int ci_paged_attention(const ci_paged_cache *c, const ci_paged_batch *batch, const uint16_t *d_q, int64_t ldq, uint32_t n_q,
@@ -694,8 +765,9 @@ int ci_paged_attention(const ci_paged_cache *c, const ci_paged_batch *batch, con
     CI_REQUIRE((uint64_t)a.p.T * n_q <= 0x7FFFFFFFu, "%u tokens of %u query heads", a.p.T, n_q);
     if (a.p.T == 0 || a.p.B == 0) return CI_OK;
     CI_REQUIRE(d_workspace != nullptr && (reinterpret_cast<uintptr_t>(d_workspace) & 15u) == 0, "attention needs an aligned workspace");
-    if (workspace_bytes < ci_paged_attention_workspace_bytes(c->head_dim)) {
-        set_error("attention workspace of %zu bytes, %zu needed", workspace_bytes, ci_paged_attention_workspace_bytes(c->head_dim));
+    const size_t need = ci_paged_attention_workspace_bytes(c, batch, n_q, max_q_len);
+    if (workspace_bytes < need) {
+        set_error("attention workspace of %zu bytes, %zu needed", workspace_bytes, need);
         return CI_E_WORKSPACE;
     }
     a.k = (const uint8_t *)c->k; a.v = (const uint8_t *)c->v; a.ks = c->k_scale; a.vs = c->v_scale;
@@ -713,17 +785,20 @@ int ci_paged_attention(const ci_paged_cache *c, const ci_paged_batch *batch, con
     a.desc = (int32_t *)d_workspace;
     a.ml = (float *)(a.desc + blocks * 8);
     a.partial = a.ml + blocks * 2 * kPaMaxRows * 2;
-    const uint64_t longest = batch->q_starts == nullptr ? 1 : max_q_len && max_q_len < a.p.T ? max_q_len : a.p.T;
-    // Sequences of many new tokens go to the tensor cores' kernel, the others to this one; both look at every sequence.
-    const bool prompts = batch->q_starts != nullptr && longest * a.group > kPaRows && a.group <= 128;
+    const bool prompts = has_prompts(batch, a.group, max_q_len);
     a.max_rows = prompts ? kPaRows : 0xFFFFFFFFu;
-    const bool wide = longest * a.group > 8;
+    PromptPlan plan = {};
+    if (prompts) {
+        plan = prompt_plan(c->head_dim, c->page_size, c->n_kv, batch, a.group, a.window, a.sinks, kPaRows, (uint8_t *)d_workspace + few_bytes(c->head_dim));
+        CI_REQUIRE((uint64_t)plan.count * c->n_kv <= 0x7FFFFFFFu, "too many blocks");
+    }
+    const bool wide = longest_of(batch, max_q_len) * a.group > 8;
     cudaStream_t s = (cudaStream_t)stream;
-    const int rc = c->head_dim == 64    ? launch_attention_bits<64>(a, c->bits, wide, s)
-                   : c->head_dim == 128 ? launch_attention_bits<128>(a, c->bits, wide, s)
-                                        : launch_attention_bits<256>(a, c->bits, wide, s);
+    const int rc = c->head_dim == 64    ? launch_attention_bits<64>(a, plan, c->bits, wide, s)
+                   : c->head_dim == 128 ? launch_attention_bits<128>(a, plan, c->bits, wide, s)
+                                        : launch_attention_bits<256>(a, plan, c->bits, wide, s);
     if (rc != CI_OK || !prompts) return rc;
-    return launch_paged_prompt(c, a.p, d_q, ldq, n_q, a.window, a.sinks, a.scale_log2, kPaRows, d_out, ldo, s);
+    return launch_paged_prompt(c, a.p, plan, d_q, ldq, n_q, a.scale_log2, d_out, ldo, s);
 }
 
 }  // extern "C"

@@ -26,7 +26,6 @@
 
 namespace ci {
 
-constexpr uint32_t kKt = 128;                // positions per tile
 constexpr float kLazy = 8.f;
 __device__ uint32_t g_prompt_status;         // code of a wait that ran out
 
@@ -34,11 +33,13 @@ struct PromptArgs {
     PagedBatch p;
     const uint8_t *k, *v;                    // 4 bits only
     const uint32_t *ks, *vs;
-    uint32_t n_q, group, tt, min_rows, negate;
+    uint32_t n_q, group, tt, negate;
     int32_t window, sinks;
     float scale_log2;                        // not negative
     uint16_t *out;
     int64_t ldo;
+    const int4 *plan, *cuts;                 // see PromptPlan
+    float *ml, *partial;                     // of pieces: [slots][NT 128][2], [slots][NT 128][D]
 };
 
 template <int D, int BITS>
@@ -86,6 +87,19 @@ struct KeyTiles {
     __device__ __forceinline__ bool seen_by(const QueryTile &q, int32_t i) const {
         const int32_t f = first(i);
         return q.p1 >= q.p0 && f < q.hi && (i < n_sink || f + (int32_t)kKt > q.lo);
+    }
+    // Of these tiles only those of one piece of several.  The first tokens of a window go with the first one.
+    __device__ __forceinline__ void take(uint32_t piece, uint32_t pieces) {
+        auto begin = [&](uint32_t k) {
+            const int32_t x = (int32_t)((uint64_t)n * k / pieces);
+            return x == 0 ? 0 : max(x, n_sink);
+        };
+        const int32_t i0 = begin(piece), i1 = begin(piece + 1);
+        if (i0) {
+            t_lo += i0 - n_sink;
+            n_sink = 0;
+        }
+        n = i1 - i0;
     }
 };
 
@@ -181,45 +195,18 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // ---- which sequence, which tokens -------------------------------------------------------------------------
-    const uint32_t kvh = blockIdx.x % p.n_kv, item = blockIdx.x / p.n_kv, per_item = NT * a.tt;
-    if (warp == 0) {
-        auto tiles_of = [&](uint32_t b) {
-            const Seq s = load_seq(p, b);
-            return (uint64_t)s.q_len * a.group <= a.min_rows ? 0u : ((uint32_t)s.q_len + per_item - 1) / per_item;
-        };
-        const uint32_t per = (p.B + 31) / 32, b0 = min(lane * per, p.B), b1 = min(b0 + per, p.B);
-        uint32_t mine = 0;
-        for (uint32_t b = b0; b < b1; ++b) mine += tiles_of(b);
-        uint32_t incl = mine;
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t x = __shfl_up_sync(kFull, incl, o);
-            if (lane >= (uint32_t)o) incl += x;
-        }
-        if (lane == 0) s_item[0] = p.B;
-        __syncwarp();
-        uint32_t before = incl - mine;
-        if (before <= item && item < incl)
-            for (uint32_t b = b0; b < b1; ++b) {
-                const uint32_t n = tiles_of(b);
-                if (item < before + n) {
-                    s_item[0] = b;
-                    s_item[1] = n - 1 - (item - before);        // the longest first: they see the most
-                    break;
-                }
-                before += n;
-            }
-    }
-    __syncthreads();
-    const uint32_t b = s_item[0];
+    const uint32_t kvh = blockIdx.x % p.n_kv;
+    const int4 w0 = __ldcg(a.plan + blockIdx.x / p.n_kv * 2), w1 = __ldcg(a.plan + blockIdx.x / p.n_kv * 2 + 1);
+    const uint32_t b = (uint32_t)uniform(w0.x), item = (uint32_t)uniform(w0.y);
     if (b >= p.B) return;
-    const Seq s = load_seq(p, b);
+    const Seq s = {uniform(w1.y), uniform(w1.z), uniform(w1.w)};
     QueryTile qt[NT];
     KeyTiles kt;
     kt.lo = p.cap;
     kt.hi = 0;
 #pragma unroll
     for (uint32_t t = 0; t < NT; ++t) {
-        const int32_t i0 = (int32_t)((s_item[1] * NT + t) * a.tt), n = min(max(s.q_len - i0, 0), (int32_t)a.tt);
+        const int32_t i0 = (int32_t)((item * NT + t) * a.tt), n = min(max(s.q_len - i0, 0), (int32_t)a.tt);
         qt[t].p0 = s.kv_len - s.q_len + i0;
         qt[t].p1 = qt[t].p0 + n - 1;
         qt[t].hi = n ? max(min(qt[t].p1 + 1, p.cap), 0) : 0;
@@ -233,6 +220,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     kt.t_lo = kt.lo / (int32_t)kKt;
     kt.n_sink = a.window ? min((min(a.sinks, kt.hi) + (int32_t)kKt - 1) / (int32_t)kKt, kt.t_lo) : 0;
     kt.n = kt.n_sink + (kt.hi + (int32_t)kKt - 1) / (int32_t)kKt - kt.t_lo;
+    if (w0.w > 1) kt.take((uint32_t)w0.z, (uint32_t)w0.w);
     kt.lo = uniform(kt.lo);
     kt.hi = uniform(kt.hi);
     kt.t_lo = uniform(kt.t_lo);
@@ -240,7 +228,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     kt.n = uniform(kt.n);
 #pragma unroll
     for (uint32_t t = 0; t < NT; ++t) qt[t] = {uniform(qt[t].p0), uniform(qt[t].p1), uniform(qt[t].lo), uniform(qt[t].hi)};
-    const int32_t q_row = s.q0 + (int32_t)(s_item[1] * NT * a.tt);              // first token of the block
+    const int32_t q_row = s.q0 + (int32_t)(item * NT * a.tt);              // first token of the block
 
     if (threadIdx.x == 0) {
         mbar_init(bar(Sh::bQ), 1);
@@ -258,6 +246,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         mbar_init(bar(Sh::bTurn + 1), 1);
         mbar_init(bar(Sh::bQh), 4 * NT);
         *s_abort = 0;
+        s_item[0] = (uint32_t)w0.w;                             // pieces; this one's slot: for the end
+        s_item[1] = (uint32_t)(w1.x + w0.z);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == Sh::kMma) tmem_alloc(smem_s + Sh::oBar + Sh::oTmem, 512);
@@ -474,6 +464,9 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             const bool live = tok < a.tt && pos <= q.p1;
             const float inv = m == -INFINITY ? 0.f : 1.f / l;     // (nothing seen: zeros)
             const float up = BITS == 4 ? power_of_2(v_exp / 2) : 1.f, up2 = BITS == 4 ? power_of_2(v_exp - v_exp / 2) : 1.f;
+            const uint32_t pieces = s_item[0];
+            const size_t part = ((size_t)s_item[1] * p.n_kv + kvh) * (NT * 128) + t * 128 + row;
+            if (pieces > 1 && live) *reinterpret_cast<float2 *>(a.ml + part * 2) = make_float2(m, l);
             uint16_t *dst = a.out + (int64_t)(q_row + (int32_t)(t * a.tt + tok)) * a.ldo + (size_t)(kvh * a.group + head) * D;
 #pragma unroll 1
             for (uint32_t j = 0; j < D / 32; ++j) {
@@ -484,7 +477,13 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = 0;
                 }
-                if (live) {
+                if (live && pieces > 1) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        *reinterpret_cast<float4 *>(a.partial + part * D + j * 32 + e * 4) =
+                            make_float4(__uint_as_float(o[4 * e]) * up * up2, __uint_as_float(o[4 * e + 1]) * up * up2,
+                                        __uint_as_float(o[4 * e + 2]) * up * up2, __uint_as_float(o[4 * e + 3]) * up * up2);
+                } else if (live) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         uint32_t y[4];
@@ -728,12 +727,71 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     if (warp == Sh::kMma) tmem_dealloc(tmem, 512);
 }
 
+// Joins the pieces of an item, 32 rows to a block: D / 4 threads to a row.  In order: the same sum every time.
+template <int D>
+__global__ void __launch_bounds__(256) k_prompt_join(const __grid_constant__ PromptArgs a) {
+    constexpr uint32_t NT = PromptShape<D, 16>::NT, kLanes = D / 4, kRows = 256 / kLanes;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t kvh = blockIdx.x % a.p.n_kv;
+    const int4 *d = a.cuts + (1 + blockIdx.x / a.p.n_kv) * 2;
+    const int32_t cuts = __ldcg(&a.cuts->x);
+    const int4 w0 = __ldcg(d), w1 = __ldcg(d + 1);
+    if (blockIdx.x / a.p.n_kv >= (uint32_t)cuts) return;
+    const uint32_t item = (uint32_t)w0.y, pieces = (uint32_t)w0.w, slot = (uint32_t)w1.x, q_len = (uint32_t)w1.z;
+    const int32_t q0 = w1.y;
+    for (uint32_t r = blockIdx.y * 32 + threadIdx.x / kLanes; r < blockIdx.y * 32 + 32; r += kRows) {
+        const uint32_t t = r / 128, tok = r % 128 / a.group, c = threadIdx.x % kLanes * 4;
+        const uint32_t at = (item * NT + t) * a.tt + tok;     // the row's token
+        if (tok >= a.tt || at >= q_len) continue;
+        auto part = [&](uint32_t i) { return ((size_t)(slot + i) * a.p.n_kv + kvh) * (NT * 128) + r; };
+        float M = -INFINITY, L = 0.f;
+#pragma unroll 8
+        for (uint32_t i = 0; i < pieces; ++i) M = fmaxf(M, __ldcg(a.ml + part(i) * 2));
+        const float safe = M == -INFINITY ? 0.f : M;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (uint32_t i = 0; i < pieces; ++i) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.ml + part(i) * 2));
+            const float4 z = __ldcg(reinterpret_cast<const float4 *>(a.partial + part(i) * D + c));
+            const float e = ml.x == -INFINITY ? 0.f : ex2f(ml.x - safe);
+            L += e * ml.y;
+            y.x += e * z.x; y.y += e * z.y; y.z += e * z.z; y.w += e * z.w;
+        }
+        const float inv = M == -INFINITY ? 0.f : 1.f / L;
+        *reinterpret_cast<uint2 *>(a.out + (int64_t)(q0 + (int32_t)at) * a.ldo + (size_t)(kvh * a.group + r % 128 % a.group) * D + c) =
+            make_uint2(pack_bf16(y.x * inv, y.y * inv), pack_bf16(y.z * inv, y.w * inv));
+    }
+}
+
+static size_t prompt_slot_rows(uint32_t head_dim) { return (size_t)sm_count() * (head_dim == 256 ? 128 : 256); }     // of all slots
+
+PromptPlan prompt_plan(uint32_t head_dim, uint32_t page_size, uint32_t n_kv, const ci_paged_batch *b, uint32_t group, int32_t window,
+                       int32_t sinks, uint32_t min_rows, void *workspace) {
+    PromptPlan l;
+    l.group = group;
+    l.per_item = (head_dim == 256 ? 1 : 2) * (128 / group);
+    l.min_rows = min_rows;
+    l.sms = (uint32_t)sm_count();
+    // Lengths are the device's to know: items and pieces as many as there can be, blocks without one leave at once.
+    l.may_cut = (uint64_t)b->max_pages * page_size > kFewest * kKt;
+    l.count = b->T / l.per_item + b->B + (l.may_cut ? l.sms / n_kv : 0);
+    l.window = window;
+    l.sinks = sinks;
+    l.cuts = (int4 *)workspace;
+    l.pieces = l.cuts + ((size_t)l.sms / 2 + 2) * 2;
+    return l;
+}
+size_t prompt_workspace_bytes(uint32_t head_dim, const PromptPlan &l) {
+    return (((size_t)l.sms / 2 + 2 + l.count) * 2) * sizeof(int4) + prompt_slot_rows(head_dim) * (2 + (size_t)head_dim) * sizeof(float);
+}
+
 template <int D, int BITS>
-static int launch_prompt(const PromptArgs &a, const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t s) {
+static int launch_prompt(const PromptArgs &a, const PromptPlan &l, const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t s) {
     using Sh = PromptShape<D, BITS>;
     static SmemLimit lim = {};
     if (int rc = ensure_smem_limit(lim, (const void *)k_paged_prompt<D, BITS>, Sh::kSmem)) return rc;
-    const uint64_t items = (uint64_t)a.p.T / (Sh::NT * a.tt) + a.p.B, blocks = items * a.p.n_kv;
+    const uint64_t blocks = (uint64_t)l.count * a.p.n_kv;
     CI_REQUIRE(blocks <= 0x7FFFFFFFu, "too many blocks");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
@@ -746,6 +804,11 @@ static int launch_prompt(const PromptArgs &a, const CUtensorMap &qm, const CUten
     cfg.attrs = at;
     cfg.numAttrs = 1;
     CI_CUDA(cudaLaunchKernelEx(&cfg, k_paged_prompt<D, BITS>, a, qm, km, vm));
+    if (!l.may_cut) return CI_OK;
+    cfg.gridDim = dim3(l.sms / 2 + 1, Sh::NT * 4);              // (two pieces at least to a cut item)
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    CI_CUDA(cudaLaunchKernelEx(&cfg, k_prompt_join<D>, a));
     return CI_OK;
 }
 
@@ -762,9 +825,9 @@ static int pool_map(CUtensorMap *m, const ci_paged_cache *c, void *base) {
     return CI_OK;
 }
 
-// Sequences with more than min_rows query rows per key/value head.  Needs group <= 128.
-int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const uint16_t *q, int64_t ldq, uint32_t n_q, int32_t window,
-                        int32_t sinks, float scale_log2, uint32_t min_rows, uint16_t *out, int64_t ldo, cudaStream_t s) {
+// The pieces of a plan that is there when the kernel runs.  Needs group <= 128.
+int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const PromptPlan &l, const uint16_t *q, int64_t ldq, uint32_t n_q,
+                        float scale_log2, uint16_t *out, int64_t ldo, cudaStream_t s) {
     CI_REQUIRE(encode_tiled_fn() != nullptr, "the driver has no cuTensorMapEncodeTiled");
     CI_REQUIRE(c->bits == 4 || (uint64_t)c->num_pages * c->n_kv * c->page_size <= 0x7FFFFFFFu, "a pool of more than 2^31 rows");
     PromptArgs a;
@@ -773,11 +836,14 @@ int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const uint
     a.n_q = n_q;
     a.group = n_q / c->n_kv;
     a.tt = 128 / a.group;
-    a.min_rows = min_rows;
     a.negate = scale_log2 < 0.f;
-    a.window = window; a.sinks = sinks;
+    a.window = l.window; a.sinks = l.sinks;
     a.scale_log2 = fmaxf(fabsf(scale_log2), 1e-30f);            // not 0: hidden scores are -inf before they are scaled
     a.out = out; a.ldo = ldo;
+    a.plan = l.pieces;
+    a.cuts = l.cuts;
+    a.ml = (float *)(l.pieces + (size_t)l.count * 2);
+    a.partial = a.ml + prompt_slot_rows(c->head_dim) * 2;
     CUtensorMap qm, km, vm;
     memset(&km, 0, sizeof km);
     memset(&vm, 0, sizeof vm);
@@ -794,11 +860,11 @@ int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const uint
     if (c->bits == 16) {
         if (int rc = pool_map(&km, c, c->k)) return rc;
         if (int rc = pool_map(&vm, c, c->v)) return rc;
-        return c->head_dim == 64 ? launch_prompt<64, 16>(a, qm, km, vm, s) : c->head_dim == 128 ? launch_prompt<128, 16>(a, qm, km, vm, s)
-                                                                                             : launch_prompt<256, 16>(a, qm, km, vm, s);
+        return c->head_dim == 64 ? launch_prompt<64, 16>(a, l, qm, km, vm, s) : c->head_dim == 128 ? launch_prompt<128, 16>(a, l, qm, km, vm, s)
+                                                                                             : launch_prompt<256, 16>(a, l, qm, km, vm, s);
     }
-    return c->head_dim == 64 ? launch_prompt<64, 4>(a, qm, km, vm, s) : c->head_dim == 128 ? launch_prompt<128, 4>(a, qm, km, vm, s)
-                                                                                         : launch_prompt<256, 4>(a, qm, km, vm, s);
+    return c->head_dim == 64 ? launch_prompt<64, 4>(a, l, qm, km, vm, s) : c->head_dim == 128 ? launch_prompt<128, 4>(a, l, qm, km, vm, s)
+                                                                                         : launch_prompt<256, 4>(a, l, qm, km, vm, s);
 }
 
 }  // namespace ci

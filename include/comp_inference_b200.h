@@ -440,9 +440,10 @@ int ci_paged_gather(const ci_paged_cache *cache, const ci_paged_batch *batch, ui
  * j <= i of the token's sequence (i: the token's own position) with i - j < window or j < sinks; window = 0: all j <= i.  A
  * token that sees nothing gets zeros.  q rows ldq elements apart, heads head_dim apart, both 16-byte aligned, and out alike
  * with ldo.  max_q_len: no sequence has more new tokens (0: not known; it chooses kernels, and longer ones are served all
- * the same).  d_workspace: ci_paged_attention_workspace_bytes, 16-byte aligned, its contents do not matter; calls that
+ * the same).  d_workspace: ci_paged_attention_workspace_bytes of the same arguments, 16-byte aligned, its contents do not matter; calls that
  * overlap on the GPU must not share one. */
-size_t ci_paged_attention_workspace_bytes(uint32_t head_dim);
+size_t ci_paged_attention_workspace_bytes(const ci_paged_cache *cache, const ci_paged_batch *batch, uint32_t n_q,
+                                          uint32_t max_q_len);
 int ci_paged_attention(const ci_paged_cache *cache, const ci_paged_batch *batch, const uint16_t *d_q, int64_t ldq, uint32_t n_q,
                        uint32_t max_q_len, uint32_t window, uint32_t sinks, float scale, void *d_workspace,
                        size_t workspace_bytes, uint16_t *d_out, int64_t ldo, ci_stream_t stream);
@@ -456,7 +457,7 @@ int ci_paged_status(uint32_t *code, int clear, ci_stream_t stream);
  *   + the sum of d_bias[b][i] over the i with d_bias_ids[b][i] == token;
  *   -inf for tokens whose bit (token % 32 of word token / 32 of d_mask[b]) is 0.
  * Null d_tokens, d_repetition, d_presence, d_frequency, d_mask or n_bias = 0 leaves that step out; null d_prompt_lens: all of the
- * history counts.  Token ids outside [0, V) are passed over.  No counterpart in the reference. */
+ * history counts.  Token ids outside [0, V) are passed over; L < 2^20.  No counterpart in the reference. */
 typedef struct ci_logit_adjust {
     const uint16_t *d_in;
     uint16_t *d_out;

@@ -257,6 +257,27 @@ def test_several_new_tokens(d, group, n_kv, page, new, kv, window, sinks, bits):
     assert a.shape == b.shape == (sum(new), group * n_kv * d)
 
 
+LONG = [  # few new tokens of a long sequence, whose keys are shared among the multiprocessors
+    (128, 4, 2, 64, [40, 3, 70], [5000, 900, 70], 0, 0),
+    (64, 1, 3, 128, [130], [4100], 0, 0),
+    (256, 8, 1, 32, [17, 9, 90], [3000, 20, 100], 0, 0),
+    (128, 5, 1, 16, [30] * 40, [30 + 61 * i for i in range(40)], 0, 0),
+    (64, 2, 1, 64, [150], [9000], 6000, 300),
+]
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("d,group,n_kv,page,new,kv,window,sinks", LONG)
+def test_new_tokens_of_long_sequences(d, group, n_kv, page, new, kv, window, sinks, bits):
+    g = gen(sum(kv) + d)
+    pages = sum(-(-n // page) for n in kv) + 1
+    cache, table = make_cache(g, pages, page, n_kv, d, bits), make_table(g, kv, page, pages)
+    q = (2 * rnd(g, sum(new), group * n_kv, d)).to(torch.bfloat16).to(DEV)
+    a = check_attention(q, cache, table, kv, new, window=window, sinks=sinks)
+    b = ci().paged_attention(q, cache, table.to(DEV), i32(kv), starts_of(new), max_q_len=max(new), window=window, sinks=sinks)
+    assert torch.equal(a, b)                            # the same sums every time
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 def test_more_sequences_than_threads_and_uneven_lengths(bits):
     g = gen(9)
@@ -458,7 +479,8 @@ def bf16_close(got, want):
 
 
 LOGITS = [(1, 1000, 5, 0, False), (3, 4097, 40, 7, True), (2, 8192, 0, 3, True), (5, 32, 100, 1, False), (2, 31, 9, 2, True),
-          (1, 1, 3, 1, True), (4, 12000, 3000, 300, True), (2, 16400, 50, 1100, False)]
+          (1, 1, 3, 1, True), (4, 12000, 3000, 300, True), (2, 16400, 50, 1100, False),
+          (3, 2051, 10, 40, True), (2, 100003, 700, 512, True), (64, 20011, 30, 5, True)]
 
 
 @pytest.mark.parametrize("B,V,L,n_bias,masked", LOGITS)
@@ -489,6 +511,30 @@ def test_adjust_logits(B, V, L, n_bias, masked):
         a = ci().adjust_logits(dev[0], **{n: dev[i] for n, i in kw.items()})
         names = {"tokens": "tok"}
         assert bf16_close(a, ref.adjust(logits, **{names.get(n, n): host[i] for n, i in kw.items()}))
+
+
+@pytest.mark.parametrize("shift", range(8))
+def test_adjust_logits_wherever_rows_start(shift):
+    """Rows that start on every even address of a 16-byte word, the output on another."""
+    g = gen(shift)
+    V, ld = 2100 + shift, 2200 + 3 * shift
+    room = torch.full((3 * ld + 16,), 9.0, dtype=torch.bfloat16, device=DEV)
+    x = room[shift:shift + 3 * ld].view(3, ld)[:, :V]
+    x.copy_((4 * rnd(g, 3, V)).to(torch.bfloat16))
+    tok = torch.randint(0, V, (3, 20), generator=g)
+    tok[:, :4] = torch.tensor([0, V - 1, -1, V])
+    lens, mask = torch.full((3,), 20, dtype=torch.int32), torch.randint(-2 ** 31, 2 ** 31, (3, -(-V // 32)), generator=g).to(torch.int32)
+    f = torch.rand(3, generator=g)
+    want = ref.adjust(x.cpu(), tok, lens, frequency=f, mask=mask)
+    args = dict(tokens=tok.to(DEV), lens=lens.to(DEV), frequency=f.to(DEV), mask=mask.to(DEV))
+    assert bf16_close(ci().adjust_logits(x, **args), want)
+    other = torch.full((3 * (V + 5) + 16,), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = other[3:3 + 3 * (V + 5)].view(3, V + 5)[:, 2:2 + V]
+    assert bf16_close(ci().adjust_logits(x, out=out, **args), want)
+    ci().adjust_logits(x, out=x, **args)
+    assert bf16_close(x, want)
+    assert bool((room[:shift] == 9).all()) and bool((room[shift:shift + 3 * ld].view(3, ld)[:, V:] == 9).all())
+    assert bool((other[3:3 + 3 * (V + 5)].view(3, V + 5)[:, :2] == 7).all()) and bool((other[3:3 + 3 * (V + 5)].view(3, V + 5)[:, 2 + V:] == 7).all())
 
 
 def test_adjust_logits_of_strided_rows_and_extremes():
