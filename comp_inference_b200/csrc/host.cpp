@@ -503,9 +503,11 @@ PyObject *linear_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
 // ---- serving over a paged cache --------------------------------------------------------------------------
 // Shapes and types first, the device last: what is wrong with a call shows without one.
 
-void refuse(bool wrong, const std::string &what) {
-    if (wrong) throw py::value_error(what);
-}
+// (a macro: the message is made where it is needed, not in every call)
+#define REFUSE(wrong, ...)                                      \
+    do {                                                        \
+        if (wrong) throw py::value_error(__VA_ARGS__);          \
+    } while (0)
 std::string shape_of(const Tensor &t) {
     std::ostringstream o;
     o << t.sizes();
@@ -529,21 +531,21 @@ struct PagedCache {
         const bool four = k.scalar_type() == at::kByte;
         TORCH_CHECK(four || k.scalar_type() == at::kBFloat16, "pages must be bfloat16, or uint8 for codes of 4 bits, got torch.", k.scalar_type());
         want(v, k.scalar_type(), "pages of values");
-        refuse(k.dim() != 4 || k.sizes() != v.sizes(), "pages must be two tensors [num_pages, n_kv, page_size, row], got " + shape_of(k) + " and " + shape_of(v));
-        refuse(!k.is_contiguous() || !v.is_contiguous(), "pages must be contiguous");
+        REFUSE(k.dim() != 4 || k.sizes() != v.sizes(), "pages must be two tensors [num_pages, n_kv, page_size, row], got " + shape_of(k) + " and " + shape_of(v));
+        REFUSE(!k.is_contiguous() || !v.is_contiguous(), "pages must be contiguous");
         const int64_t d = k.size(3) * (four ? 2 : 1);
-        refuse(d != 64 && d != 128 && d != 256, "head dimension " + std::to_string(d) + " must be 64, 128 or 256");
+        REFUSE(d != 64 && d != 128 && d != 256, "head dimension " + std::to_string(d) + " must be 64, 128 or 256");
         const int64_t page = k.size(2);
-        refuse(page != 16 && page != 32 && page != 64 && page != 128, "pages of " + std::to_string(page) + " tokens; 16, 32, 64 or 128");
-        refuse(k.size(0) < 1 || k.size(0) > 0x7FFFFFFF || k.size(1) < 1 || k.size(1) > 65535, "a cache of " + shape_of(k));
-        refuse(four != (ks.has_value() && vs.has_value()) || ks.has_value() != vs.has_value(), "a cache of 4 bits, and no other, has two tensors of steps and lowest values");
+        REFUSE(page != 16 && page != 32 && page != 64 && page != 128, "pages of " + std::to_string(page) + " tokens; 16, 32, 64 or 128");
+        REFUSE(k.size(0) < 1 || k.size(0) > 0x7FFFFFFF || k.size(1) < 1 || k.size(1) > 65535, "a cache of " + shape_of(k));
+        REFUSE(four != (ks.has_value() && vs.has_value()) || ks.has_value() != vs.has_value(), "a cache of 4 bits, and no other, has two tensors of steps and lowest values");
         if (four) {
             k_scale = *ks;
             v_scale = *vs;
             want(k_scale, at::kBFloat16, "steps and lowest values");
             want(v_scale, at::kBFloat16, "steps and lowest values");
             const std::vector<int64_t> s{k.size(0), k.size(1), page, d / 64, 2};
-            refuse(k_scale.sizes() != at::IntArrayRef(s) || v_scale.sizes() != at::IntArrayRef(s) || !k_scale.is_contiguous() || !v_scale.is_contiguous(),
+            REFUSE(k_scale.sizes() != at::IntArrayRef(s) || v_scale.sizes() != at::IntArrayRef(s) || !k_scale.is_contiguous() || !v_scale.is_contiguous(),
                    "steps and lowest values must be contiguous [num_pages, n_kv, page_size, head_dim / 64, 2], got " + shape_of(k_scale) + " and " + shape_of(v_scale));
         }
         require_cuda(k, "pages");
@@ -562,13 +564,13 @@ struct PagedCache {
         c.n_kv = (uint32_t)k.size(1);
         c.head_dim = (uint32_t)d;
         c.bits = four ? 4 : 16;
-        for (const Tensor *t : {&k, &v, &k_scale, &v_scale}) refuse(t->defined() && !aligned16(*t), "pages must be 16-byte aligned");
+        for (const Tensor *t : {&k, &v, &k_scale, &v_scale}) REFUSE(t->defined() && !aligned16(*t), "pages must be 16-byte aligned");
         bytes = k.nbytes();
         scale_bytes = four ? k_scale.nbytes() : 0;
     }
     // A tensor may have been given other memory since (resize_, .data): the kernels go by what it has now.
     const ci_paged_cache *now() {
-        refuse((size_t)k.nbytes() != bytes || (size_t)v.nbytes() != bytes || (k_scale.defined() && ((size_t)k_scale.nbytes() != scale_bytes || (size_t)v_scale.nbytes() != scale_bytes)),
+        REFUSE((size_t)k.nbytes() != bytes || (size_t)v.nbytes() != bytes || (k_scale.defined() && ((size_t)k_scale.nbytes() != scale_bytes || (size_t)v_scale.nbytes() != scale_bytes)),
                "the pages have another size than when the cache was made");
         c.k = k.data_ptr();
         c.v = v.data_ptr();
@@ -586,17 +588,17 @@ private:
 ci_paged_batch paged_batch(const PagedCache &cache, const Tensor &table, const Tensor &kv_lens, const OptTensor &q_starts, int64_t T) {
     want(table, at::kInt, "block_table");
     want(kv_lens, at::kInt, "kv_lens");
-    refuse(table.dim() != 2 || (table.size(1) > 1 && table.stride(1) != 1), "block_table must be [sequences, pages] with unit inner stride");
+    REFUSE(table.dim() != 2 || (table.size(1) > 1 && table.stride(1) != 1), "block_table must be [sequences, pages] with unit inner stride");
     const int64_t B = table.size(0);
-    refuse(kv_lens.dim() != 1 || kv_lens.size(0) != B || (B > 1 && kv_lens.stride(0) != 1), "kv_lens must have one entry for each of " + std::to_string(B) + " sequences");
+    REFUSE(kv_lens.dim() != 1 || kv_lens.size(0) != B || (B > 1 && kv_lens.stride(0) != 1), "kv_lens must have one entry for each of " + std::to_string(B) + " sequences");
     const int64_t stride = B > 1 ? table.stride(0) : table.size(1);
-    refuse(B > (1 << 20) || T > (1 << 30), "too many sequences or tokens");
-    refuse(stride < table.size(1) || stride > 0x7FFFFFFF || table.size(1) * (int64_t)cache.c.page_size > (1 << 30), "a block table of " + shape_of(table));
+    REFUSE(B > (1 << 20) || T > (1 << 30), "too many sequences or tokens");
+    REFUSE(stride < table.size(1) || stride > 0x7FFFFFFF || table.size(1) * (int64_t)cache.c.page_size > (1 << 30), "a block table of " + shape_of(table));
     if (q_starts.has_value()) {
         want(*q_starts, at::kInt, "q_starts");
-        refuse(q_starts->dim() != 1 || q_starts->size(0) != B + 1 || q_starts->stride(0) != 1, "q_starts must have " + std::to_string(B + 1) + " entries");
+        REFUSE(q_starts->dim() != 1 || q_starts->size(0) != B + 1 || q_starts->stride(0) != 1, "q_starts must have " + std::to_string(B + 1) + " entries");
     } else {
-        refuse(T != B, std::to_string(T) + " tokens for " + std::to_string(B) + " sequences: q_starts says which are whose");
+        REFUSE(T != B, std::to_string(T) + " tokens for " + std::to_string(B) + " sequences: q_starts says which are whose");
     }
     same_device(table, cache.k, "block_table");
     same_device(kv_lens, cache.k, "kv_lens");
@@ -621,12 +623,12 @@ struct HeadRows {
 };
 HeadRows head_rows(const Tensor &x, int64_t d, const char *name, bool align) {
     want(x, at::kBFloat16, name);
-    refuse(x.dim() < 2 || x.dim() > 3 || (x.dim() == 3 ? x.size(2) != d : x.size(1) % d != 0),
+    REFUSE(x.dim() < 2 || x.dim() > 3 || (x.dim() == 3 ? x.size(2) != d : x.size(1) % d != 0),
            std::string(name) + " must be [tokens, heads, " + std::to_string(d) + "] or [tokens, heads * " + std::to_string(d) + "], got " + shape_of(x));
     HeadRows r;
     r.T = x.size(0);
     r.heads = x.dim() == 3 ? x.size(1) : x.size(1) / d;
-    refuse(r.heads < 1 || r.heads > 65535, std::string(name) + " has " + std::to_string(r.heads) + " heads");
+    REFUSE(r.heads < 1 || r.heads > 65535, std::string(name) + " has " + std::to_string(r.heads) + " heads");
     const bool side_by_side = x.stride(-1) == 1 && (x.dim() == 2 || x.size(1) == 1 || x.stride(1) == d);
     // rows that overlap (an expanded tensor) are copied too
     const bool rows = r.T <= 1 || x.stride(0) >= r.heads * d;
@@ -642,17 +644,17 @@ Tensor paged_append(PagedCache &cache, const Tensor &q, const Tensor &k, const T
                     const Tensor &table, const Tensor &kv_lens, const OptTensor &q_starts, const OptTensor &out) {
     const int64_t d = cache.c.head_dim, n_kv = cache.c.n_kv;
     const HeadRows rq = head_rows(q, d, "q", false), rk = head_rows(k, d, "k", false), rv = head_rows(v, d, "v", false);
-    refuse(rk.T != rq.T || rv.T != rq.T, "q, k and v have " + std::to_string(rq.T) + ", " + std::to_string(rk.T) + " and " + std::to_string(rv.T) + " tokens");
-    refuse(rk.heads != n_kv || rv.heads != n_kv, "k and v have " + std::to_string(rk.heads) + " and " + std::to_string(rv.heads) + " heads, the cache " + std::to_string(n_kv));
+    REFUSE(rk.T != rq.T || rv.T != rq.T, "q, k and v have " + std::to_string(rq.T) + ", " + std::to_string(rk.T) + " and " + std::to_string(rv.T) + " tokens");
+    REFUSE(rk.heads != n_kv || rv.heads != n_kv, "k and v have " + std::to_string(rk.heads) + " and " + std::to_string(rv.heads) + " heads, the cache " + std::to_string(n_kv));
     want(cos, at::kBFloat16, "cos");
     want(sin, at::kBFloat16, "sin");
-    refuse(cos.dim() != 2 || cos.size(1) != d || cos.sizes() != sin.sizes() || !cos.is_contiguous() || !sin.is_contiguous() || cos.size(0) > 0x7FFFFFFF,
+    REFUSE(cos.dim() != 2 || cos.size(1) != d || cos.sizes() != sin.sizes() || !cos.is_contiguous() || !sin.is_contiguous() || cos.size(0) > 0x7FFFFFFF,
            "cos and sin must be contiguous tables [positions, " + std::to_string(d) + "]");
     Tensor y;
     if (out.has_value()) {
         y = *out;
         want(y, at::kBFloat16, "out");
-        refuse(y.numel() != rq.T * rq.heads * d || !y.is_contiguous() || !aligned16(y), "out must be a contiguous, 16-byte aligned tensor of the size of q");
+        REFUSE(y.numel() != rq.T * rq.heads * d || !y.is_contiguous() || !aligned16(y), "out must be a contiguous, 16-byte aligned tensor of the size of q");
     }
     const ci_paged_batch b = paged_batch(cache, table, kv_lens, q_starts, rq.T);
     for (const Tensor *t : {&q, &k, &v, &cos, &sin}) same_device(*t, cache.k, "an argument");
@@ -666,7 +668,7 @@ Tensor paged_append(PagedCache &cache, const Tensor &q, const Tensor &k, const T
 }
 
 py::tuple paged_gather(PagedCache &cache, const Tensor &table, const Tensor &kv_lens, const OptTensor &starts, int64_t total) {
-    refuse(total < 0, "a negative number of rows");
+    REFUSE(total < 0, "a negative number of rows");
     const ci_paged_batch b = paged_batch(cache, table, kv_lens, starts, total);
     const c10::cuda::CUDAGuard guard(cache.k.device());
     const auto options = cache.k.options().dtype(at::kBFloat16);
@@ -679,15 +681,15 @@ Tensor paged_attention(PagedCache &cache, const Tensor &q, const Tensor &table, 
                        int64_t max_q_len, int64_t window, int64_t sinks, std::optional<double> scale, const OptTensor &out) {
     const int64_t d = cache.c.head_dim;
     const HeadRows r = head_rows(q, d, "q", true);
-    refuse(r.heads % cache.c.n_kv != 0, std::to_string(r.heads) + " query heads over " + std::to_string(cache.c.n_kv) + " key/value heads");
-    refuse(window < 0 || sinks < 0 || max_q_len < 0, "window, sinks and max_q_len must not be negative");
+    REFUSE(r.heads % cache.c.n_kv != 0, std::to_string(r.heads) + " query heads over " + std::to_string(cache.c.n_kv) + " key/value heads");
+    REFUSE(window < 0 || sinks < 0 || max_q_len < 0, "window, sinks and max_q_len must not be negative");
     constexpr int64_t most = 0x7FFFFFFF;
-    refuse(r.T * r.heads > most, std::to_string(r.T) + " tokens of " + std::to_string(r.heads) + " heads");
+    REFUSE(r.T * r.heads > most, std::to_string(r.T) + " tokens of " + std::to_string(r.heads) + " heads");
     Tensor y;
     if (out.has_value()) {
         y = *out;
         want(y, at::kBFloat16, "out");
-        refuse(y.dim() != 2 || y.size(0) != r.T || y.size(1) != r.heads * d || (r.T && y.stride(1) != 1) || (r.T > 1 && (y.stride(0) % 8 || y.stride(0) < r.heads * d)) || !aligned16(y),
+        REFUSE(y.dim() != 2 || y.size(0) != r.T || y.size(1) != r.heads * d || (r.T && y.stride(1) != 1) || (r.T > 1 && (y.stride(0) % 8 || y.stride(0) < r.heads * d)) || !aligned16(y),
                "out must be [tokens, heads * head_dim] with 16-byte aligned rows");
     }
     const ci_paged_batch b = paged_batch(cache, table, kv_lens, q_starts, r.T);
@@ -710,7 +712,7 @@ Tensor adjust_logits(const Tensor &logits, const OptTensor &tokens, const OptTen
                      const OptTensor &presence, const OptTensor &frequency, const OptTensor &bias_ids, const OptTensor &bias,
                      const OptTensor &mask, const OptTensor &out) {
     want(logits, at::kBFloat16, "logits");
-    refuse(logits.dim() != 2 || logits.size(1) < 1 || logits.size(1) > 0x7FFFFFFF || logits.size(0) > 65535 || logits.stride(1) != 1 ||
+    REFUSE(logits.dim() != 2 || logits.size(1) < 1 || logits.size(1) > 0x7FFFFFFF || logits.size(0) > 65535 || logits.stride(1) != 1 ||
                (logits.size(0) > 1 && logits.stride(0) < logits.size(1)),
            "logits must be [sequences, vocabulary] with unit inner stride, got " + shape_of(logits));
     const int64_t B = logits.size(0), V = logits.size(1);
@@ -721,26 +723,26 @@ Tensor adjust_logits(const Tensor &logits, const OptTensor &tokens, const OptTen
     std::vector<std::pair<const Tensor *, const char *>> given;
     auto rows = [&](const OptTensor &t, at::ScalarType type, int64_t cols, const char *name, int64_t &ld) -> const void * {
         want(*t, type, name);
-        refuse(t->dim() != 2 || t->size(0) != B || (cols >= 0 && t->size(1) < cols) || (t->size(1) > 1 && t->stride(1) != 1),
+        REFUSE(t->dim() != 2 || t->size(0) != B || (cols >= 0 && t->size(1) < cols) || (t->size(1) > 1 && t->stride(1) != 1),
                std::string(name) + " must have a row for each of " + std::to_string(B) + " sequences" + (cols > 0 ? ", of " + std::to_string(cols) + " entries" : "") + ", got " + shape_of(*t));
         ld = B > 1 ? t->stride(0) : t->size(1);
-        refuse(ld < t->size(1), std::string(name) + " has rows that overlap");
+        REFUSE(ld < t->size(1), std::string(name) + " has rows that overlap");
         given.emplace_back(&*t, name);
         return t->data_ptr();
     };
     auto each = [&](const OptTensor &t, at::ScalarType type, const char *name) -> const void * {
         if (!t.has_value()) return nullptr;
         want(*t, type, name);
-        refuse(t->dim() != 1 || t->size(0) != B || (B > 1 && t->stride(0) != 1), std::string(name) + " must have one entry for each of " + std::to_string(B) + " sequences");
+        REFUSE(t->dim() != 1 || t->size(0) != B || (B > 1 && t->stride(0) != 1), std::string(name) + " must have one entry for each of " + std::to_string(B) + " sequences");
         given.emplace_back(&*t, name);
         return t->data_ptr();
     };
-    refuse(!tokens.has_value() && (lens.has_value() || prompt_lens.has_value() || repetition.has_value() || presence.has_value() || frequency.has_value()),
+    REFUSE(!tokens.has_value() && (lens.has_value() || prompt_lens.has_value() || repetition.has_value() || presence.has_value() || frequency.has_value()),
            "penalties need the tokens that have been");
     if (tokens.has_value()) {
-        refuse(!lens.has_value(), "tokens need their lengths");
+        REFUSE(!lens.has_value(), "tokens need their lengths");
         a.d_tokens = (const int64_t *)rows(tokens, at::kLong, -1, "tokens", a.ld_tokens);
-        refuse(tokens->size(1) >= (1 << 20), "a history of " + shape_of(*tokens));
+        REFUSE(tokens->size(1) >= (1 << 20), "a history of " + shape_of(*tokens));
         a.L = (uint32_t)tokens->size(1);
         a.d_lens = (const int32_t *)each(lens, at::kInt, "lens");
         a.d_prompt_lens = (const int32_t *)each(prompt_lens, at::kInt, "prompt_lens");
@@ -748,12 +750,12 @@ Tensor adjust_logits(const Tensor &logits, const OptTensor &tokens, const OptTen
         a.d_presence = (const float *)each(presence, at::kFloat, "presence");
         a.d_frequency = (const float *)each(frequency, at::kFloat, "frequency");
     }
-    refuse(bias_ids.has_value() != bias.has_value(), "biases need their tokens, and the tokens their biases");
+    REFUSE(bias_ids.has_value() != bias.has_value(), "biases need their tokens, and the tokens their biases");
     if (bias.has_value()) {
         int64_t ld = 0;
         a.d_bias_ids = (const int64_t *)rows(bias_ids, at::kLong, -1, "bias_ids", a.ld_bias);
         a.d_bias = (const float *)rows(bias, at::kFloat, -1, "bias", ld);
-        refuse(bias->sizes() != bias_ids->sizes() || (B > 1 && ld != a.ld_bias) || bias->size(1) > 0x7FFFFFFF, "bias and bias_ids must be laid out alike");
+        REFUSE(bias->sizes() != bias_ids->sizes() || (B > 1 && ld != a.ld_bias) || bias->size(1) > 0x7FFFFFFF, "bias and bias_ids must be laid out alike");
         a.n_bias = (uint32_t)bias->size(1);
     }
     if (mask.has_value()) a.d_mask = (const uint32_t *)rows(mask, at::kInt, (V + 31) / 32, "mask", a.ld_mask);
@@ -761,7 +763,7 @@ Tensor adjust_logits(const Tensor &logits, const OptTensor &tokens, const OptTen
     if (out.has_value()) {
         y = *out;
         want(y, at::kBFloat16, "out");
-        refuse(y.sizes() != logits.sizes() || y.stride(1) != 1 || (B > 1 && y.stride(0) < V), "out must be like logits, with unit inner stride");
+        REFUSE(y.sizes() != logits.sizes() || y.stride(1) != 1 || (B > 1 && y.stride(0) < V), "out must be like logits, with unit inner stride");
     }
     require_cuda(logits, "logits");
     for (const auto &g : given) same_device(*g.first, logits, g.second);

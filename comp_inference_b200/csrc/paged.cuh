@@ -33,7 +33,7 @@ struct PromptPlan {
     uint32_t group, per_item, min_rows, sms, count, may_cut;     // min_rows: sequences with as many query rows or fewer are not in it
     int32_t window, sinks;
     int4 *pieces;                            // [count][2]: sequence (B: none), item, piece, pieces; slot of the item's first, q0, q_len, kv_len
-    int4 *cuts;                              // [0].x: items in several pieces (of each head); [1 + i][2]: the i-th's first piece
+    int4 *cuts;                              // [0]: items in several pieces (of each head), 0: blocks count on; [1 + i][2]: the i-th's first piece
 };
 
 #ifdef __CUDACC__

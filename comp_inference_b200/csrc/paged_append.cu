@@ -112,7 +112,7 @@ struct TokenPart {
 // lie in eight lanes (four of them, both halves, for D = 64).  Two rounds of heads are in flight.  8000 tokens of 32 + 8 + 8
 // heads of 128: YYYY.
 template <int D, int BITS>
-__global__ void __launch_bounds__(256) k_rope_append(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(256, BITS == 16 ? 4 : 3) k_rope_append(const __grid_constant__ AppendArgs a) {
     constexpr uint32_t LANES = D / 16, G = D / kGroup, PER = 32 / LANES, FLIGHT = 2;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -263,7 +263,11 @@ __global__ void __launch_bounds__(256) k_paged_gather(const __grid_constant__ Ga
                 const float step = lo_bf16(sc), low = hi_bf16(sc);
                 float f[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = step * (float)(w >> (4 * (i / 2) + 16 * (i % 2)) & 15u) + low;   // the product is exact
+                for (int i = 0; i < 8; ++i) {                   // the code where it lies in the mantissa of 2^23, and the step by as much less
+                    const int at = 4 * (i / 2);
+                    const float c = __uint_as_float(((i % 2 ? w >> 16 : w) & 15u << at) | 0x4B000000u) - 8388608.f;
+                    f[i] = step * (1.f / (1 << at)) * c + low;  // all exact but the sum
+                }
                 o = pack(f);
             }
         }

@@ -39,8 +39,12 @@ struct PromptArgs {
     uint16_t *out;
     int64_t ldo;
     const int4 *plan, *cuts;                 // see PromptPlan
+    int32_t *next;                           // the first piece that no block has yet
+    uint32_t count;                          // pieces and places for them, each for every head
     float *ml, *partial;                     // of pieces: [slots][NT 128][2], [slots][NT 128][D]
 };
+
+constexpr uint32_t kItemWords = 20;          // of a piece in shared memory: PieceWords
 
 template <int D, int BITS>
 struct PromptShape {
@@ -49,23 +53,24 @@ struct PromptShape {
     static constexpr uint32_t NS = D == 64 ? 6 : D == 128 ? 4 : 2;           // ring of K and V tiles
     static constexpr uint32_t SPLIT = BITS == 4 && D > 64 ? 2 : 1;           // threads that share a position's codes
     static constexpr uint32_t PW = BITS == 16 ? 1 : 4 * SPLIT;               // producer warps
-    static constexpr uint32_t kProd = 4 * NT, kMma = kProd + PW;
+    static constexpr uint32_t kProd = 4 * NT, kMma = kProd + PW, kSched = kMma + NT;
     // Whole warpgroups (but where nothing is gained), so that registers can go where the scores are held: setmaxnreg takes them
     // up or down from what the block is launched with, within its sum.
     static constexpr bool kMove = NT == 2 || BITS == 4;
-    static constexpr uint32_t kWarps = kMove ? (kMma + NT + 3) / 4 * 4 : kMma + NT, kThreads = kWarps * 32;
+    static constexpr uint32_t kWarps = kMove ? (kSched + 4) / 4 * 4 : kSched + 1, kThreads = kWarps * 32;
     static constexpr uint32_t kLaunchRegs = 65536 / kThreads / 8 * 8;
     static constexpr uint32_t kSoftRegs = BITS == 16 ? 200 : D == 64 ? 160 : D == 128 ? 152 : 176;
     static constexpr uint32_t kProdRegs = BITS == 16 ? 104 : D == 64 ? 120 : D == 128 ? 64 : 104;
     static constexpr uint32_t kMmaRegs = BITS == 16 ? kProdRegs : D == 64 ? 72 : D == 128 ? 48 : 112;
     static_assert(!kMove || (kSoftRegs >= kLaunchRegs && kProdRegs <= kLaunchRegs && kMmaRegs <= kLaunchRegs &&
                              NT * 128 * kSoftRegs + (BITS == 16 ? 128 * kProdRegs : PW * 32 * kProdRegs + 128 * kMmaRegs) <= kThreads * kLaunchRegs), "registers");
-    static constexpr uint32_t oQ = 0, oRing = NT * kTile, oBar = oRing + NS * kTile, kSmem = oBar + 384 + 1024;
+    static constexpr uint32_t oQ = 0, oRing = NT * kTile, oBar = oRing + NS * kTile, kMisc = 640, kSmem = oBar + kMisc + 1024;
     // barriers
-    static constexpr uint32_t bQ = 0, bFull = 1, bEmpty = bFull + NS, bS = bEmpty + NS, bP = bS + NT, bO = bP + 2 * NT, bTurn = bO + 1, bQh = bTurn + 2;
-    static constexpr uint32_t oTmem = (bQh + 1) * 8, oAbort = oTmem + 4, oItem = oTmem + 8;
-    static constexpr uint32_t oScale = oItem + 8, oLargest = oScale + 64;    // 4 bits: exponents of eight tiles' K and V; of warps
-    static_assert(oLargest + 64 <= 384, "barrier region");
+    static constexpr uint32_t bQ = 0, bFull = 1, bEmpty = bFull + NS, bS = bEmpty + NS, bP = bS + NT, bO = bP + 2 * NT, bRead = bO + NT, bTurn = bRead + NT,
+                              bQh = bTurn + 2, bQfree = bQh + 1, bItem = bQfree + 1, bTaken = bItem + 2, bEnd = bTaken + 2;
+    static constexpr uint32_t oTmem = (bEnd + 1) * 8, oAbort = oTmem + 4, oItem = oTmem + 8;
+    static constexpr uint32_t oScale = oItem + 2 * kItemWords * 4, oLargest = oScale + 64;   // 4 bits: exponents of eight tiles' K and V; of warps
+    static_assert(oLargest + 64 <= kMisc, "barrier region");
     static constexpr int kHeld = BITS == 16 ? 4 : 2;                         // groups of 32 scores that a row's thread holds
     static constexpr uint32_t cO = NT * kKt;                                 // first column of O
 };
@@ -102,6 +107,10 @@ struct KeyTiles {
         n = i1 - i0;
     }
 };
+
+// A piece as the scheduling warp hands it to the others; sequence < 0: there is no more.
+enum PieceWords : uint32_t { kSequence, kHead, kFirstRow, kPieces, kSlot, kTilesAt, kQueriesAt = kTilesAt + 5 };
+static_assert(kQueriesAt + 8 <= kItemWords, "room for two query tiles");
 
 // The same in every lane: said to the compiler, which then forms what depends on it in uniform registers.
 __device__ __forceinline__ int32_t uniform(int32_t v) { return __shfl_sync(kFull, v, 0); }
@@ -189,46 +198,10 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     auto bar = [&](uint32_t i) { return smem_s + Sh::oBar + i * 8; };
     volatile uint32_t *s_tmem = reinterpret_cast<volatile uint32_t *>(smem + Sh::oBar + Sh::oTmem);
     volatile uint32_t *s_abort = reinterpret_cast<volatile uint32_t *>(smem + Sh::oBar + Sh::oAbort);
-    volatile uint32_t *s_item = reinterpret_cast<volatile uint32_t *>(smem + Sh::oBar + Sh::oItem);
+    volatile int32_t *s_items = reinterpret_cast<volatile int32_t *>(smem + Sh::oBar + Sh::oItem);
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-    // ---- which sequence, which tokens -------------------------------------------------------------------------
-    const uint32_t kvh = blockIdx.x % p.n_kv;
-    const int4 w0 = __ldcg(a.plan + blockIdx.x / p.n_kv * 2), w1 = __ldcg(a.plan + blockIdx.x / p.n_kv * 2 + 1);
-    const uint32_t b = (uint32_t)uniform(w0.x), item = (uint32_t)uniform(w0.y);
-    if (b >= p.B) return;
-    const Seq s = {uniform(w1.y), uniform(w1.z), uniform(w1.w)};
-    QueryTile qt[NT];
-    KeyTiles kt;
-    kt.lo = p.cap;
-    kt.hi = 0;
-#pragma unroll
-    for (uint32_t t = 0; t < NT; ++t) {
-        const int32_t i0 = (int32_t)((item * NT + t) * a.tt), n = min(max(s.q_len - i0, 0), (int32_t)a.tt);
-        qt[t].p0 = s.kv_len - s.q_len + i0;
-        qt[t].p1 = qt[t].p0 + n - 1;
-        qt[t].hi = n ? max(min(qt[t].p1 + 1, p.cap), 0) : 0;
-        qt[t].lo = a.window ? min(max(qt[t].p0 - a.window + 1, 0), qt[t].hi) : 0;
-        if (n) {
-            kt.lo = min(kt.lo, qt[t].lo);
-            kt.hi = max(kt.hi, qt[t].hi);
-        }
-    }
-    kt.lo = min(kt.lo, kt.hi);
-    kt.t_lo = kt.lo / (int32_t)kKt;
-    kt.n_sink = a.window ? min((min(a.sinks, kt.hi) + (int32_t)kKt - 1) / (int32_t)kKt, kt.t_lo) : 0;
-    kt.n = kt.n_sink + (kt.hi + (int32_t)kKt - 1) / (int32_t)kKt - kt.t_lo;
-    if (w0.w > 1) kt.take((uint32_t)w0.z, (uint32_t)w0.w);
-    kt.lo = uniform(kt.lo);
-    kt.hi = uniform(kt.hi);
-    kt.t_lo = uniform(kt.t_lo);
-    kt.n_sink = uniform(kt.n_sink);
-    kt.n = uniform(kt.n);
-#pragma unroll
-    for (uint32_t t = 0; t < NT; ++t) qt[t] = {uniform(qt[t].p0), uniform(qt[t].p1), uniform(qt[t].lo), uniform(qt[t].hi)};
-    const int32_t q_row = s.q0 + (int32_t)(item * NT * a.tt);              // first token of the block
 
     if (threadIdx.x == 0) {
         mbar_init(bar(Sh::bQ), 1);
@@ -241,13 +214,20 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             mbar_init(bar(Sh::bP + 2 * t), 4);
             mbar_init(bar(Sh::bP + 2 * t + 1), 4);
         }
-        mbar_init(bar(Sh::bO), NT);
+        for (uint32_t t = 0; t < NT; ++t) {
+            mbar_init(bar(Sh::bO + t), 1);
+            mbar_init(bar(Sh::bRead + t), 4);
+        }
         mbar_init(bar(Sh::bTurn), 1);
         mbar_init(bar(Sh::bTurn + 1), 1);
         mbar_init(bar(Sh::bQh), 4 * NT);
+        mbar_init(bar(Sh::bQfree), NT);
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(bar(Sh::bItem + i), 1);
+            mbar_init(bar(Sh::bTaken + i), Sh::kSched);         // all other warps
+        }
+        mbar_init(bar(Sh::bEnd), NT);
         *s_abort = 0;
-        s_item[0] = (uint32_t)w0.w;                             // pieces; this one's slot: for the end
-        s_item[1] = (uint32_t)(w1.x + w0.z);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == Sh::kMma) tmem_alloc(smem_s + Sh::oBar + Sh::oTmem, 512);
@@ -259,19 +239,52 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         if (lane == 0) { atomicExch(&g_prompt_status, code); *s_abort = 1; }
     };
 
+    // ---- pieces, one after the other: the roles run ahead of each other across their borders ------------------------
+    QueryTile qt[NT];
+    KeyTiles kt;
+    uint32_t b = 0, kvh = 0;
+    int32_t q_row = 0;                                          // first token of the piece
+    uint32_t ring0 = 0, q_count = 0;                            // tiles of K and V, and of Q, before this piece
+    auto get_item = [&](uint32_t k) {                           // false: there is none (or the wait ran out)
+        if (!__all_sync(kFull, mbar_wait(bar(Sh::bItem + k % 2), k / 2 & 1))) {
+            give_up(20);
+            return false;
+        }
+        volatile const int32_t *x = s_items + k % 2 * kItemWords;
+        if (x[kSequence] < 0 || *s_abort) return false;
+        b = (uint32_t)uniform(x[kSequence]);
+        kvh = (uint32_t)uniform(x[kHead]);
+        q_row = uniform(x[kFirstRow]);
+        kt = {uniform(x[kTilesAt]), uniform(x[kTilesAt + 1]), uniform(x[kTilesAt + 2]), uniform(x[kTilesAt + 3]), uniform(x[kTilesAt + 4])};
+#pragma unroll
+        for (uint32_t t = 0; t < NT; ++t)
+            qt[t] = {uniform(x[kQueriesAt + 4 * t]), uniform(x[kQueriesAt + 4 * t + 1]), uniform(x[kQueriesAt + 4 * t + 2]), uniform(x[kQueriesAt + 4 * t + 3])};
+        return true;
+    };
+    auto leave_item = [&](uint32_t k) {                         // this warp has read what it wants of it
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(Sh::bTaken + k % 2));
+    };
+    auto end_item = [&]() {
+        ring0 += 2 * (uint32_t)kt.n;
+        q_count += kt.n > 0;
+    };
+
     if (warp < 4 * NT) {
         if (Sh::kMove) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::kSoftRegs));
         // =========================== softmax: one thread per query row ===============================================
         const uint32_t t = warp >> 2, w = warp & 3, row = w * 32 + lane;
         const uint32_t tok = row / a.group, head = row % a.group;
+        uint32_t turn = 0;                                      // products of all pieces so far
+        bool ok = true;
+        for (uint32_t k = 0; ok && get_item(k); ++k) {
         QueryTile q = qt[0];
         if (NT == 2 && t == 1) q = qt[NT - 1];
         const int32_t pos = q.p0 + (int32_t)tok, last = min(pos, p.cap - 1);
         const uint32_t s_addr = tmem + ((w * 32u) << 16) + t * kKt, o_addr = tmem + ((w * 32u) << 16) + Sh::cO + t * D;
         float m = -INFINITY;
         uint64_t l2[4] = {0, 0, 0, 0};                          // sums of weights, eight at once
-        uint32_t done = 0;                                      // products so far
-        bool ok = true;
+        bool done = false;                                      // a product of this piece has been
         const uint32_t ids = kKt >> p.page_shift;               // pages of a tile
         auto page_id = [&](int32_t i) {                         // of tile i, one per lane; 0 where there is none to ask for
             const int32_t at = kt.first(i) + (int32_t)(lane << p.page_shift);
@@ -282,7 +295,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         volatile const int32_t *s_scale = reinterpret_cast<volatile const int32_t *>(smem + Sh::oBar + Sh::oScale);
         int32_t v_exp = 0;                                      // O stands for O 2^v_exp
         if (BITS == 4 && kt.n > 0) {                            // this row of Q to fp16, its largest value below 2^15
-            ok = __all_sync(kFull, mbar_wait(bar(Sh::bQ), 0));
+            ok = __all_sync(kFull, mbar_wait(bar(Sh::bQ), q_count & 1));
             if (!ok) give_up(18);
             const uint32_t q_s = smem_s + Sh::oQ + t * Sh::kTile + row * 128;
             auto chunk = [&](uint32_t c) { return q_s + (c / 8) * Sh::kBlock + ((c % 8 ^ (row & 7)) << 4); };
@@ -320,7 +333,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             const int32_t f = kt.first(i);
             const bool edge = gone || f + (int32_t)kKt - 1 > min(q.p0, p.cap - 1) ||
                               (a.window && f <= q.p1 - a.window && f + (int32_t)kKt > a.sinks);
-            if (!__all_sync(kFull, mbar_wait(bar(Sh::bS + t), done & 1))) {
+            if (!__all_sync(kFull, mbar_wait(bar(Sh::bS + t), turn & 1))) {
                 give_up(11);
                 ok = false;
                 break;
@@ -330,12 +343,13 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             if (BITS == 4) {
                 // The tile of V cannot be replaced before this row's weights are out, so its barrier can be waited on here; the
                 // exponents of the tile were written before it.
-                if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + (2 * i + 1) % NS), ((2 * i + 1) / NS) & 1))) {
+                const uint32_t c = ring0 + 2 * (uint32_t)i + 1, at = c / 2 % 8;
+                if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1))) {
                     give_up(19);
                     ok = false;
                     break;
                 }
-                const int32_t ke = s_scale[i % 8], ve = s_scale[8 + i % 8];
+                const int32_t ke = s_scale[at], ve = s_scale[8 + at];
                 scale = fmaxf(row_scale * power_of_2(ke / 2) * power_of_2(ke - ke / 2), 1.2e-38f);
                 v_down = done ? power_of_2(v_exp - ve) : 1.f;
                 v_exp = ve;
@@ -400,7 +414,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             // its number; both query tiles write them, as neither waits for the other.  (The copying warp alone took 15 us over a
             // tile: a prompt of 16001 under a window of 4096 1225 us instead of 780.)
             if (BITS == 16 && (f + (int32_t)kKt > kt.hi || (a.window && f < kt.lo && f + (int32_t)kKt > a.sinks))) {
-                const uint32_t c = 2 * (uint32_t)i + 1;
+                const uint32_t c = ring0 + 2 * (uint32_t)i + 1;
                 if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1))) {
                     give_up(16);
                     ok = false;
@@ -447,7 +461,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             };
             if (edge) weights(std::false_type());
             else weights(std::true_type());
-            ++done;
+            done = true;
+            ++turn;
         }
         float l = 0.f;
 #pragma unroll
@@ -457,15 +472,16 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             l += l0 + l1;
         }
         // ---- the row's result ----------------------------------------------------------------------------------
-        if (ok && !mbar_wait(bar(Sh::bO), 0)) { give_up(12); ok = false; }
-        ok = __all_sync(kFull, ok) && !*s_abort;
+        if (ok && !mbar_wait(bar(Sh::bO + t), k & 1)) { give_up(12); ok = false; }
+        ok = __all_sync(kFull, ok && !*s_abort);
         if (__all_sync(kFull, ok)) {
             tc_fence_after();
             const bool live = tok < a.tt && pos <= q.p1;
             const float inv = m == -INFINITY ? 0.f : 1.f / l;     // (nothing seen: zeros)
             const float up = BITS == 4 ? power_of_2(v_exp / 2) : 1.f, up2 = BITS == 4 ? power_of_2(v_exp - v_exp / 2) : 1.f;
-            const uint32_t pieces = s_item[0];
-            const size_t part = ((size_t)s_item[1] * p.n_kv + kvh) * (NT * 128) + t * 128 + row;
+            volatile const int32_t *item = s_items + k % 2 * kItemWords;
+            const uint32_t pieces = (uint32_t)item[kPieces];
+            const size_t part = ((size_t)(uint32_t)item[kSlot] * p.n_kv + kvh) * (NT * 128) + t * 128 + row;
             if (pieces > 1 && live) *reinterpret_cast<float2 *>(a.ml + part * 2) = make_float2(m, l);
             uint16_t *dst = a.out + (int64_t)(q_row + (int32_t)(t * a.tt + tok)) * a.ldo + (size_t)(kvh * a.group + head) * D;
 #pragma unroll 1
@@ -495,6 +511,12 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 }
             }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(Sh::bRead + t));         // O may be written again
+        leave_item(k);
+        end_item();
+        }
     } else {
         if (Sh::kMove) {                                        // by warpgroups: 4 bits have one of producers, one for the products
             if (BITS == 4 && warp >= Sh::kMma) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kMmaRegs));
@@ -508,16 +530,16 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         // One warp per query tile, in turns: while one tile's products run, the other's rows are at their exponentials.  Without
         // turns both come to do the same at the same time (4250 cycles for a pair of query tiles and a key tile instead of 2800).
         const uint32_t t = warp - Sh::kMma, idesc_s = kIdescS | (a.negate ? 1u << 13 : 0u);
-        QueryTile q = qt[0];
-        if (NT == 2 && t == 1) q = qt[NT - 1];
-        uint32_t made = 0;                                      // products with V issued
+        QueryTile q;
+        uint32_t made = 0, round = 0;                           // products with V issued, and key tiles, of all pieces
+        bool ok = true;
         const uint64_t q_desc = umma_desc_sw128(smem_s + Sh::oQ + t * Sh::kTile), k_desc = umma_desc_sw128(smem_s + Sh::oRing);
         const uint64_t v_desc = umma_desc_sw128_mn(smem_s + Sh::oRing, Sh::kBlock);
         const uint32_t s_col = tmem + t * kKt, o_col = tmem + Sh::cO + t * D;
         auto full = [&](uint32_t c) { return mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1); };
         auto scores = [&](int32_t i) {
             tc_fence_after();
-            const uint64_t kd = k_desc + ((2 * i) % NS) * (Sh::kTile >> 4);
+            const uint64_t kd = k_desc + ((ring0 + 2 * i) % NS) * (Sh::kTile >> 4);
             if (elect_one()) {
 #pragma unroll
                 for (uint32_t kk = 0; kk < D / 16; ++kk) {
@@ -532,19 +554,31 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             if (elect_one()) umma_commit(bar(Sh::bEmpty + c % NS));
             __syncwarp();
         };
-        bool ok = kt.n == 0 || __all_sync(kFull, mbar_wait(bar(BITS == 16 ? Sh::bQ : Sh::bQh), 0) && full(0));
-        if (ok && kt.n > 0) {
+        auto q_read = [&]() {                                   // Q may be written once the products so far are done
+            if (elect_one()) umma_commit(bar(Sh::bQfree));
+            __syncwarp();
+        };
+        for (uint32_t k = 0; ok && get_item(k); ++k) {
+        leave_item(k);
+        q = qt[0];
+        if (NT == 2 && t == 1) q = qt[NT - 1];
+        bool first = true;                                      // no product with V yet: O is written, not added to
+        if (kt.n > 0) {
+            ok = __all_sync(kFull, mbar_wait(bar(BITS == 16 ? Sh::bQ : Sh::bQh), q_count & 1) && full(ring0));
+            if (!ok) break;
             if (kt.seen_by(q, 0)) scores(0);
-            release(0);
+            release(ring0);
+            if (kt.n == 1) q_read();
         }
         for (int32_t i = 0; i < kt.n && ok; ++i) {
-            if (NT == 2 && (t == 1 || i > 0)) {
-                ok = __all_sync(kFull, mbar_wait(bar(Sh::bTurn + t), (t == 1 ? i : i - 1) & 1));
+            if (NT == 2 && (t == 1 || round > 0)) {
+                ok = __all_sync(kFull, mbar_wait(bar(Sh::bTurn + t), (t == 1 ? round : round - 1) & 1));
                 if (!ok) break;
             }
+            ++round;
             if (kt.seen_by(q, i)) {
-                const uint64_t vd = v_desc + ((2 * i + 1) % NS) * (Sh::kTile >> 4);
-                ok = __all_sync(kFull, full(2 * i + 1));
+                const uint64_t vd = v_desc + ((ring0 + 2 * i + 1) % NS) * (Sh::kTile >> 4);
+                ok = __all_sync(kFull, full(ring0 + 2 * i + 1));
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h) {              // the weights come in two halves
                     ok = ok && __all_sync(kFull, mbar_wait(bar(Sh::bP + 2 * t + h), made & 1));
@@ -553,49 +587,126 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t kk = h * (kKt / 32); kk < (h + 1) * (kKt / 32); ++kk)
-                            umma_ts(o_col, s_col + kk * 8, vd + kk * (2048 >> 4), kIdescO, made != 0 || kk != 0);
+                            umma_ts(o_col, s_col + kk * 8, vd + kk * (2048 >> 4), kIdescO, !first || kk != 0);
                     }
                     __syncwarp();
                 }
                 if (!ok) break;
                 ++made;
+                first = false;
             }
-            release(2 * i + 1);
+            release(ring0 + 2 * i + 1);
             if (i + 1 < kt.n) {
                 if (kt.seen_by(q, i + 1)) {
-                    ok = __all_sync(kFull, full(2 * i + 2));
+                    ok = __all_sync(kFull, full(ring0 + 2 * i + 2));
                     if (!ok) break;
                     scores(i + 1);
                 }
-                release(2 * i + 2);
+                release(ring0 + 2 * i + 2);
+                if (i + 2 == kt.n) q_read();
             }
             if (NT == 2 && lane == 0) mbar_arrive(bar(Sh::bTurn + (t ^ 1)));
             __syncwarp();
         }
-        if (!ok) give_up(13);
-        if (elect_one()) umma_commit(bar(Sh::bO));
+        if (!ok) break;
+        // (not before the rows' threads have waited for the piece before: a phase that nobody has seen would be lost)
+        if (k > 0 && !__all_sync(kFull, mbar_wait(bar(Sh::bRead + t), (k - 1) & 1))) {
+            ok = false;
+            break;
+        }
+        if (elect_one()) umma_commit(bar(Sh::bO + t));
         __syncwarp();
-        if (!__all_sync(kFull, mbar_wait(bar(Sh::bO), 0))) give_up(14);       // tensor memory is given back behind the last product
-    } else if (warp >= Sh::kMma + NT) {
+        end_item();
+        }
+        if (!ok) give_up(13);
+        if (elect_one()) umma_commit(bar(Sh::bEnd));
+        __syncwarp();
+        if (!__all_sync(kFull, mbar_wait(bar(Sh::bEnd), 0))) give_up(14);     // tensor memory is given back behind the last product
+    } else if (warp == Sh::kSched) {
+        // =========================== which piece next ===============================================================
+        for (uint32_t k = 0;; ++k) {
+            if (!mbar_wait_warp(bar(Sh::bTaken + k % 2), (k / 2 & 1) ^ 1)) { give_up(21); break; }
+            uint32_t v = 0;
+            if (lane == 0) v = (uint32_t)atomicAdd(a.next, 1);
+            v = __shfl_sync(kFull, v, 0);
+            int4 w0 = make_int4((int32_t)p.B, 0, 0, 0), w1 = make_int4(0, 0, 0, 0);
+            if (v < a.count && !*s_abort) {
+                w0 = __ldcg(a.plan + (size_t)(v / p.n_kv) * 2);
+                w1 = __ldcg(a.plan + (size_t)(v / p.n_kv) * 2 + 1);
+            }
+            const bool there = (uint32_t)w0.x < p.B;
+            const int32_t q0 = w1.y, q_len = w1.z, kv_len = w1.w;
+            kt.lo = p.cap;
+            kt.hi = 0;
+#pragma unroll
+            for (uint32_t t = 0; t < NT; ++t) {
+                const int32_t i0 = (int32_t)(((uint32_t)w0.y * NT + t) * a.tt), n = min(max(q_len - i0, 0), (int32_t)a.tt);
+                qt[t].p0 = kv_len - q_len + i0;
+                qt[t].p1 = qt[t].p0 + n - 1;
+                qt[t].hi = n ? max(min(qt[t].p1 + 1, p.cap), 0) : 0;
+                qt[t].lo = a.window ? min(max(qt[t].p0 - a.window + 1, 0), qt[t].hi) : 0;
+                if (n) {
+                    kt.lo = min(kt.lo, qt[t].lo);
+                    kt.hi = max(kt.hi, qt[t].hi);
+                }
+            }
+            kt.lo = min(kt.lo, kt.hi);
+            kt.t_lo = kt.lo / (int32_t)kKt;
+            kt.n_sink = a.window ? min((min(a.sinks, kt.hi) + (int32_t)kKt - 1) / (int32_t)kKt, kt.t_lo) : 0;
+            kt.n = kt.n_sink + (kt.hi + (int32_t)kKt - 1) / (int32_t)kKt - kt.t_lo;
+            if (w0.w > 1) kt.take((uint32_t)w0.z, (uint32_t)w0.w);
+            if (lane == 0) {
+                volatile int32_t *x = s_items + k % 2 * kItemWords;
+                x[kSequence] = there ? w0.x : -1;
+                x[kHead] = (int32_t)(v % p.n_kv);
+                x[kFirstRow] = q0 + (int32_t)((uint32_t)w0.y * NT * a.tt);
+                x[kPieces] = w0.w;
+                x[kSlot] = w1.x + w0.z;
+                x[kTilesAt] = kt.lo;
+                x[kTilesAt + 1] = kt.hi;
+                x[kTilesAt + 2] = kt.t_lo;
+                x[kTilesAt + 3] = kt.n_sink;
+                x[kTilesAt + 4] = kt.n;
+#pragma unroll
+                for (uint32_t t = 0; t < NT; ++t) {
+                    x[kQueriesAt + 4 * t] = qt[t].p0;
+                    x[kQueriesAt + 4 * t + 1] = qt[t].p1;
+                    x[kQueriesAt + 4 * t + 2] = qt[t].lo;
+                    x[kQueriesAt + 4 * t + 3] = qt[t].hi;
+                }
+                mbar_arrive(bar(Sh::bItem + k % 2));
+            }
+            __syncwarp();
+            if (!there) break;
+        }
+    } else if (warp > Sh::kSched) {
         // (warps that fill a warpgroup)
     } else if constexpr (BITS == 16) {
         // =========================== TMA copies ====================================================================
         const uint32_t ids = kKt >> p.page_shift;
-        if (lane == 0 && kt.n > 0) {
-            const uint32_t bytes = a.tt * a.group * 128;        // of a block of 64 channels
-            mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
-            for (uint32_t t = 0; t < NT; ++t)
-                for (uint32_t c = 0; c < NB; ++c)
-                    tma_load_3d(smem_s + Sh::oQ + t * Sh::kTile + c * Sh::kBlock, &q_map, (int32_t)(c * 64), (int32_t)(kvh * a.group),
-                                q_row + (int32_t)(t * a.tt), bar(Sh::bQ));
-        }
-        uint32_t issued = 0;
+        uint32_t issued = 0, queries = 0;                       // copies asked for
         bool ok = true;
+        auto load_q = [&]() {
+            if (q_count && !mbar_wait_warp(bar(Sh::bQfree), (q_count - 1) & 1)) return false;
+            if (lane == 0) {
+                const uint32_t bytes = a.tt * a.group * 128;    // of a block of 64 channels
+                mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
+                for (uint32_t t = 0; t < NT; ++t)
+                    for (uint32_t c = 0; c < NB; ++c)
+                        tma_load_3d(smem_s + Sh::oQ + t * Sh::kTile + c * Sh::kBlock, &q_map, (int32_t)(c * 64), (int32_t)(kvh * a.group),
+                                    q_row + (int32_t)(t * a.tt), bar(Sh::bQ));
+            }
+            __syncwarp();
+            ++queries;
+            return true;
+        };
         auto row_of = [&](int32_t i) {                          // this lane's page of tile i, as a row of the pool
             const int32_t at = kt.first(i) + (int32_t)(lane << p.page_shift);
             const int32_t id = lane < ids && at < kt.hi ? page_of(p, b, at) : -1;
             return id < 0 ? -(int32_t)kKt : (int32_t)row_index(p, id, kvh, at);
         };
+        for (uint32_t k = 0; ok && get_item(k); ++k) {
+        leave_item(k);
         int32_t next = kt.n > 0 ? row_of(0) : 0;
         for (int32_t i = 0; i < kt.n && ok; ++i) {
             const int32_t r = next;
@@ -611,11 +722,14 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     for (uint32_t c = 0; c < NB; ++c)
                         tma_load_2d(dst + c * Sh::kBlock + (lane << p.page_shift) * 128, kv ? &v_map : &k_map, (int32_t)(c * 64), r, to);
                 __syncwarp();
+                if (i == 0 && kv == 0 && !load_q()) { give_up(22); ok = false; ++issued; break; }
             }
+        }
+        end_item();
         }
         if (!ok)                                                // copies under way end before the block does
             for (uint32_t c = issued > NS ? issued - NS : 0; c < issued; ++c) (void)mbar_wait_warp(bar(Sh::bFull + c % NS), (c / NS) & 1);
-        if (!ok && kt.n > 0) (void)mbar_wait_warp(bar(Sh::bQ), 0);
+        if (!ok && queries) (void)mbar_wait_warp(bar(Sh::bQ), (queries - 1) & 1);
     } else {
         // =========================== codes to fp16: a thread, or two, per position ==========================================
         constexpr uint32_t G = D / 64;
@@ -624,16 +738,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         const bool first_thread = threadIdx.x == Sh::kProd * 32;
         volatile int32_t *s_scale = reinterpret_cast<volatile int32_t *>(smem + Sh::oBar + Sh::oScale);
         volatile uint32_t *s_largest = reinterpret_cast<volatile uint32_t *>(smem + Sh::oBar + Sh::oLargest);
-        if (first_thread && kt.n > 0) {
-            const uint32_t bytes = a.tt * a.group * 128;
-            mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
-            for (uint32_t t = 0; t < NT; ++t)
-                for (uint32_t c = 0; c < NB; ++c)
-                    tma_load_3d(smem_s + Sh::oQ + t * Sh::kTile + c * Sh::kBlock, &q_map, (int32_t)(c * 64), (int32_t)(kvh * a.group),
-                                q_row + (int32_t)(t * a.tt), bar(Sh::bQ));
-        }
-        uint32_t issued = 0;
-        int32_t v_exp = -1000;                                  // (no tile of V yet)
+        uint32_t issued = 0, queries = 0;
+        int32_t v_exp;
         bool ok = true;
         // What this thread's position of a tile holds, fetched while the tile before is turned.
         struct Codes {
@@ -681,7 +787,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 ok = false;
             }
             if (!ok) return;
-            if (first_thread) s_scale[kv * 8 + i % 8] = e;
+            if (first_thread) s_scale[kv * 8 + issued / 2 % 8] = e;
 #pragma unroll
             for (uint32_t g = 0; g < G; ++g) {
                 const float step = lo_bf16(sc[g]) * down * down2, low = hi_bf16(sc[g]) * down * down2;
@@ -705,9 +811,28 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(Sh::bFull + slot));
         };
+        for (uint32_t k = 0; ok && get_item(k); ++k) {
+        leave_item(k);
+        v_exp = -1000;                                          // (no tile of V yet)
         Codes f0, f1;
         int32_t id = page_at(0), id_next = page_at(1);
-        if (kt.n > 0) fetch(f0, id, 0, 0);
+        if (kt.n > 0) {
+            fetch(f0, id, 0, 0);
+            if (warp == Sh::kProd) {
+                if (q_count) ok = mbar_wait_warp(bar(Sh::bQfree), (q_count - 1) & 1);
+                if (!ok) give_up(22);
+                if (ok && lane == 0) {
+                    const uint32_t bytes = a.tt * a.group * 128;
+                    mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
+                    for (uint32_t t = 0; t < NT; ++t)
+                        for (uint32_t c = 0; c < NB; ++c)
+                            tma_load_3d(smem_s + Sh::oQ + t * Sh::kTile + c * Sh::kBlock, &q_map, (int32_t)(c * 64), (int32_t)(kvh * a.group),
+                                        q_row + (int32_t)(t * a.tt), bar(Sh::bQ));
+                }
+                queries += ok;
+                __syncwarp();
+            }
+        }
         for (int32_t i = 0; i < kt.n; ++i) {
             fetch(f1, id, i, 1);
             turn(f0, id, i, 0);
@@ -719,7 +844,9 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             turn(f1, id_here, i, 1);
             ++issued;
         }
-        if (!ok && kt.n > 0) (void)mbar_wait_warp(bar(Sh::bQ), 0);
+        end_item();
+        }
+        if (!ok && queries) (void)mbar_wait_warp(bar(Sh::bQ), (queries - 1) & 1);
     }
     }
     tc_fence_before();
@@ -794,7 +921,7 @@ static int launch_prompt(const PromptArgs &a, const PromptPlan &l, const CUtenso
     const uint64_t blocks = (uint64_t)l.count * a.p.n_kv;
     CI_REQUIRE(blocks <= 0x7FFFFFFFu, "too many blocks");
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.gridDim = dim3((unsigned)(blocks < l.sms ? blocks : l.sms));
     cfg.blockDim = dim3(Sh::kThreads);
     cfg.dynamicSmemBytes = Sh::kSmem;
     cfg.stream = s;
@@ -842,6 +969,8 @@ int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const Prom
     a.out = out; a.ldo = ldo;
     a.plan = l.pieces;
     a.cuts = l.cuts;
+    a.next = &l.cuts->y;
+    a.count = l.count * p.n_kv;
     a.ml = (float *)(l.pieces + (size_t)l.count * 2);
     a.partial = a.ml + prompt_slot_rows(c->head_dim) * 2;
     CUtensorMap qm, km, vm;
