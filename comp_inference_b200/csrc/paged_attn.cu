@@ -586,13 +586,11 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
 // Joins the parts of an item that several blocks had: block c has the item that block c of the attention began, all rows at once, if
 // that has few parts.  Items of many parts are few, and the blocks share their rows: a block per row, its threads over the
 // parts (5 items of 59 parts, heads of 256: the join's 55 us become XXXX).  Everything in a fixed order: the same sum every time.
-constexpr int32_t kFewParts = 16;
+constexpr int32_t kFewParts = 8;
 
 template <int D, int RT>
 __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PromptPlan plan) {
-    constexpr uint32_t kPer = 256 / RT;                         // threads that look for a row's maximum
     constexpr uint32_t kLanes = D / 4, kShares = 256 / kLanes;  // threads of a row, and such rows of threads
-    __shared__ float s_m[RT], s_inv[RT];
     __shared__ __align__(16) float4 s_y[kShares][kLanes];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -614,35 +612,33 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Page
     const int4 head = __ldcg(reinterpret_cast<const int4 *>(d));
     if (head.x > 0 && head.x <= kFewParts) {
         const int32_t parts = head.x, kvh = __ldcg(d + 4);
-        {
-            const uint32_t r = threadIdx.x / kPer;
-            float M = kNone, L = 0.f;
-            for (int32_t i = threadIdx.x % kPer; i < parts; i += kPer) M = fmaxf(M, __ldcg(a.ml + (slot(blockIdx.x, i) * RT + r) * 2));
-            for (uint32_t o = kPer / 2; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
-            for (int32_t i = threadIdx.x % kPer; i < parts; i += kPer) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.ml + (slot(blockIdx.x, i) * RT + r) * 2));
-                L += ml.x == kNone ? 0.f : ex2(ml.x - M) * ml.y;
-            }
-            for (uint32_t o = kPer / 2; o; o >>= 1) L += __shfl_xor_sync(kFull, L, o);
-            if (threadIdx.x % kPer == 0) {
-                s_m[r] = M == kNone ? 0.f : M;
-                s_inv[r] = M == kNone ? 0.f : 1.f / L;
-            }
-        }
-        __syncthreads();
-        for (uint32_t x = threadIdx.x; x < RT * D / 4; x += 256) {
-            const uint32_t r = x / (D / 4), c = x % (D / 4) * 4, row = (uint32_t)head.w + r;
+#pragma unroll 1
+        for (uint32_t x = threadIdx.x; x < RT * kLanes; x += 256) {
+            const uint32_t r = x / kLanes, c = x % kLanes * 4, row = (uint32_t)head.w + r;
             if ((int32_t)row >= head.z) continue;
-            const float M = s_m[r];
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int32_t i = 0; i < parts; ++i) {
-                const float m = __ldcg(a.ml + (slot(blockIdx.x, i) * RT + r) * 2);
-                const float4 z = __ldcg(reinterpret_cast<const float4 *>(a.partial + (slot(blockIdx.x, i) * RT + r) * D + c));
-                const float e = m == kNone ? 0.f : ex2(m - M);
-                y.x += e * z.x; y.y += e * z.y; y.z += e * z.z; y.w += e * z.w;
+            float2 ml[kFewParts];                               // asked for at once, (max, sum) and outputs
+            float4 z[kFewParts];
+#pragma unroll
+            for (int32_t i = 0; i < kFewParts; ++i) {
+                ml[i] = make_float2(kNone, 0.f);
+                z[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < parts) {
+                    ml[i] = __ldcg(reinterpret_cast<const float2 *>(a.ml + (slot(blockIdx.x, i) * RT + r) * 2));
+                    z[i] = __ldcg(reinterpret_cast<const float4 *>(a.partial + (slot(blockIdx.x, i) * RT + r) * D + c));
+                }
             }
-            store(head, kvh, row, c, y, s_inv[r]);
+            float M = kNone, L = 0.f;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int32_t i = 0; i < kFewParts; ++i) M = fmaxf(M, ml[i].x);
+            const float safe = M == kNone ? 0.f : M;
+#pragma unroll
+            for (int32_t i = 0; i < kFewParts; ++i) {
+                const float e = ml[i].x == kNone ? 0.f : ex2(ml[i].x - safe);
+                L += e * ml[i].y;
+                y.x += e * z[i].x; y.y += e * z[i].y; y.z += e * z[i].z; y.w += e * z[i].w;
+            }
+            store(head, kvh, row, c, y, M == kNone ? 0.f : 1.f / L);
         }
     }
     for (; rows_here; rows_here &= rows_here - 1) {
@@ -652,20 +648,23 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Page
         if ((int32_t)row >= h.z) continue;
         const int32_t parts = h.x, kvh = __ldcg(a.desc + c * 8 + 4);
         const uint32_t lane = lane_id();
-        float M = kNone, L = 0.f;                               // in every warp
+        float M = kNone, L = 0.f;                               // in every warp: lane l has parts l, l + 32, ...
+        const float2 mine = (int32_t)lane < parts ? __ldcg(reinterpret_cast<const float2 *>(a.ml + (slot(c, lane) * RT + r) * 2)) : make_float2(kNone, 0.f);
+        M = mine.x;
 #pragma unroll 4
-        for (int32_t i = lane; i < parts; i += 32) M = fmaxf(M, __ldcg(a.ml + (slot(c, i) * RT + r) * 2));
+        for (int32_t i = lane + 32; i < parts; i += 32) M = fmaxf(M, __ldcg(a.ml + (slot(c, i) * RT + r) * 2));
         for (uint32_t o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
         const float safe = M == kNone ? 0.f : M;
+        L = mine.x == kNone ? 0.f : ex2(mine.x - safe) * mine.y;
 #pragma unroll 4
-        for (int32_t i = lane; i < parts; i += 32) {
+        for (int32_t i = lane + 32; i < parts; i += 32) {
             const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.ml + (slot(c, i) * RT + r) * 2));
             L += ml.x == kNone ? 0.f : ex2(ml.x - safe) * ml.y;
         }
         for (uint32_t o = 16; o; o >>= 1) L += __shfl_xor_sync(kFull, L, o);
         const uint32_t at = threadIdx.x % kLanes, share = threadIdx.x / kLanes;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+#pragma unroll 4
         for (int32_t i = share; i < parts; i += kShares) {
             const float m = __ldcg(a.ml + (slot(c, i) * RT + r) * 2);
             const float4 z = __ldcg(reinterpret_cast<const float4 *>(a.partial + (slot(c, i) * RT + r) * D + at * 4));

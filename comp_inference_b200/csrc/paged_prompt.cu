@@ -59,9 +59,9 @@ struct PromptShape {
     static constexpr bool kMove = NT == 2 || BITS == 4;
     static constexpr uint32_t kWarps = kMove ? (kSched + 4) / 4 * 4 : kSched + 1, kThreads = kWarps * 32;
     static constexpr uint32_t kLaunchRegs = 65536 / kThreads / 8 * 8;
-    static constexpr uint32_t kSoftRegs = BITS == 16 ? 200 : D == 64 ? 160 : D == 128 ? 152 : 176;
+    static constexpr uint32_t kSoftRegs = BITS == 16 ? 200 : D == 64 ? 160 : D == 128 ? 144 : 176;
     static constexpr uint32_t kProdRegs = BITS == 16 ? 104 : D == 64 ? 120 : D == 128 ? 64 : 104;
-    static constexpr uint32_t kMmaRegs = BITS == 16 ? kProdRegs : D == 64 ? 72 : D == 128 ? 48 : 112;
+    static constexpr uint32_t kMmaRegs = BITS == 16 ? kProdRegs : D == 64 ? 72 : D == 128 ? 64 : 112;
     static_assert(!kMove || (kSoftRegs >= kLaunchRegs && kProdRegs <= kLaunchRegs && kMmaRegs <= kLaunchRegs &&
                              NT * 128 * kSoftRegs + (BITS == 16 ? 128 * kProdRegs : PW * 32 * kProdRegs + 128 * kMmaRegs) <= kThreads * kLaunchRegs), "registers");
     static constexpr uint32_t oQ = 0, oRing = NT * kTile, oBar = oRing + NS * kTile, kMisc = 640, kSmem = oBar + kMisc + 1024;
@@ -81,18 +81,16 @@ __device__ __forceinline__ float ex2f(float x) {
     return y;
 }
 
-// A query tile: positions of its first and last token (p1 < p0: it has none) and the range that they see.
+// A query tile: positions of its first and last token (p1 < p0: it has none), and which of the block's key tiles they see: the
+// first tokens' and [from, to).
 struct QueryTile {
-    int32_t p0, p1, lo, hi;
+    int32_t p0, p1, from, to;
 };
 // The key tiles that a block visits: tile i of n starts at first(i).
 struct KeyTiles {
     int32_t lo, hi, t_lo, n_sink, n;
     __device__ __forceinline__ int32_t first(int32_t i) const { return (i < n_sink ? i : t_lo + i - n_sink) * (int32_t)kKt; }
-    __device__ __forceinline__ bool seen_by(const QueryTile &q, int32_t i) const {
-        const int32_t f = first(i);
-        return q.p1 >= q.p0 && f < q.hi && (i < n_sink || f + (int32_t)kKt > q.lo);
-    }
+    __device__ __forceinline__ bool seen_by(const QueryTile &q, int32_t i) const { return i < q.to && (i < n_sink || i >= q.from); }
     // Of these tiles only those of one piece of several.  The first tokens of a window go with the first one.
     __device__ __forceinline__ void take(uint32_t piece, uint32_t pieces) {
         auto begin = [&](uint32_t k) {
@@ -242,8 +240,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     // ---- pieces, one after the other: the roles run ahead of each other across their borders ------------------------
     QueryTile qt[NT];
     KeyTiles kt;
-    uint32_t b = 0, kvh = 0;
-    int32_t q_row = 0;                                          // first token of the piece
+    uint32_t b = 0;
     uint32_t ring0 = 0, q_count = 0;                            // tiles of K and V, and of Q, before this piece
     auto get_item = [&](uint32_t k) {                           // false: there is none (or the wait ran out)
         if (!__all_sync(kFull, mbar_wait(bar(Sh::bItem + k % 2), k / 2 & 1))) {
@@ -253,14 +250,14 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         volatile const int32_t *x = s_items + k % 2 * kItemWords;
         if (x[kSequence] < 0 || *s_abort) return false;
         b = (uint32_t)uniform(x[kSequence]);
-        kvh = (uint32_t)uniform(x[kHead]);
-        q_row = uniform(x[kFirstRow]);
         kt = {uniform(x[kTilesAt]), uniform(x[kTilesAt + 1]), uniform(x[kTilesAt + 2]), uniform(x[kTilesAt + 3]), uniform(x[kTilesAt + 4])};
 #pragma unroll
         for (uint32_t t = 0; t < NT; ++t)
             qt[t] = {uniform(x[kQueriesAt + 4 * t]), uniform(x[kQueriesAt + 4 * t + 1]), uniform(x[kQueriesAt + 4 * t + 2]), uniform(x[kQueriesAt + 4 * t + 3])};
         return true;
     };
+    auto head_of = [&](uint32_t k) { return (uint32_t)uniform(s_items[k % 2 * kItemWords + kHead]); };
+    auto first_row_of = [&](uint32_t k) { return uniform(s_items[k % 2 * kItemWords + kFirstRow]); };       // first token of the piece
     auto leave_item = [&](uint32_t k) {                         // this warp has read what it wants of it
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(Sh::bTaken + k % 2));
@@ -283,7 +280,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         const int32_t pos = q.p0 + (int32_t)tok, last = min(pos, p.cap - 1);
         const uint32_t s_addr = tmem + ((w * 32u) << 16) + t * kKt, o_addr = tmem + ((w * 32u) << 16) + Sh::cO + t * D;
         float m = -INFINITY;
-        uint64_t l2[4] = {0, 0, 0, 0};                          // sums of weights, eight at once
+        constexpr int kSums = BITS == 16 ? 4 : 2;
+        uint64_t l2[kSums] = {};                                // sums of weights, two in each
         bool done = false;                                      // a product of this piece has been
         const uint32_t ids = kKt >> p.page_shift;               // pages of a tile
         auto page_id = [&](int32_t i) {                         // of tile i, one per lane; 0 where there is none to ask for
@@ -397,7 +395,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 float c = grow ? ex2f(m - mx) : 1.f;
                 if (grow) m = mx;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) l2[e] = fma2(l2[e], pair(c, c), 0);
+                for (int e = 0; e < kSums; ++e) l2[e] = fma2(l2[e], pair(c, c), 0);
                 c *= v_down;
                 if (done) {
 #pragma unroll 1
@@ -447,7 +445,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                             e0 = ex2f(e0);
                             e1 = ex2f(e1);
                         }
-                        l2[j % 4] = add2(l2[j % 4], pair(e0, e1));
+                        l2[j % kSums] = add2(l2[j % kSums], pair(e0, e1));
                         pk[j] = BITS == 16 ? pack_bf16(e0, e1) : pack_f16(e0, e1);
                     }
                     tmem_st16(s_addr + c * 16, pk);
@@ -466,7 +464,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         }
         float l = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < kSums; ++e) {
             float l0, l1;
             split(l2[e], l0, l1);
             l += l0 + l1;
@@ -480,7 +478,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             const float inv = m == -INFINITY ? 0.f : 1.f / l;     // (nothing seen: zeros)
             const float up = BITS == 4 ? power_of_2(v_exp / 2) : 1.f, up2 = BITS == 4 ? power_of_2(v_exp - v_exp / 2) : 1.f;
             volatile const int32_t *item = s_items + k % 2 * kItemWords;
-            const uint32_t pieces = (uint32_t)item[kPieces];
+            const uint32_t pieces = (uint32_t)item[kPieces], kvh = head_of(k);
+            const int32_t q_row = first_row_of(k);
             const size_t part = ((size_t)(uint32_t)item[kSlot] * p.n_kv + kvh) * (NT * 128) + t * 128 + row;
             if (pieces > 1 && live) *reinterpret_cast<float2 *>(a.ml + part * 2) = make_float2(m, l);
             uint16_t *dst = a.out + (int64_t)(q_row + (int32_t)(t * a.tt + tok)) * a.ldo + (size_t)(kvh * a.group + head) * D;
@@ -638,16 +637,17 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             const int32_t q0 = w1.y, q_len = w1.z, kv_len = w1.w;
             kt.lo = p.cap;
             kt.hi = 0;
+            int32_t lo[NT], hi[NT];                             // what a query tile sees
 #pragma unroll
             for (uint32_t t = 0; t < NT; ++t) {
                 const int32_t i0 = (int32_t)(((uint32_t)w0.y * NT + t) * a.tt), n = min(max(q_len - i0, 0), (int32_t)a.tt);
                 qt[t].p0 = kv_len - q_len + i0;
                 qt[t].p1 = qt[t].p0 + n - 1;
-                qt[t].hi = n ? max(min(qt[t].p1 + 1, p.cap), 0) : 0;
-                qt[t].lo = a.window ? min(max(qt[t].p0 - a.window + 1, 0), qt[t].hi) : 0;
+                hi[t] = n ? max(min(qt[t].p1 + 1, p.cap), 0) : 0;
+                lo[t] = a.window ? min(max(qt[t].p0 - a.window + 1, 0), hi[t]) : 0;
                 if (n) {
-                    kt.lo = min(kt.lo, qt[t].lo);
-                    kt.hi = max(kt.hi, qt[t].hi);
+                    kt.lo = min(kt.lo, lo[t]);
+                    kt.hi = max(kt.hi, hi[t]);
                 }
             }
             kt.lo = min(kt.lo, kt.hi);
@@ -655,6 +655,11 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             kt.n_sink = a.window ? min((min(a.sinks, kt.hi) + (int32_t)kKt - 1) / (int32_t)kKt, kt.t_lo) : 0;
             kt.n = kt.n_sink + (kt.hi + (int32_t)kKt - 1) / (int32_t)kKt - kt.t_lo;
             if (w0.w > 1) kt.take((uint32_t)w0.z, (uint32_t)w0.w);
+#pragma unroll
+            for (uint32_t t = 0; t < NT; ++t) {
+                qt[t].from = lo[t] / (int32_t)kKt - kt.t_lo + kt.n_sink;
+                qt[t].to = qt[t].p1 < qt[t].p0 ? 0 : (hi[t] + (int32_t)kKt - 1) / (int32_t)kKt - kt.t_lo + kt.n_sink;
+            }
             if (lane == 0) {
                 volatile int32_t *x = s_items + k % 2 * kItemWords;
                 x[kSequence] = there ? w0.x : -1;
@@ -671,8 +676,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 for (uint32_t t = 0; t < NT; ++t) {
                     x[kQueriesAt + 4 * t] = qt[t].p0;
                     x[kQueriesAt + 4 * t + 1] = qt[t].p1;
-                    x[kQueriesAt + 4 * t + 2] = qt[t].lo;
-                    x[kQueriesAt + 4 * t + 3] = qt[t].hi;
+                    x[kQueriesAt + 4 * t + 2] = qt[t].from;
+                    x[kQueriesAt + 4 * t + 3] = qt[t].to;
                 }
                 mbar_arrive(bar(Sh::bItem + k % 2));
             }
@@ -684,7 +689,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     } else if constexpr (BITS == 16) {
         // =========================== TMA copies ====================================================================
         const uint32_t ids = kKt >> p.page_shift;
-        uint32_t issued = 0, queries = 0;                       // copies asked for
+        uint32_t issued = 0, queries = 0, kvh = 0;              // copies asked for; the piece's head
+        int32_t q_row = 0;                                      // and first token
         bool ok = true;
         auto load_q = [&]() {
             if (q_count && !mbar_wait_warp(bar(Sh::bQfree), (q_count - 1) & 1)) return false;
@@ -706,6 +712,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             return id < 0 ? -(int32_t)kKt : (int32_t)row_index(p, id, kvh, at);
         };
         for (uint32_t k = 0; ok && get_item(k); ++k) {
+        kvh = head_of(k);
+        q_row = first_row_of(k);
         leave_item(k);
         int32_t next = kt.n > 0 ? row_of(0) : 0;
         for (int32_t i = 0; i < kt.n && ok; ++i) {
@@ -738,8 +746,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         const bool first_thread = threadIdx.x == Sh::kProd * 32;
         volatile int32_t *s_scale = reinterpret_cast<volatile int32_t *>(smem + Sh::oBar + Sh::oScale);
         volatile uint32_t *s_largest = reinterpret_cast<volatile uint32_t *>(smem + Sh::oBar + Sh::oLargest);
-        uint32_t issued = 0, queries = 0;
-        int32_t v_exp;
+        uint32_t issued = 0, queries = 0, kvh = 0;
+        int32_t q_row = 0, v_exp;
         bool ok = true;
         // What this thread's position of a tile holds, fetched while the tile before is turned.
         struct Codes {
@@ -812,6 +820,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             if (lane == 0) mbar_arrive(bar(Sh::bFull + slot));
         };
         for (uint32_t k = 0; ok && get_item(k); ++k) {
+        kvh = head_of(k);
+        q_row = first_row_of(k);
         leave_item(k);
         v_exp = -1000;                                          // (no tile of V yet)
         Codes f0, f1;
