@@ -520,6 +520,15 @@ void same_device(const Tensor &t, const Tensor &like, const char *name) {
     require_cuda(t, name);
     TORCH_CHECK(t.device() == like.device(), name, " is on ", t.device(), ", the others on ", like.device());
 }
+// Whether rows of `a_cols` elements from a, `lda` apart, and such of b share memory.  Columns of one wider matrix do not.
+bool overlap(const void *a, int64_t a_rows, int64_t a_cols, int64_t lda, const void *b, int64_t b_rows, int64_t b_cols, int64_t ldb) {
+    if (a_rows == 0 || b_rows == 0 || a_cols == 0 || b_cols == 0) return false;
+    const int64_t x = (int64_t)(reinterpret_cast<uintptr_t>(a) / 2), y = (int64_t)(reinterpret_cast<uintptr_t>(b) / 2);
+    if (x + (a_rows - 1) * lda + a_cols <= y || y + (b_rows - 1) * ldb + b_cols <= x) return false;
+    if (lda != ldb || a_rows == 1 || b_rows == 1) return true;
+    const int64_t off = ((y - x) % lda + lda) % lda;
+    return off < a_cols || off + b_cols > lda;
+}
 bool aligned16(const Tensor &t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
 
 // Pages of one layer and their descriptor.
@@ -548,12 +557,8 @@ struct PagedCache {
             REFUSE(k_scale.sizes() != at::IntArrayRef(s) || v_scale.sizes() != at::IntArrayRef(s) || !k_scale.is_contiguous() || !v_scale.is_contiguous(),
                    "steps and lowest values must be contiguous [num_pages, n_kv, page_size, head_dim / 64, 2], got " + shape_of(k_scale) + " and " + shape_of(v_scale));
         }
-        require_cuda(k, "pages");
-        same_device(v, k, "pages of values");
-        if (four) {
-            same_device(k_scale, k, "steps and lowest values");
-            same_device(v_scale, k, "steps and lowest values");
-        }
+        // (that they are on a GPU is for the calls to see)
+        for (const Tensor *t : {&v, &k_scale, &v_scale}) TORCH_CHECK(!t->defined() || t->device() == k.device(), "pages on ", k.device(), " and ", t->device());
         memset(&c, 0, sizeof c);
         c.k = k.data_ptr();
         c.v = v.data_ptr();
@@ -662,6 +667,9 @@ Tensor paged_append(PagedCache &cache, const Tensor &q, const Tensor &k, const T
     if (out.has_value()) same_device(y, cache.k, "out");
     else y = at::empty({rq.T, rq.heads, d}, q.options());
     if (rq.T == 0 || b.B == 0) return y;
+    const int64_t w = rq.heads * d, wk = rk.heads * d;
+    REFUSE((y.data_ptr() != (const void *)rq.ptr || (rq.T > 1 && rq.ld != w)) && overlap(y.data_ptr(), rq.T, w, w, rq.ptr, rq.T, w, rq.ld), "out overlaps q; it may be all of q, or none");
+    REFUSE(overlap(y.data_ptr(), rq.T, w, w, rk.ptr, rq.T, wk, rk.ld) || overlap(y.data_ptr(), rq.T, w, w, rv.ptr, rq.T, wk, rv.ld), "out overlaps k or v");
     check(ci_rope_paged_append(cache.now(), &b, rq.ptr, rq.ld, rk.ptr, rk.ld, rv.ptr, rv.ld, (uint32_t)rq.heads, (const uint16_t *)cos.data_ptr(),
                                (const uint16_t *)sin.data_ptr(), (uint32_t)cos.size(0), (uint16_t *)y.data_ptr(), stream()));
     return y;
@@ -698,6 +706,7 @@ Tensor paged_attention(PagedCache &cache, const Tensor &q, const Tensor &table, 
     if (out.has_value()) same_device(y, cache.k, "out");
     else y = at::empty({r.T, r.heads * d}, q.options());
     if (r.T == 0 || b.B == 0) return y;
+    REFUSE(overlap(y.data_ptr(), r.T, r.heads * d, r.T > 1 ? y.stride(0) : r.heads * d, r.ptr, r.T, r.heads * d, r.ld), "out overlaps q");
     // of this call: from the allocator's pool of the stream, or of the graph that is being captured
     const ci_paged_cache *c = cache.now();
     const uint32_t longest = (uint32_t)std::min(max_q_len, most);
@@ -771,6 +780,8 @@ Tensor adjust_logits(const Tensor &logits, const OptTensor &tokens, const OptTen
     if (out.has_value()) same_device(y, logits, "out");
     else y = at::empty({B, V}, logits.options());
     if (B == 0) return y;
+    const bool same = y.data_ptr() == logits.data_ptr() && (B == 1 || y.stride(0) == logits.stride(0));
+    REFUSE(!same && overlap(y.data_ptr(), B, V, B > 1 ? y.stride(0) : V, logits.data_ptr(), B, V, B > 1 ? logits.stride(0) : V), "out overlaps logits; it may be all of them, or none");
     a.d_in = (const uint16_t *)logits.data_ptr();
     a.d_out = (uint16_t *)y.data_ptr();
     a.ld_in = B > 1 ? logits.stride(0) : V;

@@ -74,24 +74,34 @@ __global__ void __launch_bounds__(THREADS) k_adjust_logits(const __grid_constant
     }
     const float r = a.repetition ? __ldg(a.repetition + b) : 1.f, f = a.frequency ? __ldg(a.frequency + b) : 0.f;
     const float p = a.presence ? __ldg(a.presence + b) : 0.f;
-    for (uint32_t i = threadIdx.x; i < CHUNK / 4; i += THREADS) reinterpret_cast<uint4 *>(s_word)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    auto place = [&](int64_t id) { return (uint64_t)id < a.V ? (uint64_t)(id - v0) : ~0ull; };
+    // Lengths and the first biases are asked for now too.  (Tokens of the history as well: 15.4 us instead of 14.0, most rows have few.)
     const uint32_t n_bias = min(a.n_bias, kBiases);
     const int64_t *bias_ids = a.bias_ids + (int64_t)b * a.ld_bias;
     const float *bias = a.bias + (int64_t)b * a.ld_bias;
+    const int64_t *tok = a.tokens + (int64_t)b * a.ld_tokens;
+    int64_t id0 = -1;
+    float bias0 = 0.f;
+    uint32_t len = 0, prompt = 0;
+    if (a.tokens) {
+        len = (uint32_t)min(max(__ldg(a.lens + b), 0), (int32_t)a.L);
+        prompt = a.prompt_lens ? (uint32_t)max(__ldg(a.prompt_lens + b), 0) : 0;
+    }
+    if (threadIdx.x < n_bias) {
+        id0 = __ldg(bias_ids + threadIdx.x);
+        bias0 = __ldg(bias + threadIdx.x);
+    }
+    for (uint32_t i = threadIdx.x; i < CHUNK / 4; i += THREADS) reinterpret_cast<uint4 *>(s_word)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    auto place = [&](int64_t id) { return (uint64_t)id < a.V ? (uint64_t)(id - v0) : ~0ull; };
     for (uint32_t i = threadIdx.x; i < n_bias; i += THREADS) {
-        const uint64_t at = place(__ldg(bias_ids + i));
+        const uint64_t at = place(i == threadIdx.x ? id0 : __ldg(bias_ids + i));
         if (at < CHUNK) atomicMax(&s_word[at], kBiased | (kBiases - i) << kPlace);      // the first one's place is the largest
         s_at[i] = at < CHUNK ? (int32_t)at : -1;
-        s_bias[i] = __ldg(bias + i);
+        s_bias[i] = i == threadIdx.x ? bias0 : __ldg(bias + i);
         s_more[i] = 0;
     }
     if (a.n_bias) __syncthreads();
     if (a.tokens) {
-        const uint32_t len = (uint32_t)min(max(__ldg(a.lens + b), 0), (int32_t)a.L);
-        const uint32_t prompt = a.prompt_lens ? (uint32_t)min(max(__ldg(a.prompt_lens + b), 0), (int32_t)len) : 0;
-        const int64_t *tok = a.tokens + (int64_t)b * a.ld_tokens;
 #pragma unroll 4
         for (uint32_t i = threadIdx.x; i < len; i += THREADS) {
             const uint64_t at = place(__ldg(tok + i));
@@ -102,27 +112,30 @@ __global__ void __launch_bounds__(THREADS) k_adjust_logits(const __grid_constant
         }
     }
     auto first_bias = [&](uint32_t word) { return kBiases - (word >> kPlace & 1023u); };        // kBiases: none of the kept ones
-    if (a.n_bias) {
-        for (uint32_t i = threadIdx.x; i < n_bias; i += THREADS)
-            if (s_at[i] >= 0) {
-                const uint32_t first = first_bias(*(volatile uint32_t *)&s_word[s_at[i]]);
-                if (first != i) s_more[first] = 1;
+    bool again = false;                                         // a token has several biases
+    for (uint32_t i = threadIdx.x; i < n_bias; i += THREADS)
+        if (s_at[i] >= 0) {
+            const uint32_t first = first_bias(*(volatile uint32_t *)&s_word[s_at[i]]);
+            if (first != i) {
+                s_more[first] = 1;
+                again = true;
             }
-        for (uint32_t i = kBiases + threadIdx.x; i < a.n_bias; i += THREADS) {
-            const uint64_t at = place(__ldg(bias_ids + i));
-            if (at < CHUNK) atomicOr(&s_word[at], kBiased);
         }
-        __syncthreads();
+    for (uint32_t i = kBiases + threadIdx.x; i < a.n_bias; i += THREADS) {
+        const uint64_t at = place(__ldg(bias_ids + i));
+        if (at < CHUNK) atomicOr(&s_word[at], kBiased);
+    }
+    if (__syncthreads_or(again)) {
         for (uint32_t i = threadIdx.x; i < n_bias; i += THREADS)
             if (s_more[i]) {                                    // in order: the same sum every time
                 const int32_t at = s_at[i];
                 float sum = s_bias[i];
 #pragma unroll 8
                 for (uint32_t k = i + 1; k < n_bias; ++k) sum = s_at[k] == at ? sum + s_bias[k] : sum;
-                s_bias[i] = sum;                                // (read by this thread alone so far)
+                s_bias[i] = sum;                                // (no other thread reads it for its own sum)
             }
+        __syncthreads();
     }
-    __syncthreads();
     auto one = [&](float y, uint32_t i) {
         const uint32_t w = s_word[i], count = w & kCount;
         if (w) {

@@ -13,7 +13,17 @@ All three live on the GPU and are read when the kernels run: nothing waits for t
 hold when its graph is replayed.  Rows behind the last sequence are left as they were.  No counterpart in the reference,
 which leaves cache, attention and sampling to Hugging Face's ``generate`` (tests/test_rans_pytorch_runtime.py:89-118).
 
-Calls are queued on the current stream of the cache's device, whichever device is current.
+Calls are queued on the current stream of the cache's device, whichever device is current.  A kernel whose internal wait ran
+out leaves a code that ``check_status`` raises.  Argument errors raise ValueError or RuntimeError before anything is queued.
+
+    cache = PagedKVCache(num_pages=4096, page_size=64, n_kv=8, head_dim=128, bits=4)       # one for each layer
+    # prompts: T rows, q_starts says whose
+    q = rope_paged_append(q, k, v, cos, sin, cache, block_table, kv_lens, q_starts)
+    o = paged_attention(q, cache, block_table, kv_lens, q_starts, max_q_len=longest)
+    # a decode step: one row per sequence, kv_lens already counts it
+    q = rope_paged_append(q, k, v, cos, sin, cache, block_table, kv_lens)
+    o = paged_attention(q, cache, block_table, kv_lens)
+    logits = adjust_logits(logits, tokens, lens, prompt_lens, repetition=r, mask=allowed)   # before ops.greedy_step
 """
 import torch
 
@@ -64,6 +74,7 @@ def rope_paged_append(q, k, v, cos, sin, cache, block_table, kv_lens, q_starts=N
 
     A cache of 4 bits takes of each 64 channels (keys: after rotation and rounding to bf16) lowest = min, step =
     bf16((max - min) / 15) and code = round((x - lowest) / step); a NaN, or a span that is not finite, makes the group NaN.
+    ``out``: all of a contiguous q, or a contiguous tensor apart from q, k and v.
     Tokens whose position is negative or past the tables get zero queries and go nowhere; so do keys and values whose
     position has no page.  No two tokens of a call may go to the same place."""
     return cache._handle.append(q, k, v, cos, sin, block_table, kv_lens, q_starts, out)
@@ -82,7 +93,8 @@ def paged_attention(q, cache, block_table, kv_lens, q_starts=None, max_q_len=0, 
 
     ``window`` > 0: a token at position i sees positions j with i - j < window, and those with j < ``sinks``.  A token that
     sees nothing (no tokens, no pages) gets zeros.  ``max_q_len``: no sequence has more new tokens than that, 0 if it is not
-    known; it chooses between kernels, and a longer sequence is served all the same.  ``scale``: head_dim ** -0.5.
+    known; it chooses between kernels, and a longer sequence is served all the same.  ``scale``: head_dim ** -0.5 if not given.
+    ``out``: rows that do not overlap q, 16-byte aligned (columns of a wider matrix included).
 
     Where several new tokens of one sequence stand in one call, an infinity or a NaN in a value that a later one sees may
     reach the earlier ones; what lies behind a sequence's end, outside everyone's window or on no page reaches nobody."""
@@ -99,5 +111,6 @@ def adjust_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=N
         -inf for tokens whose bit (token % 32 of mask[b, token // 32]) is 0
 
     tokens, bias_ids int64; lens, prompt_lens, mask int32; the rest float32.  What is not given is left out; without
-    prompt_lens all of the history counts; ids outside [0, V) are passed over.  ``out`` may be ``logits``."""
+    prompt_lens all of the history counts; ids outside [0, V) are passed over; histories of less than 2^20 tokens.  ``out`` may
+    be ``logits``; otherwise it does not overlap them."""
     return _lib.host().adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, mask, out)

@@ -555,3 +555,122 @@ def test_adjust_logits_of_strided_rows_and_extremes():
     a = ci().adjust_logits(x, hist, i32([20, 20]), presence=one)
     assert float(a[0, 2]) == -float("inf") and float(a[1, 4]) == -1.0 and float(a[1, 20]) == 0.0
     assert ci().adjust_logits(x, hist, i32([2 ** 31 - 1, -5]), presence=one)[1].eq(0).all()     # lengths outside the row
+
+
+# ---------------------------------------------------------------------------------------------- together
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_run_of_them(bits):
+    """Prompts of three lengths, then steps that grow past their pages: append, attention, adjusted logits, the token picked."""
+    c, g = ci(), gen(31)
+    B, d, n_q, n_kv, page, V = 3, 64, 4, 2, 16, 512
+    new = [37, 130, 5]
+    E = (0.7 * rnd(g, V, (n_q + 2 * n_kv) * d)).to(torch.bfloat16).to(DEV)
+    W = (0.2 * rnd(g, n_q * d, V)).to(torch.bfloat16).to(DEV)
+    cos, sin = rope_tables(200, d)
+    cache = make_cache(g, 20, page, n_kv, d, bits)
+    table = make_table(g, [n + 20 for n in new], page, 20)
+    history = torch.zeros(B, 200, dtype=torch.int64, device=DEV)
+    for b, n in enumerate(new):
+        history[b, :n] = torch.randint(0, V, (n,), generator=g).to(DEV)
+    kv = torch.tensor(new, dtype=torch.int32, device=DEV)
+    prompt_lens = kv.clone()
+    r, p = torch.full((B,), 1.3, device=DEV), torch.full((B,), 0.2, device=DEV)
+    mask = torch.randint(-2 ** 31, 2 ** 31, (B, V // 32), generator=g).to(torch.int32).to(DEV)
+    tok, pos, done = torch.zeros(B, dtype=torch.int64, device=DEV), torch.zeros(1, dtype=torch.int64, device=DEV), torch.zeros(1, dtype=torch.int64, device=DEV)
+    picked, ticket = torch.zeros(B, 10, dtype=torch.int64, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    starts = starts_of(new)
+    ids = torch.cat([history[b, :n] for b, n in enumerate(new)])
+    for step in range(5):
+        x = E[ids]
+        q, k, v = x[:, :n_q * d], x[:, n_q * d:(n_q + n_kv) * d], x[:, (n_q + n_kv) * d:]
+        q = c.rope_paged_append(q, k, v, cos, sin, cache, table.to(DEV), kv, starts)
+        o = c.paged_attention(q, cache, table.to(DEV), kv, starts, max_q_len=max(new) if step == 0 else 1)
+        want, bound = ref.attention(q, cache, table, kv.tolist(), starts)
+        assert bool(((o.double().view_as(want) - want).abs() <= bound).all())
+        last = o if step else o[(starts[1:] - 1).long()]
+        logits = last @ W
+        got = c.adjust_logits(logits, history, kv, prompt_lens, repetition=r, presence=p, mask=mask)
+        assert bf16_close(got, ref.adjust(logits.cpu(), history.cpu(), kv.cpu(), prompt_lens.cpu(), r.cpu(), p.cpu(), mask=mask.cpu()))
+        c.ops.greedy_step(got, tok, pos, done, picked, ticket)
+        assert torch.equal(tok, got.float().argmax(1)) and torch.equal(picked[:, step + 1], tok)
+        history[torch.arange(B), kv.long()] = tok
+        kv += 1
+        starts, ids = None, tok.clone()
+    gk, _ = c.paged_gather(cache, table.to(DEV), kv - 1, starts_of((kv - 1).tolist()), int((kv - 1).sum()))
+    assert gk.shape == (int((kv - 1).sum()), n_kv, d)
+
+
+def test_outputs_that_overlap_inputs():
+    c, g = ci(), gen(33)
+    d, T = 64, 4
+    cache = make_cache(g, 4, 16, 1, d, 16)
+    table, kv = i32([[0], [1], [2], [3]]), i32([3, 1, 9, 16])
+    cos, sin = rope_tables(16, d)
+    qkv = rnd(g, T, 4 * d).to(torch.bfloat16).to(DEV)
+    q, k, v = qkv[:, :2 * d], qkv[:, 2 * d:3 * d], qkv[:, 3 * d:]
+    own = q.contiguous()
+    want = c.rope_paged_append(q, k, v, cos, sin, cache, table, kv)
+    assert torch.equal(c.rope_paged_append(own, k, v, cos, sin, cache, table, kv, out=own).view_as(want), want)      # all of q
+    flat = torch.zeros(3 * T * d, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="overlaps"):
+        c.rope_paged_append(flat[:2 * T * d].view(T, 2 * d), k, v, cos, sin, cache, table, kv, out=flat[d:d + 2 * T * d].view(T, 2 * d))
+    with pytest.raises(ValueError, match="overlaps"):
+        c.rope_paged_append(qkv.view(2 * T, 2 * d)[:T], k, v, cos, sin, cache, table, kv, out=qkv.view(2 * T, 2 * d)[:T])
+    want = c.paged_attention(q, cache, table, kv)
+    assert torch.equal(c.paged_attention(q, cache, table, kv, out=qkv[:, 2 * d:]), want)        # other columns of the same rows
+    with pytest.raises(ValueError, match="overlaps"):
+        c.paged_attention(q, cache, table, kv, out=q)
+    with pytest.raises(ValueError, match="overlaps"):
+        c.paged_attention(q, cache, table, kv, out=qkv[:, d:3 * d])
+    x = rnd(g, 3, 100).to(torch.bfloat16).to(DEV)
+    with pytest.raises(ValueError, match="overlaps"):
+        c.adjust_logits(x[:2], out=x[1:])
+
+
+def test_a_tensor_on_the_wrong_device():
+    c, g = ci(), gen(35)
+    cache = make_cache(g, 4, 16, 1, 64, 16)
+    q, table, kv = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device=DEV), i32([[0], [1]]), i32([3, 1])
+    for args in ((q.cpu(), cache, table, kv), (q, cache, table.cpu(), kv), (q, cache, table, kv.cpu())):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            c.paged_attention(*args)
+    host = c.PagedKVCache(4, 16, 1, 64, device="cpu")
+    with pytest.raises(RuntimeError):
+        c.paged_attention(q, host, table, kv)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_prompts_in_a_graph_beside_eager_ones(bits):
+    """A captured call of prompts and steps, replayed with other lengths on its stream while another stream makes the same calls."""
+    c, g = ci(), gen(37)
+    B, d, n_q, n_kv, page = 4, 128, 4, 1, 32
+    cache, table = make_cache(g, 80, page, n_kv, d, bits), make_table(g, [600] * B, page, 80)
+    q = rnd(g, 400, n_q, d).to(torch.bfloat16).to(DEV)
+    t, kv, starts = table.to(DEV), i32([500, 40, 300, 100]), starts_of([150, 1, 90, 100])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph, o = torch.cuda.CUDAGraph(), torch.full((400, n_q * d), 7.0, dtype=torch.bfloat16, device=DEV)
+    c.paged_attention(q, cache, t, kv, starts, out=o)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        c.paged_attention(q, cache, t, kv, starts, out=o)
+    for lens, new in (([500, 40, 300, 100], [150, 1, 90, 100]), ([600, 2, 1, 17], [280, 2, 1, 17]), ([0, 0, 0, 590], [0, 0, 0, 399])):
+        kv.copy_(i32(lens))
+        starts.copy_(starts_of(new))
+        o.fill_(7.0)
+        torch.cuda.synchronize()
+        eager = [c.paged_attention(q, cache, t, kv, starts, out=torch.full_like(o, 7.0)) for _ in range(3)]
+        with torch.cuda.stream(side):
+            graph.replay()
+        eager += [c.paged_attention(q, cache, t, kv, starts, out=torch.full_like(o, 7.0)) for _ in range(3)]
+        torch.cuda.synchronize()
+        want, bound = ref.attention(q, cache, table, lens, starts)
+        n = sum(new)
+        assert bool(((o[:n].double().view_as(want[:n]) - want[:n]).abs() <= bound[:n]).all()) and bool((o[n:] == 7).all())
+        assert all(torch.equal(e, o) for e in eager)
+    assert _status() is None
+
+
+def _status():
+    return ci().check_status()
