@@ -22,11 +22,12 @@ struct PagedBatch {
 };
 
 // How the prompts' kernel (paged_prompt.cu) shares its work, made on the device by k_paged_join, which runs before it.  An item is
-// per_item tokens of a sequence for one key/value head, a block's work.  Where items are few, those with more key tiles than a
-// multiprocessor's share of all of them are cut into pieces no shorter than the share: as many pieces as there are
-// multiprocessors at most, all at once.  (Pieces no longer than the share would be up to one more for every item, and a second
-// round of blocks.)  Not shorter than kFewest either: a piece begins with queries and first keys one after the other and ends
-// with k_prompt_join.  32 tokens behind 8000 others, eight sequences of it: XXXX us, uncut YYYY.
+// per_item tokens of a sequence for one key/value head.  Items with many more key tiles than others are cut into pieces: no shorter
+// than a multiprocessor's share of all tiles where there are no more items than multiprocessors, so that the pieces are not
+// more either and run at once (pieces no longer than the share would be up to one more for every item, a second round: 16
+// sequences of 32 new tokens and 2048 in all 67 us instead of 42); half of that where a multiprocessor has several items anyway.
+// Not shorter than kFewest either: a piece begins with queries and first keys one after the other and ends with k_prompt_join.
+// 32 tokens behind 8000 others, eight sequences of it: 79 us, uncut 108; 64 tokens behind 32000: 87 us, uncut 402.
 constexpr uint32_t kKt = 128;                // positions per key tile
 constexpr uint32_t kFewest = 4;
 struct PromptPlan {
@@ -99,14 +100,19 @@ __device__ __forceinline__ void plan_prompts(const PagedBatch &p, const PromptPl
         if (l.window) n = min(n, ((uint32_t)l.sinks + kKt - 1) / kKt + ((uint32_t)l.window + l.per_item) / kKt + 2);    // (below 2^31 each)
         tiles = max(n, 1u);
     };
-    float all = 0.f;
+    float all = 0.f, blocks = 0.f;
     for (uint32_t b = b0; b < b1; ++b) {
         at(b);
         all += (float)items * (float)tiles;
+        blocks += (float)items;
     }
-    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(kFull, all, o);
-    // one more than the share: sums in fp32 may be short of it by less, where anything is cut (fewer than 2^23 tiles)
-    const uint32_t most = max((uint32_t)fminf(all * (float)p.n_kv / (float)l.sms, 1e9f) + 1, kFewest);
+    for (int o = 16; o; o >>= 1) {
+        all += __shfl_xor_sync(kFull, all, o);
+        blocks += __shfl_xor_sync(kFull, blocks, o);
+    }
+    const float share = all * (float)p.n_kv / (float)l.sms;
+    // one more: sums in fp32 may be short of the share by less, where anything is cut (fewer than 2^23 tiles)
+    const uint32_t most = max((uint32_t)fminf(blocks * (float)p.n_kv > (float)l.sms ? 0.5f * share : share, 1e9f) + 1, kFewest);
     uint32_t mine = 0, cut = 0;                                  // pieces; slots, and in the upper half cut items
     for (uint32_t b = b0; b < b1; ++b) {
         at(b);

@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
 // Joins the parts of an item that several blocks had: block c has the item that block c of the attention began, all rows at once, if
 // that has few parts.  Items of many parts are few, and the blocks share their rows: a block per row, its threads over the
 // parts (5 items of 59 parts, heads of 256: the join's 55 us become XXXX).  Everything in a fixed order: the same sum every time.
-constexpr int32_t kFewParts = 8;
+constexpr int32_t kFewParts = 16, kAtOnce = 8;
 
 template <int D, int RT>
 __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PromptPlan plan) {
@@ -616,27 +616,35 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Page
         for (uint32_t x = threadIdx.x; x < RT * kLanes; x += 256) {
             const uint32_t r = x / kLanes, c = x % kLanes * 4, row = (uint32_t)head.w + r;
             if ((int32_t)row >= head.z) continue;
-            float2 ml[kFewParts];                               // asked for at once, (max, sum) and outputs
-            float4 z[kFewParts];
-#pragma unroll
-            for (int32_t i = 0; i < kFewParts; ++i) {
-                ml[i] = make_float2(kNone, 0.f);
-                z[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (i < parts) {
-                    ml[i] = __ldcg(reinterpret_cast<const float2 *>(a.ml + (slot(blockIdx.x, i) * RT + r) * 2));
-                    z[i] = __ldcg(reinterpret_cast<const float4 *>(a.partial + (slot(blockIdx.x, i) * RT + r) * D + c));
-                }
-            }
             float M = kNone, L = 0.f;
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (int32_t i0 = 0; i0 < parts; i0 += kAtOnce) {
+                float2 ml[kAtOnce];                             // asked for together: (max, sum) and outputs
+                float4 z[kAtOnce];
 #pragma unroll
-            for (int32_t i = 0; i < kFewParts; ++i) M = fmaxf(M, ml[i].x);
-            const float safe = M == kNone ? 0.f : M;
+                for (int32_t i = 0; i < kAtOnce; ++i) {
+                    ml[i] = make_float2(kNone, 0.f);
+                    z[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (i0 + i < parts) {
+                        ml[i] = __ldcg(reinterpret_cast<const float2 *>(a.ml + (slot(blockIdx.x, i0 + i) * RT + r) * 2));
+                        z[i] = __ldcg(reinterpret_cast<const float4 *>(a.partial + (slot(blockIdx.x, i0 + i) * RT + r) * D + c));
+                    }
+                }
+                float most = M;
 #pragma unroll
-            for (int32_t i = 0; i < kFewParts; ++i) {
-                const float e = ml[i].x == kNone ? 0.f : ex2(ml[i].x - safe);
-                L += e * ml[i].y;
-                y.x += e * z[i].x; y.y += e * z[i].y; y.z += e * z[i].z; y.w += e * z[i].w;
+                for (int32_t i = 0; i < kAtOnce; ++i) most = fmaxf(most, ml[i].x);
+                if (most == kNone) continue;
+                const float down = M == kNone ? 0.f : ex2(M - most);
+                M = most;
+                L *= down;
+                y.x *= down; y.y *= down; y.z *= down; y.w *= down;
+#pragma unroll
+                for (int32_t i = 0; i < kAtOnce; ++i) {
+                    const float e = ml[i].x == kNone ? 0.f : ex2(ml[i].x - M);
+                    L += e * ml[i].y;
+                    y.x += e * z[i].x; y.y += e * z[i].y; y.z += e * z[i].z; y.w += e * z[i].w;
+                }
             }
             store(head, kvh, row, c, y, M == kNone ? 0.f : 1.f / L);
         }

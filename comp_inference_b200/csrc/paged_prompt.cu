@@ -864,7 +864,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     if (warp == Sh::kMma) tmem_dealloc(tmem, 512);
 }
 
-// Joins the pieces of an item, 32 rows to a block: D / 4 threads to a row.  In order: the same sum every time.
+// Joins the pieces of an item, kJoinRows rows to a block: D / 4 threads to a row.  In order: the same sum every time.
+constexpr uint32_t kJoinRows = 16;
 template <int D>
 __global__ void __launch_bounds__(256) k_prompt_join(const __grid_constant__ PromptArgs a) {
     constexpr uint32_t NT = PromptShape<D, 16>::NT, kLanes = D / 4, kRows = 256 / kLanes;
@@ -877,23 +878,40 @@ __global__ void __launch_bounds__(256) k_prompt_join(const __grid_constant__ Pro
     if (blockIdx.x / a.p.n_kv >= (uint32_t)cuts) return;
     const uint32_t item = (uint32_t)w0.y, pieces = (uint32_t)w0.w, slot = (uint32_t)w1.x, q_len = (uint32_t)w1.z;
     const int32_t q0 = w1.y;
-    for (uint32_t r = blockIdx.y * 32 + threadIdx.x / kLanes; r < blockIdx.y * 32 + 32; r += kRows) {
+    for (uint32_t r = blockIdx.y * kJoinRows + threadIdx.x / kLanes; r < (blockIdx.y + 1) * kJoinRows; r += kRows) {
         const uint32_t t = r / 128, tok = r % 128 / a.group, c = threadIdx.x % kLanes * 4;
         const uint32_t at = (item * NT + t) * a.tt + tok;     // the row's token
         if (tok >= a.tt || at >= q_len) continue;
         auto part = [&](uint32_t i) { return ((size_t)(slot + i) * a.p.n_kv + kvh) * (NT * 128) + r; };
         float M = -INFINITY, L = 0.f;
-#pragma unroll 8
-        for (uint32_t i = 0; i < pieces; ++i) M = fmaxf(M, __ldcg(a.ml + part(i) * 2));
-        const float safe = M == -INFINITY ? 0.f : M;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (uint32_t i = 0; i < pieces; ++i) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.ml + part(i) * 2));
-            const float4 z = __ldcg(reinterpret_cast<const float4 *>(a.partial + part(i) * D + c));
-            const float e = ml.x == -INFINITY ? 0.f : ex2f(ml.x - safe);
-            L += e * ml.y;
-            y.x += e * z.x; y.y += e * z.y; y.z += e * z.z; y.w += e * z.w;
+#pragma unroll 1
+        for (uint32_t i0 = 0; i0 < pieces; i0 += 8) {
+            float2 ml[8];                                       // asked for together: (max, sum) and outputs
+            float4 z[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                ml[i] = make_float2(-INFINITY, 0.f);
+                z[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i0 + i < pieces) {
+                    ml[i] = __ldcg(reinterpret_cast<const float2 *>(a.ml + part(i0 + i) * 2));
+                    z[i] = __ldcg(reinterpret_cast<const float4 *>(a.partial + part(i0 + i) * D + c));
+                }
+            }
+            float most = M;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) most = fmaxf(most, ml[i].x);
+            if (most == -INFINITY) continue;
+            const float down = M == -INFINITY ? 0.f : ex2f(M - most);
+            M = most;
+            L *= down;
+            y.x *= down; y.y *= down; y.z *= down; y.w *= down;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const float e = ml[i].x == -INFINITY ? 0.f : ex2f(ml[i].x - M);
+                L += e * ml[i].y;
+                y.x += e * z[i].x; y.y += e * z[i].y; y.z += e * z[i].z; y.w += e * z[i].w;
+            }
         }
         const float inv = M == -INFINITY ? 0.f : 1.f / L;
         *reinterpret_cast<uint2 *>(a.out + (int64_t)(q0 + (int32_t)at) * a.ldo + (size_t)(kvh * a.group + r % 128 % a.group) * D + c) =
@@ -901,7 +919,7 @@ __global__ void __launch_bounds__(256) k_prompt_join(const __grid_constant__ Pro
     }
 }
 
-static size_t prompt_slot_rows(uint32_t head_dim) { return (size_t)sm_count() * (head_dim == 256 ? 128 : 256); }     // of all slots
+static size_t prompt_slot_rows(uint32_t head_dim) { return 2 * (size_t)sm_count() * (head_dim == 256 ? 128 : 256); }     // of all slots
 
 PromptPlan prompt_plan(uint32_t head_dim, uint32_t page_size, uint32_t n_kv, const ci_paged_batch *b, uint32_t group, int32_t window,
                        int32_t sinks, uint32_t min_rows, void *workspace) {
@@ -912,15 +930,15 @@ PromptPlan prompt_plan(uint32_t head_dim, uint32_t page_size, uint32_t n_kv, con
     l.sms = (uint32_t)sm_count();
     // Lengths are the device's to know: items and pieces as many as there can be, blocks without one leave at once.
     l.may_cut = (uint64_t)b->max_pages * page_size > kFewest * kKt;
-    l.count = b->T / l.per_item + b->B + (l.may_cut ? l.sms / n_kv : 0);
+    l.count = b->T / l.per_item + b->B + (l.may_cut ? 2 * l.sms / n_kv : 0);
     l.window = window;
     l.sinks = sinks;
     l.cuts = (int4 *)workspace;
-    l.pieces = l.cuts + ((size_t)l.sms / 2 + 2) * 2;
+    l.pieces = l.cuts + ((size_t)l.sms + 2) * 2;
     return l;
 }
 size_t prompt_workspace_bytes(uint32_t head_dim, const PromptPlan &l) {
-    return (((size_t)l.sms / 2 + 2 + l.count) * 2) * sizeof(int4) + prompt_slot_rows(head_dim) * (2 + (size_t)head_dim) * sizeof(float);
+    return (((size_t)l.sms + 2 + l.count) * 2) * sizeof(int4) + prompt_slot_rows(head_dim) * (2 + (size_t)head_dim) * sizeof(float);
 }
 
 template <int D, int BITS>
@@ -942,7 +960,7 @@ static int launch_prompt(const PromptArgs &a, const PromptPlan &l, const CUtenso
     cfg.numAttrs = 1;
     CI_CUDA(cudaLaunchKernelEx(&cfg, k_paged_prompt<D, BITS>, a, qm, km, vm));
     if (!l.may_cut) return CI_OK;
-    cfg.gridDim = dim3(l.sms / 2 + 1, Sh::NT * 4);              // (two pieces at least to a cut item)
+    cfg.gridDim = dim3(l.sms + 1, Sh::NT * 128 / kJoinRows);    // (two pieces at least to a cut item)
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     CI_CUDA(cudaLaunchKernelEx(&cfg, k_prompt_join<D>, a));
