@@ -12,6 +12,11 @@
 // The work of all sequences, key heads and groups of queries is one line of tiles that the blocks share evenly, so that
 // one long sequence among short ones, or a single sequence, fills the machine; what a block boundary cuts is joined by
 // k_paged_join from (max, sum, output) of the parts.  Lengths are read on the device: a captured call serves any.
+//
+// What bounds it: in bf16 memory (32 sequences of 1 to 16000 tokens, 251 MB: 50 us, 5.0 TB/s, 45 of them this kernel); heads of 64
+// and small pages latency (67 MB of a window: 18 us); 4 bits the instructions that turn codes into operands, 7 for eight keys and 11
+// for eight values beside the permutes (417 MB: 142 us, 2.9 TB/s, integer pipe 59 % and issue slots 54 % of the time; four or five
+// blocks of fewer registers on a multiprocessor 151 to 191 us); a short step the launches (513 tokens of 32 heads: 10.9 us).
 #include "paged.cuh"
 #include "ptx.cuh"
 
@@ -585,7 +590,7 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
 
 // Joins the parts of an item that several blocks had: block c has the item that block c of the attention began, all rows at once, if
 // that has few parts.  Items of many parts are few, and the blocks share their rows: a block per row, its threads over the
-// parts (5 items of 59 parts, heads of 256: the join's 55 us become XXXX).  Everything in a fixed order: the same sum every time.
+// parts (5 items of 59 parts, heads of 256: the join's 55 us became 13).  Everything in a fixed order: the same sum every time.
 constexpr int32_t kFewParts = 16, kAtOnce = 8;
 
 template <int D, int RT>

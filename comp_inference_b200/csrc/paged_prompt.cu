@@ -8,15 +8,24 @@
 //   O += P . V         P from tensor memory, V as it lies (its rows are the k index: an MN-major operand), O in tensor memory
 // While one tile's threads are at their exponentials the tensor cores work for the other; the weights are handed over in two
 // halves.  The maximum that a row's weights refer to moves only when it is exceeded by 2^8 (kLazy), so O is rarely rescaled; the
-// row's own thread does that too, between two products, when nothing else touches it.  Tiles that no row sees are not visited; a page that does not exist
-// is fetched from outside the tensor, which gives zeros.
+// row's own thread does that too, between two products, when nothing else touches it.  Tiles that no row sees are not
+// visited; a page that does not exist is fetched from outside the tensor, which gives zeros.
+//
+// Blocks stay, one on each multiprocessor, and take piece after piece of the plan that k_paged_join has made (PromptPlan): one warp
+// fetches the next piece and says what it sees, one issues the TMA copies, one per query tile the products, and each goes on to the
+// next piece when its own part is done, so that queries, first keys and first scores of the next are there when the rows of
+// this one are written (4096 tokens, 32 heads of 128 over 8: a block for each piece 135 us, 127 so; six prompts of 1024, 64 heads of
+// 64 over 16, under a window of 256: 123 and 89).  mbarriers connect the roles.  All waits are bounded: on expiry a role sets the
+// status word and the abort flag, and everyone leaves.
 //
 // A cache of 4 bits is turned into fp16 on its way into shared memory by four or eight warps, so that what codes stand for, and the
 // weights, are rounded by 2^-12 and not 2^-9 (error of a prompt's outputs against 64 bits 0.0017 instead of 0.0034; bf16's own
 // rounding of the result is 0.0016).  fp16 has no range for that by itself: every key tile is scaled by the power of two that
 // its largest value asks for, the values by one that only grows, O following it, and a query row by its own.
 //
-// One warp per query tile issues the products, one the TMA copies; mbarriers connect them.  All waits are bounded: on expiry a role sets the status word and the abort flag, and everyone leaves.
+// What bounds it: in bf16 the chain from a tile's scores over its exponentials to its product, with two tiles in turn (tensor
+// pipe 61 % active, issue slots 47 %, special functions 47 %; 16001 tokens under a window of 4096: 772 us, 1214 TFLOP/s, 0.73 of the
+// measured rate); in 4 bits the arithmetic of turning codes (4096 tokens 197 us, without it 158; tensor pipe 35 %, issue slots 53 %).
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -136,7 +145,7 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // 2^x of two values, x <= 2^6, in the fused multiply-add units: the integer next to x goes into the exponent field, 2^f for the rest
 // in [-1/2, 1/2] is a polynomial of degree 3 fitted for the smallest largest relative error, 7.5e-5, a fiftieth of what rounding to
 // bf16 loses.  The special-function unit makes four results per cycle and scheduler; a quarter of the weights comes from here
-// (4096 tokens, 32 heads of 128 over 8: 160.6 us; none of them 167.6, half 181.8).  For x of
+// (4096 tokens, 32 heads of 128 over 8: 160.6 us when it was tried, none of them 167.6, half 181.8).  For x of
 // -126 and less it gives 2^-126, not 0: not for tiles with hidden scores.
 constexpr float kExp0 = 0.99992812f, kExp1 = 0.69326097f, kExp2 = 0.24261075f, kExp3 = 0.05517141f;
 __device__ __forceinline__ void ex2_poly(uint64_t x, float &r0, float &r1) {
@@ -267,261 +276,260 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         q_count += kt.n > 0;
     };
 
+    if (Sh::kMove) {                                            // by warpgroups: 4 bits have some of producers, one for the products
+        if (warp < 4 * NT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::kSoftRegs));
+        else if (BITS == 4 && warp >= Sh::kMma) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kMmaRegs));
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kProdRegs));
+    }
     if (warp < 4 * NT) {
-        if (Sh::kMove) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::kSoftRegs));
         // =========================== softmax: one thread per query row ===============================================
         const uint32_t t = warp >> 2, w = warp & 3, row = w * 32 + lane;
         const uint32_t tok = row / a.group, head = row % a.group;
         uint32_t turn = 0;                                      // products of all pieces so far
         bool ok = true;
         for (uint32_t k = 0; ok && get_item(k); ++k) {
-        QueryTile q = qt[0];
-        if (NT == 2 && t == 1) q = qt[NT - 1];
-        const int32_t pos = q.p0 + (int32_t)tok, last = min(pos, p.cap - 1);
-        const uint32_t s_addr = tmem + ((w * 32u) << 16) + t * kKt, o_addr = tmem + ((w * 32u) << 16) + Sh::cO + t * D;
-        float m = -INFINITY;
-        constexpr int kSums = BITS == 16 ? 4 : 2;
-        uint64_t l2[kSums] = {};                                // sums of weights, two in each
-        bool done = false;                                      // a product of this piece has been
-        const uint32_t ids = kKt >> p.page_shift;               // pages of a tile
-        auto page_id = [&](int32_t i) {                         // of tile i, one per lane; 0 where there is none to ask for
-            const int32_t at = kt.first(i) + (int32_t)(lane << p.page_shift);
-            return i < kt.n && lane < ids && at < kt.hi ? __ldg(p.table + (size_t)b * p.table_stride + ((uint32_t)at >> p.page_shift)) : 0;
-        };
-        int32_t id = page_id(0);
-        float scale = a.scale_log2;
-        volatile const int32_t *s_scale = reinterpret_cast<volatile const int32_t *>(smem + Sh::oBar + Sh::oScale);
-        int32_t v_exp = 0;                                      // O stands for O 2^v_exp
-        if (BITS == 4 && kt.n > 0) {                            // this row of Q to fp16, its largest value below 2^15
-            ok = __all_sync(kFull, mbar_wait(bar(Sh::bQ), q_count & 1));
-            if (!ok) give_up(18);
-            const uint32_t q_s = smem_s + Sh::oQ + t * Sh::kTile + row * 128;
-            auto chunk = [&](uint32_t c) { return q_s + (c / 8) * Sh::kBlock + ((c % 8 ^ (row & 7)) << 4); };
-            float big = 0.f;
+            QueryTile q = qt[0];
+            if (NT == 2 && t == 1) q = qt[NT - 1];
+            const int32_t pos = q.p0 + (int32_t)tok, last = min(pos, p.cap - 1);
+            const uint32_t s_addr = tmem + ((w * 32u) << 16) + t * kKt, o_addr = tmem + ((w * 32u) << 16) + Sh::cO + t * D;
+            float m = -INFINITY;
+            constexpr int kSums = BITS == 16 ? 4 : 2;
+            uint64_t l2[kSums] = {};                                // sums of weights, two in each
+            bool done = false;                                      // a product of this piece has been
+            const uint32_t ids = kKt >> p.page_shift;               // pages of a tile
+            auto page_id = [&](int32_t i) {                         // of tile i, one per lane; 0 where there is none to ask for
+                const int32_t at = kt.first(i) + (int32_t)(lane << p.page_shift);
+                return i < kt.n && lane < ids && at < kt.hi ? __ldg(p.table + (size_t)b * p.table_stride + ((uint32_t)at >> p.page_shift)) : 0;
+            };
+            int32_t id = page_id(0);
+            float scale = a.scale_log2;
+            volatile const int32_t *s_scale = reinterpret_cast<volatile const int32_t *>(smem + Sh::oBar + Sh::oScale);
+            int32_t v_exp = 0;                                      // O stands for O 2^v_exp
+            if (BITS == 4 && kt.n > 0) {                            // this row of Q to fp16, its largest value below 2^15
+                ok = __all_sync(kFull, mbar_wait(bar(Sh::bQ), q_count & 1));
+                if (!ok) give_up(18);
+                const uint32_t q_s = smem_s + Sh::oQ + t * Sh::kTile + row * 128;
+                auto chunk = [&](uint32_t c) { return q_s + (c / 8) * Sh::kBlock + ((c % 8 ^ (row & 7)) << 4); };
+                float big = 0.f;
 #pragma unroll 4
-            for (uint32_t c = 0; c < D / 8; ++c) {
+                for (uint32_t c = 0; c < D / 8; ++c) {
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) {
-                    const uint32_t x = lds_u32(chunk(c) + 4 * e);
-                    big = fmaxf(big, fmaxf(fabsf(lo_bf16(x)), fabsf(hi_bf16(x))));
-                }
-            }
-            const int32_t e = exponent_of(big) - 15;
-            const float up = power_of_2(-e / 2), up2 = power_of_2(-e - -e / 2);
-#pragma unroll 4
-            for (uint32_t c = 0; c < D / 8; ++c) {
-                uint32_t y[4];
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    const uint32_t x = lds_u32(chunk(c) + 4 * j);
-                    y[j] = pack_f16(lo_bf16(x) * up * up2, hi_bf16(x) * up * up2);
-                }
-                sts_v4(chunk(c), y[0], y[1], y[2], y[3]);
-            }
-            scale *= power_of_2(e / 2) * power_of_2(e - e / 2);
-            fence_async_proxy();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(Sh::bQh));
-        }
-        const float row_scale = scale;
-        for (int32_t i = 0; i < kt.n && ok; ++i) {
-            const uint32_t gone = __ballot_sync(kFull, (uint32_t)id >= p.num_pages);    // one bit per page that does not exist
-            id = page_id(i + 1);
-            if (!kt.seen_by(q, i)) continue;
-            const int32_t f = kt.first(i);
-            const bool edge = gone || f + (int32_t)kKt - 1 > min(q.p0, p.cap - 1) ||
-                              (a.window && f <= q.p1 - a.window && f + (int32_t)kKt > a.sinks);
-            if (!__all_sync(kFull, mbar_wait(bar(Sh::bS + t), turn & 1))) {
-                give_up(11);
-                ok = false;
-                break;
-            }
-            tc_fence_after();
-            float v_down = 1.f;                                 // what O is to be multiplied by for the scale of this tile's V
-            if (BITS == 4) {
-                // The tile of V cannot be replaced before this row's weights are out, so its barrier can be waited on here; the
-                // exponents of the tile were written before it.
-                const uint32_t c = ring0 + 2 * (uint32_t)i + 1, at = c / 2 % 8;
-                if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1))) {
-                    give_up(19);
-                    ok = false;
-                    break;
-                }
-                const int32_t ke = s_scale[at], ve = s_scale[8 + at];
-                scale = fmaxf(row_scale * power_of_2(ke / 2) * power_of_2(ke - ke / 2), 1.2e-38f);
-                v_down = done ? power_of_2(v_exp - ve) : 1.f;
-                v_exp = ve;
-            }
-            const uint64_t scale2 = pair(scale, scale);
-            uint32_t x[Sh::kHeld][32];
-            auto hide = [&](uint32_t (&v)[32], int32_t c) {     // scores of positions that the row does not see
-                const int32_t f32 = f + c * 32;
-                uint32_t seen = low_bits(last + 1 - f32);
-                if (a.window) seen &= ~low_bits(pos - a.window + 1 - f32) | low_bits(a.sinks - f32);
-                if (gone)
-#pragma unroll
-                    for (int j = 0; j < 32; j += 16)
-                        if (gone >> ((uint32_t)(c * 32 + j) >> p.page_shift) & 1) seen &= ~(0xFFFFu << j);
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (!(seen & (1u << j))) v[j] = 0xFF800000u;
-            };
-            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            auto largest = [&](const uint32_t (&v)[32]) {
-#pragma unroll
-                for (int j = 0; j < 32; j += 8)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        mx4[e] = fmaxf(fmaxf(mx4[e], __uint_as_float(v[j + e])), __uint_as_float(v[j + 4 + e]));
-            };
-            auto load = [&](int first) {                        // kHeld groups of 32 scores
-#pragma unroll
-                for (int c = 0; c < Sh::kHeld; ++c) tmem_ld32_start(s_addr + (first + c) * 32, x[c]);
-#pragma unroll
-                for (int c = 0; c < Sh::kHeld; ++c) tmem_ld_wait(x[c]);
-                if (edge)
-#pragma unroll
-                    for (int c = 0; c < Sh::kHeld; ++c) hide(x[c], first + c);
-            };
-#pragma unroll
-            for (int first = 4 - Sh::kHeld; first >= 0; first -= Sh::kHeld) {
-                load(first);
-#pragma unroll
-                for (int c = 0; c < Sh::kHeld; ++c) largest(x[c]);
-            }
-            float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;
-            const bool grow = mx > m + kLazy;
-            if (__any_sync(kFull, grow || v_down != 1.f)) {
-                float c = grow ? ex2f(m - mx) : 1.f;
-                if (grow) m = mx;
-#pragma unroll
-                for (int e = 0; e < kSums; ++e) l2[e] = fma2(l2[e], pair(c, c), 0);
-                c *= v_down;
-                if (done) {
-#pragma unroll 1
-                    for (uint32_t j = 0; j < D / 32; ++j) {
-                        uint32_t o[32];
-                        tmem_ld32(o_addr + j * 32, o);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * c);
-                        tmem_st32(o_addr + j * 32, o);
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        const uint32_t x = lds_u32(chunk(c) + 4 * e);
+                        big = fmaxf(big, fmaxf(fabsf(lo_bf16(x)), fabsf(hi_bf16(x))));
                     }
                 }
-            }
-            // Rows of V that no query of the block sees become zeros: 0 times what lies there need not be 0.  A thread has the row of
-            // its number; both query tiles write them, as neither waits for the other.  (The copying warp alone took 15 us over a
-            // tile: a prompt of 16001 under a window of 4096 1225 us instead of 780.)
-            if (BITS == 16 && (f + (int32_t)kKt > kt.hi || (a.window && f < kt.lo && f + (int32_t)kKt > a.sinks))) {
-                const uint32_t c = ring0 + 2 * (uint32_t)i + 1;
-                if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1))) {
-                    give_up(16);
-                    ok = false;
-                    break;
-                }
-                const int32_t at = f + (int32_t)row;
-                if (at >= kt.hi || (a.window && at < kt.lo && at >= a.sinks)) {
-                    const uint32_t v_s = smem_s + Sh::oRing + (c % NS) * Sh::kTile + row * 128;
+                const int32_t e = exponent_of(big) - 15;
+                const float up = power_of_2(-e / 2), up2 = power_of_2(-e - -e / 2);
+#pragma unroll 4
+                for (uint32_t c = 0; c < D / 8; ++c) {
+                    uint32_t y[4];
 #pragma unroll
-                    for (uint32_t j = 0; j < NB * 8; ++j) sts_v4(v_s + (j / 8) * Sh::kBlock + ((j + row) % 8) * 16, 0, 0, 0, 0);
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const uint32_t x = lds_u32(chunk(c) + 4 * j);
+                        y[j] = pack_f16(lo_bf16(x) * up * up2, hi_bf16(x) * up * up2);
+                    }
+                    sts_v4(chunk(c), y[0], y[1], y[2], y[3]);
                 }
+                scale *= power_of_2(e / 2) * power_of_2(e - e / 2);
                 fence_async_proxy();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(Sh::bQh));
             }
-            const float ref = m == -INFINITY ? 0.f : -m;
-            const uint64_t ref2 = pair(ref, ref);
-            auto weights = [&](auto whole) {                    // whole: no score of the tile is hidden
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c && c % Sh::kHeld == 0) load(c);
-                    const uint32_t(&v)[32] = x[c % Sh::kHeld];
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const uint64_t y = fma2(pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), scale2, ref2);
-                        float e0, e1;
-                        if (decltype(whole)::value && BITS == 16 && j % 4 == 3) {
-                            ex2_poly(y, e0, e1);
-                        } else {
-                            split(y, e0, e1);
-                            e0 = ex2f(e0);
-                            e1 = ex2f(e1);
-                        }
-                        l2[j % kSums] = add2(l2[j % kSums], pair(e0, e1));
-                        pk[j] = BITS == 16 ? pack_bf16(e0, e1) : pack_f16(e0, e1);
-                    }
-                    tmem_st16(s_addr + c * 16, pk);
-                    if (c % 2) {                                    // half of the weights are there
-                        tmem_st_wait();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(bar(Sh::bP + 2 * t + c / 2));
-                    }
+            const float row_scale = scale;
+            for (int32_t i = 0; i < kt.n && ok; ++i) {
+                const uint32_t gone = __ballot_sync(kFull, (uint32_t)id >= p.num_pages);    // one bit per page that does not exist
+                id = page_id(i + 1);
+                if (!kt.seen_by(q, i)) continue;
+                const int32_t f = kt.first(i);
+                const bool edge = gone || f + (int32_t)kKt - 1 > min(q.p0, p.cap - 1) ||
+                                  (a.window && f <= q.p1 - a.window && f + (int32_t)kKt > a.sinks);
+                if (!__all_sync(kFull, mbar_wait(bar(Sh::bS + t), turn & 1))) {
+                    give_up(11);
+                    ok = false;
+                    break;
                 }
-            };
-            if (edge) weights(std::false_type());
-            else weights(std::true_type());
-            done = true;
-            ++turn;
-        }
-        float l = 0.f;
+                tc_fence_after();
+                float v_down = 1.f;                                 // what O is to be multiplied by for the scale of this tile's V
+                if (BITS == 4) {
+                    // The tile of V cannot be replaced before this row's weights are out, so its barrier can be waited on here; the
+                    // exponents of the tile were written before it.
+                    const uint32_t c = ring0 + 2 * (uint32_t)i + 1, at = c / 2 % 8;
+                    if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1))) {
+                        give_up(19);
+                        ok = false;
+                        break;
+                    }
+                    const int32_t ke = s_scale[at], ve = s_scale[8 + at];
+                    scale = fmaxf(row_scale * power_of_2(ke / 2) * power_of_2(ke - ke / 2), 1.2e-38f);
+                    v_down = done ? power_of_2(v_exp - ve) : 1.f;
+                    v_exp = ve;
+                }
+                const uint64_t scale2 = pair(scale, scale);
+                uint32_t x[Sh::kHeld][32];
+                auto hide = [&](uint32_t (&v)[32], int32_t c) {     // scores of positions that the row does not see
+                    const int32_t f32 = f + c * 32;
+                    uint32_t seen = low_bits(last + 1 - f32);
+                    if (a.window) seen &= ~low_bits(pos - a.window + 1 - f32) | low_bits(a.sinks - f32);
+                    if (gone)
 #pragma unroll
-        for (int e = 0; e < kSums; ++e) {
-            float l0, l1;
-            split(l2[e], l0, l1);
-            l += l0 + l1;
-        }
-        // ---- the row's result ----------------------------------------------------------------------------------
-        if (ok && !mbar_wait(bar(Sh::bO + t), k & 1)) { give_up(12); ok = false; }
-        ok = __all_sync(kFull, ok && !*s_abort);
-        if (__all_sync(kFull, ok)) {
-            tc_fence_after();
-            const bool live = tok < a.tt && pos <= q.p1;
-            const float inv = m == -INFINITY ? 0.f : 1.f / l;     // (nothing seen: zeros)
-            const float up = BITS == 4 ? power_of_2(v_exp / 2) : 1.f, up2 = BITS == 4 ? power_of_2(v_exp - v_exp / 2) : 1.f;
-            volatile const int32_t *item = s_items + k % 2 * kItemWords;
-            const uint32_t pieces = (uint32_t)item[kPieces], kvh = head_of(k);
-            const int32_t q_row = first_row_of(k);
-            const size_t part = ((size_t)(uint32_t)item[kSlot] * p.n_kv + kvh) * (NT * 128) + t * 128 + row;
-            if (pieces > 1 && live) *reinterpret_cast<float2 *>(a.ml + part * 2) = make_float2(m, l);
-            uint16_t *dst = a.out + (int64_t)(q_row + (int32_t)(t * a.tt + tok)) * a.ldo + (size_t)(kvh * a.group + head) * D;
+                        for (int j = 0; j < 32; j += 16)
+                            if (gone >> ((uint32_t)(c * 32 + j) >> p.page_shift) & 1) seen &= ~(0xFFFFu << j);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (!(seen & (1u << j))) v[j] = 0xFF800000u;
+                };
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                auto largest = [&](const uint32_t (&v)[32]) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            mx4[e] = fmaxf(fmaxf(mx4[e], __uint_as_float(v[j + e])), __uint_as_float(v[j + 4 + e]));
+                };
+                auto load = [&](int first) {                        // kHeld groups of 32 scores
+#pragma unroll
+                    for (int c = 0; c < Sh::kHeld; ++c) tmem_ld32_start(s_addr + (first + c) * 32, x[c]);
+#pragma unroll
+                    for (int c = 0; c < Sh::kHeld; ++c) tmem_ld_wait(x[c]);
+                    if (edge)
+#pragma unroll
+                        for (int c = 0; c < Sh::kHeld; ++c) hide(x[c], first + c);
+                };
+#pragma unroll
+                for (int first = 4 - Sh::kHeld; first >= 0; first -= Sh::kHeld) {
+                    load(first);
+#pragma unroll
+                    for (int c = 0; c < Sh::kHeld; ++c) largest(x[c]);
+                }
+                float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;
+                const bool grow = mx > m + kLazy;
+                if (__any_sync(kFull, grow || v_down != 1.f)) {
+                    float c = grow ? ex2f(m - mx) : 1.f;
+                    if (grow) m = mx;
+#pragma unroll
+                    for (int e = 0; e < kSums; ++e) l2[e] = fma2(l2[e], pair(c, c), 0);
+                    c *= v_down;
+                    if (done) {
 #pragma unroll 1
-            for (uint32_t j = 0; j < D / 32; ++j) {
-                uint32_t o[32];
-                if (done) {
-                    tmem_ld32(o_addr + j * 32, o);
-                } else {
+                        for (uint32_t j = 0; j < D / 32; ++j) {
+                            uint32_t o[32];
+                            tmem_ld32(o_addr + j * 32, o);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * c);
+                            tmem_st32(o_addr + j * 32, o);
+                        }
+                    }
                 }
-                if (live && pieces > 1) {
+                // Rows of V that no query of the block sees become zeros: 0 times what lies there need not be 0.  A thread has the row of
+                // its number; both query tiles write them, as neither waits for the other.  (The copying warp alone took 15 us over a
+                // tile: a prompt of 16001 under a window of 4096 1225 us instead of 780 then.)
+                if (BITS == 16 && (f + (int32_t)kKt > kt.hi || (a.window && f < kt.lo && f + (int32_t)kKt > a.sinks))) {
+                    const uint32_t c = ring0 + 2 * (uint32_t)i + 1;
+                    if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1))) {
+                        give_up(16);
+                        ok = false;
+                        break;
+                    }
+                    const int32_t at = f + (int32_t)row;
+                    if (at >= kt.hi || (a.window && at < kt.lo && at >= a.sinks)) {
+                        const uint32_t v_s = smem_s + Sh::oRing + (c % NS) * Sh::kTile + row * 128;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        *reinterpret_cast<float4 *>(a.partial + part * D + j * 32 + e * 4) =
-                            make_float4(__uint_as_float(o[4 * e]) * up * up2, __uint_as_float(o[4 * e + 1]) * up * up2,
-                                        __uint_as_float(o[4 * e + 2]) * up * up2, __uint_as_float(o[4 * e + 3]) * up * up2);
-                } else if (live) {
+                        for (uint32_t j = 0; j < NB * 8; ++j) sts_v4(v_s + (j / 8) * Sh::kBlock + ((j + row) % 8) * 16, 0, 0, 0, 0);
+                    }
+                    fence_async_proxy();
+                }
+                const float ref = m == -INFINITY ? 0.f : -m;
+                const uint64_t ref2 = pair(ref, ref);
+                auto weights = [&](auto whole) {                    // whole: no score of the tile is hidden
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t y[4];
+                    for (int c = 0; c < 4; ++c) {
+                        if (c && c % Sh::kHeld == 0) load(c);
+                        const uint32_t(&v)[32] = x[c % Sh::kHeld];
+                        uint32_t pk[16];
 #pragma unroll
-                        for (int h = 0; h < 4; ++h)
-                            y[h] = pack_bf16(__uint_as_float(o[8 * e + 2 * h]) * inv * up * up2, __uint_as_float(o[8 * e + 2 * h + 1]) * inv * up * up2);
-                        *reinterpret_cast<uint4 *>(dst + j * 32 + e * 8) = make_uint4(y[0], y[1], y[2], y[3]);
+                        for (int j = 0; j < 16; ++j) {
+                            const uint64_t y = fma2(pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), scale2, ref2);
+                            float e0, e1;
+                            if (decltype(whole)::value && BITS == 16 && j % 4 == 3) {
+                                ex2_poly(y, e0, e1);
+                            } else {
+                                split(y, e0, e1);
+                                e0 = ex2f(e0);
+                                e1 = ex2f(e1);
+                            }
+                            l2[j % kSums] = add2(l2[j % kSums], pair(e0, e1));
+                            pk[j] = BITS == 16 ? pack_bf16(e0, e1) : pack_f16(e0, e1);
+                        }
+                        tmem_st16(s_addr + c * 16, pk);
+                        if (c % 2) {                                    // half of the weights are there
+                            tmem_st_wait();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(bar(Sh::bP + 2 * t + c / 2));
+                        }
+                    }
+                };
+                if (edge) weights(std::false_type());
+                else weights(std::true_type());
+                done = true;
+                ++turn;
+            }
+            float l = 0.f;
+#pragma unroll
+            for (int e = 0; e < kSums; ++e) {
+                float l0, l1;
+                split(l2[e], l0, l1);
+                l += l0 + l1;
+            }
+            // ---- the row's result ----------------------------------------------------------------------------------
+            if (ok && !mbar_wait(bar(Sh::bO + t), k & 1)) { give_up(12); ok = false; }
+            ok = __all_sync(kFull, ok && !*s_abort);
+            if (__all_sync(kFull, ok)) {
+                tc_fence_after();
+                const bool live = tok < a.tt && pos <= q.p1;
+                const float inv = m == -INFINITY ? 0.f : 1.f / l;     // (nothing seen: zeros)
+                const float up = BITS == 4 ? power_of_2(v_exp / 2) : 1.f, up2 = BITS == 4 ? power_of_2(v_exp - v_exp / 2) : 1.f;
+                volatile const int32_t *item = s_items + k % 2 * kItemWords;
+                const uint32_t pieces = (uint32_t)item[kPieces], kvh = head_of(k);
+                const int32_t q_row = first_row_of(k);
+                const size_t part = ((size_t)(uint32_t)item[kSlot] * p.n_kv + kvh) * (NT * 128) + t * 128 + row;
+                if (pieces > 1 && live) *reinterpret_cast<float2 *>(a.ml + part * 2) = make_float2(m, l);
+                uint16_t *dst = a.out + (int64_t)(q_row + (int32_t)(t * a.tt + tok)) * a.ldo + (size_t)(kvh * a.group + head) * D;
+#pragma unroll 1
+                for (uint32_t j = 0; j < D / 32; ++j) {
+                    uint32_t o[32];
+                    if (done) {
+                        tmem_ld32(o_addr + j * 32, o);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0;
+                    }
+                    if (live && pieces > 1) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            *reinterpret_cast<float4 *>(a.partial + part * D + j * 32 + e * 4) =
+                                make_float4(__uint_as_float(o[4 * e]) * up * up2, __uint_as_float(o[4 * e + 1]) * up * up2,
+                                            __uint_as_float(o[4 * e + 2]) * up * up2, __uint_as_float(o[4 * e + 3]) * up * up2);
+                    } else if (live) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            uint32_t y[4];
+#pragma unroll
+                            for (int h = 0; h < 4; ++h)
+                                y[h] = pack_bf16(__uint_as_float(o[8 * e + 2 * h]) * inv * up * up2, __uint_as_float(o[8 * e + 2 * h + 1]) * inv * up * up2);
+                            *reinterpret_cast<uint4 *>(dst + j * 32 + e * 8) = make_uint4(y[0], y[1], y[2], y[3]);
+                        }
                     }
                 }
             }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(Sh::bRead + t));         // O may be written again
+            leave_item(k);
+            end_item();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(Sh::bRead + t));         // O may be written again
-        leave_item(k);
-        end_item();
-        }
-    } else {
-        if (Sh::kMove) {                                        // by warpgroups: 4 bits have one of producers, one for the products
-            if (BITS == 4 && warp >= Sh::kMma) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kMmaRegs));
-            else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kProdRegs));
-        }
-    if (warp >= Sh::kMma && warp < Sh::kMma + NT) {
+    } else if (warp >= Sh::kMma && warp < Sh::kMma + NT) {
         // =========================== products ======================================================================
         constexpr uint32_t kTypes = BITS == 16 ? (1u << 7) | (1u << 10) : 0u;       // both bf16, or both fp16
         constexpr uint32_t kIdescS = (1u << 4) | kTypes | ((kKt >> 3) << 17) | ((128u >> 4) << 24);
@@ -558,64 +566,64 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             __syncwarp();
         };
         for (uint32_t k = 0; ok && get_item(k); ++k) {
-        leave_item(k);
-        q = qt[0];
-        if (NT == 2 && t == 1) q = qt[NT - 1];
-        bool first = true;                                      // no product with V yet: O is written, not added to
-        if (kt.n > 0) {
-            ok = __all_sync(kFull, mbar_wait(bar(BITS == 16 ? Sh::bQ : Sh::bQh), q_count & 1) && full(ring0));
-            if (!ok) break;
-            if (kt.seen_by(q, 0)) scores(0);
-            release(ring0);
-            if (kt.n == 1) q_read();
-        }
-        for (int32_t i = 0; i < kt.n && ok; ++i) {
-            if (NT == 2 && (t == 1 || round > 0)) {
-                ok = __all_sync(kFull, mbar_wait(bar(Sh::bTurn + t), (t == 1 ? round : round - 1) & 1));
+            leave_item(k);
+            q = qt[0];
+            if (NT == 2 && t == 1) q = qt[NT - 1];
+            bool first = true;                                      // no product with V yet: O is written, not added to
+            if (kt.n > 0) {
+                ok = __all_sync(kFull, mbar_wait(bar(BITS == 16 ? Sh::bQ : Sh::bQh), q_count & 1) && full(ring0));
                 if (!ok) break;
+                if (kt.seen_by(q, 0)) scores(0);
+                release(ring0);
+                if (kt.n == 1) q_read();
             }
-            ++round;
-            if (kt.seen_by(q, i)) {
-                const uint64_t vd = v_desc + ((ring0 + 2 * i + 1) % NS) * (Sh::kTile >> 4);
-                ok = __all_sync(kFull, full(ring0 + 2 * i + 1));
-#pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {              // the weights come in two halves
-                    ok = ok && __all_sync(kFull, mbar_wait(bar(Sh::bP + 2 * t + h), made & 1));
+            for (int32_t i = 0; i < kt.n && ok; ++i) {
+                if (NT == 2 && (t == 1 || round > 0)) {
+                    ok = __all_sync(kFull, mbar_wait(bar(Sh::bTurn + t), (t == 1 ? round : round - 1) & 1));
                     if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) {
+                }
+                ++round;
+                if (kt.seen_by(q, i)) {
+                    const uint64_t vd = v_desc + ((ring0 + 2 * i + 1) % NS) * (Sh::kTile >> 4);
+                    ok = __all_sync(kFull, full(ring0 + 2 * i + 1));
 #pragma unroll
-                        for (uint32_t kk = h * (kKt / 32); kk < (h + 1) * (kKt / 32); ++kk)
-                            umma_ts(o_col, s_col + kk * 8, vd + kk * (2048 >> 4), kIdescO, !first || kk != 0);
+                    for (uint32_t h = 0; h < 2; ++h) {              // the weights come in two halves
+                        ok = ok && __all_sync(kFull, mbar_wait(bar(Sh::bP + 2 * t + h), made & 1));
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+#pragma unroll
+                            for (uint32_t kk = h * (kKt / 32); kk < (h + 1) * (kKt / 32); ++kk)
+                                umma_ts(o_col, s_col + kk * 8, vd + kk * (2048 >> 4), kIdescO, !first || kk != 0);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
-                }
-                if (!ok) break;
-                ++made;
-                first = false;
-            }
-            release(ring0 + 2 * i + 1);
-            if (i + 1 < kt.n) {
-                if (kt.seen_by(q, i + 1)) {
-                    ok = __all_sync(kFull, full(ring0 + 2 * i + 2));
                     if (!ok) break;
-                    scores(i + 1);
+                    ++made;
+                    first = false;
                 }
-                release(ring0 + 2 * i + 2);
-                if (i + 2 == kt.n) q_read();
+                release(ring0 + 2 * i + 1);
+                if (i + 1 < kt.n) {
+                    if (kt.seen_by(q, i + 1)) {
+                        ok = __all_sync(kFull, full(ring0 + 2 * i + 2));
+                        if (!ok) break;
+                        scores(i + 1);
+                    }
+                    release(ring0 + 2 * i + 2);
+                    if (i + 2 == kt.n) q_read();
+                }
+                if (NT == 2 && lane == 0) mbar_arrive(bar(Sh::bTurn + (t ^ 1)));
+                __syncwarp();
             }
-            if (NT == 2 && lane == 0) mbar_arrive(bar(Sh::bTurn + (t ^ 1)));
+            if (!ok) break;
+            // (not before the rows' threads have waited for the piece before: a phase that nobody has seen would be lost)
+            if (k > 0 && !__all_sync(kFull, mbar_wait(bar(Sh::bRead + t), (k - 1) & 1))) {
+                ok = false;
+                break;
+            }
+            if (elect_one()) umma_commit(bar(Sh::bO + t));
             __syncwarp();
-        }
-        if (!ok) break;
-        // (not before the rows' threads have waited for the piece before: a phase that nobody has seen would be lost)
-        if (k > 0 && !__all_sync(kFull, mbar_wait(bar(Sh::bRead + t), (k - 1) & 1))) {
-            ok = false;
-            break;
-        }
-        if (elect_one()) umma_commit(bar(Sh::bO + t));
-        __syncwarp();
-        end_item();
+            end_item();
         }
         if (!ok) give_up(13);
         if (elect_one()) umma_commit(bar(Sh::bEnd));
@@ -712,28 +720,28 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             return id < 0 ? -(int32_t)kKt : (int32_t)row_index(p, id, kvh, at);
         };
         for (uint32_t k = 0; ok && get_item(k); ++k) {
-        kvh = head_of(k);
-        q_row = first_row_of(k);
-        leave_item(k);
-        int32_t next = kt.n > 0 ? row_of(0) : 0;
-        for (int32_t i = 0; i < kt.n && ok; ++i) {
-            const int32_t r = next;
-            if (i + 1 < kt.n) next = row_of(i + 1);
-            for (uint32_t kv = 0; kv < 2; ++kv, ++issued) {
-                const uint32_t slot = issued % NS;
-                if (!mbar_wait_warp(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1) || *s_abort) { give_up(15); ok = false; break; }
-                const uint32_t to = bar(Sh::bFull + slot), dst = smem_s + Sh::oRing + slot * Sh::kTile;
-                if (lane == 0) mbar_expect_tx(to, Sh::kTile);
-                __syncwarp();
-                if (lane < ids)
+            kvh = head_of(k);
+            q_row = first_row_of(k);
+            leave_item(k);
+            int32_t next = kt.n > 0 ? row_of(0) : 0;
+            for (int32_t i = 0; i < kt.n && ok; ++i) {
+                const int32_t r = next;
+                if (i + 1 < kt.n) next = row_of(i + 1);
+                for (uint32_t kv = 0; kv < 2; ++kv, ++issued) {
+                    const uint32_t slot = issued % NS;
+                    if (!mbar_wait_warp(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1) || *s_abort) { give_up(15); ok = false; break; }
+                    const uint32_t to = bar(Sh::bFull + slot), dst = smem_s + Sh::oRing + slot * Sh::kTile;
+                    if (lane == 0) mbar_expect_tx(to, Sh::kTile);
+                    __syncwarp();
+                    if (lane < ids)
 #pragma unroll
-                    for (uint32_t c = 0; c < NB; ++c)
-                        tma_load_2d(dst + c * Sh::kBlock + (lane << p.page_shift) * 128, kv ? &v_map : &k_map, (int32_t)(c * 64), r, to);
-                __syncwarp();
-                if (i == 0 && kv == 0 && !load_q()) { give_up(22); ok = false; ++issued; break; }
+                        for (uint32_t c = 0; c < NB; ++c)
+                            tma_load_2d(dst + c * Sh::kBlock + (lane << p.page_shift) * 128, kv ? &v_map : &k_map, (int32_t)(c * 64), r, to);
+                    __syncwarp();
+                    if (i == 0 && kv == 0 && !load_q()) { give_up(22); ok = false; ++issued; break; }
+                }
             }
-        }
-        end_item();
+            end_item();
         }
         if (!ok)                                                // copies under way end before the block does
             for (uint32_t c = issued > NS ? issued - NS : 0; c < issued; ++c) (void)mbar_wait_warp(bar(Sh::bFull + c % NS), (c / NS) & 1);
@@ -820,44 +828,43 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             if (lane == 0) mbar_arrive(bar(Sh::bFull + slot));
         };
         for (uint32_t k = 0; ok && get_item(k); ++k) {
-        kvh = head_of(k);
-        q_row = first_row_of(k);
-        leave_item(k);
-        v_exp = -1000;                                          // (no tile of V yet)
-        Codes f0, f1;
-        int32_t id = page_at(0), id_next = page_at(1);
-        if (kt.n > 0) {
-            fetch(f0, id, 0, 0);
-            if (warp == Sh::kProd) {
-                if (q_count) ok = mbar_wait_warp(bar(Sh::bQfree), (q_count - 1) & 1);
-                if (!ok) give_up(22);
-                if (ok && lane == 0) {
-                    const uint32_t bytes = a.tt * a.group * 128;
-                    mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
-                    for (uint32_t t = 0; t < NT; ++t)
-                        for (uint32_t c = 0; c < NB; ++c)
-                            tma_load_3d(smem_s + Sh::oQ + t * Sh::kTile + c * Sh::kBlock, &q_map, (int32_t)(c * 64), (int32_t)(kvh * a.group),
-                                        q_row + (int32_t)(t * a.tt), bar(Sh::bQ));
+            kvh = head_of(k);
+            q_row = first_row_of(k);
+            leave_item(k);
+            v_exp = -1000;                                          // (no tile of V yet)
+            Codes f0, f1;
+            int32_t id = page_at(0), id_next = page_at(1);
+            if (kt.n > 0) {
+                fetch(f0, id, 0, 0);
+                if (warp == Sh::kProd) {
+                    if (q_count) ok = mbar_wait_warp(bar(Sh::bQfree), (q_count - 1) & 1);
+                    if (!ok) give_up(22);
+                    if (ok && lane == 0) {
+                        const uint32_t bytes = a.tt * a.group * 128;
+                        mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
+                        for (uint32_t t = 0; t < NT; ++t)
+                            for (uint32_t c = 0; c < NB; ++c)
+                                tma_load_3d(smem_s + Sh::oQ + t * Sh::kTile + c * Sh::kBlock, &q_map, (int32_t)(c * 64), (int32_t)(kvh * a.group),
+                                            q_row + (int32_t)(t * a.tt), bar(Sh::bQ));
+                    }
+                    queries += ok;
+                    __syncwarp();
                 }
-                queries += ok;
-                __syncwarp();
             }
-        }
-        for (int32_t i = 0; i < kt.n; ++i) {
-            fetch(f1, id, i, 1);
-            turn(f0, id, i, 0);
-            ++issued;
-            const int32_t id_here = id;
-            id = id_next;
-            if (i + 1 < kt.n) fetch(f0, id, i + 1, 0);
-            id_next = page_at(i + 2);
-            turn(f1, id_here, i, 1);
-            ++issued;
-        }
-        end_item();
+            for (int32_t i = 0; i < kt.n; ++i) {
+                fetch(f1, id, i, 1);
+                turn(f0, id, i, 0);
+                ++issued;
+                const int32_t id_here = id;
+                id = id_next;
+                if (i + 1 < kt.n) fetch(f0, id, i + 1, 0);
+                id_next = page_at(i + 2);
+                turn(f1, id_here, i, 1);
+                ++issued;
+            }
+            end_item();
         }
         if (!ok && queries) (void)mbar_wait_warp(bar(Sh::bQ), (queries - 1) & 1);
-    }
     }
     tc_fence_before();
     __syncthreads();

@@ -279,6 +279,28 @@ def test_new_tokens_of_long_sequences(d, group, n_kv, page, new, kv, window, sin
 
 
 @pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("said", [1, 20, 10 ** 6])
+def test_a_max_q_len_that_is_not_true(said, bits):
+    g = gen(said)
+    kv, new = [200, 90, 7], [150, 65, 0]
+    cache, table = make_cache(g, 20, 16, 1, 64, bits), make_table(g, kv, 16, 20)
+    q = rnd(g, 215, 2, 64).to(torch.bfloat16).to(DEV)
+    check_attention(q, cache, table, kv, new, max_q_len=said)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("new", [[130, 40], [2, 9]])
+def test_first_tokens_that_fill_tiles(new, bits):
+    """More first tokens than window, the window a few tokens, sequences that end in the first tokens."""
+    g = gen(41)
+    kv = [1500, 60]
+    cache, table = make_cache(g, 60, 32, 2, 128, bits), make_table(g, kv, 32, 60)
+    q = rnd(g, sum(new), 4, 128).to(torch.bfloat16).to(DEV)
+    for window, sinks in ((3, 700), (1, 128), (200, 129), (1400, 1000)):
+        check_attention(q, cache, table, kv, new, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
 def test_more_sequences_than_threads_and_uneven_lengths(bits):
     g = gen(9)
     kv = [(37 * i) % 90 for i in range(300)] + [2000]
