@@ -699,7 +699,9 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Page
 }
 
 constexpr uint32_t kPaMaxRows = 16;              // widest group of query rows of any variant
-constexpr uint32_t kPaRows = 64;                 // query rows of a sequence and key head up to which this kernel has them
+// Query rows of a sequence and key head up to which this kernel has them.  48 drawn batches with sequences around it: up to 32 rows
+// 5 % slower in the mean, 16 10 %, 8 17 % (batches of 60 to 230 rows gain up to 40 %, those that need no other kernel lose up to half).
+constexpr uint32_t kPaRows = 64;
 constexpr uint32_t kPaMaxResident = 4;           // blocks of a multiprocessor that the workspace has room for
 
 // As many blocks as fit on the device at once: a block more would start when the others have ended.
@@ -712,7 +714,9 @@ static int resident_blocks(const void *kernel, uint32_t &blocks) {
 
 template <int D, int BITS, int NR>
 static int launch_attention(const PagedAttnArgs &a, const PromptPlan &plan, cudaStream_t s) {
-    constexpr int U = BITS == 4 ? 2 : 1;
+    // 4 bits: two tiles of 16 tokens at once; heads of 256 have no registers for that (contexts of hundreds of tokens 31 -> 24 us
+    // with one, of 38000 99 -> 105).  bf16 heads of 64: 25 us with two where one takes 21.
+    constexpr int U = BITS == 4 && D < 256 ? 2 : 1;
     static uint32_t resident = 0;
     if (resident == 0)
         if (int rc = resident_blocks((const void *)k_paged_attention<D, BITS, NR, U>, resident)) return rc;

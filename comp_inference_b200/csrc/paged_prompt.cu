@@ -184,6 +184,13 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// Whether p holds in all of THREADS threads, which meet here (barrier 1).
+template <uint32_t THREADS>
+__device__ __forceinline__ bool all_of(bool p) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred P, Q;\n\tsetp.ne.u32 P, %1, 0;\n\tbar.red.and.pred Q, 1, %2, P;\n\tselp.u32 %0, 1, 0, Q;\n\t}" : "=r"(r) : "r"((uint32_t)p), "n"(THREADS) : "memory");
+    return r != 0;
+}
 // The smallest e with x < 2^e, for x >= 0 that is finite; others do not ask for a scale.
 __device__ __forceinline__ int32_t exponent_of(float x) {
     const uint32_t e = __float_as_uint(x) >> 23 & 0xFFu;
@@ -827,10 +834,14 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(Sh::bFull + slot));
         };
-        for (uint32_t k = 0; ok && get_item(k); ++k) {
-            kvh = head_of(k);
-            q_row = first_row_of(k);
-            leave_item(k);
+        for (uint32_t k = 0;; ++k) {
+            const bool have = get_item(k);
+            if (have) {
+                kvh = head_of(k);
+                q_row = first_row_of(k);
+                leave_item(k);
+            }
+            if (!all_of<PW * 32>(have && ok)) break;            // all of these warps go on or none: they meet at a barrier in every tile
             v_exp = -1000;                                          // (no tile of V yet)
             Codes f0, f1;
             int32_t id = page_at(0), id_next = page_at(1);
