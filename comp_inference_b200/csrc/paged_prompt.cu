@@ -68,8 +68,8 @@ struct PromptShape {
     static constexpr bool kMove = NT == 2 || BITS == 4;
     static constexpr uint32_t kWarps = kMove ? (kSched + 4) / 4 * 4 : kSched + 1, kThreads = kWarps * 32;
     static constexpr uint32_t kLaunchRegs = 65536 / kThreads / 8 * 8;
-    static constexpr uint32_t kSoftRegs = BITS == 16 ? 200 : D == 64 ? 160 : D == 128 ? 144 : 176;
-    static constexpr uint32_t kProdRegs = BITS == 16 ? 104 : D == 64 ? 120 : D == 128 ? 64 : 104;
+    static constexpr uint32_t kSoftRegs = BITS == 16 ? 200 : D == 64 ? 160 : D == 128 ? 136 : 176;
+    static constexpr uint32_t kProdRegs = BITS == 16 ? 104 : D == 64 ? 120 : D == 128 ? 72 : 104;
     static constexpr uint32_t kMmaRegs = BITS == 16 ? kProdRegs : D == 64 ? 72 : D == 128 ? 64 : 112;
     static_assert(!kMove || (kSoftRegs >= kLaunchRegs && kProdRegs <= kLaunchRegs && kMmaRegs <= kLaunchRegs &&
                              NT * 128 * kSoftRegs + (BITS == 16 ? 128 * kProdRegs : PW * 32 * kProdRegs + 128 * kMmaRegs) <= kThreads * kLaunchRegs), "registers");
@@ -264,7 +264,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             return false;
         }
         volatile const int32_t *x = s_items + k % 2 * kItemWords;
-        if (x[kSequence] < 0 || *s_abort) return false;
+        if (__any_sync(kFull, x[kSequence] < 0 || *s_abort)) return false;
         b = (uint32_t)uniform(x[kSequence]);
         kt = {uniform(x[kTilesAt]), uniform(x[kTilesAt + 1]), uniform(x[kTilesAt + 2]), uniform(x[kTilesAt + 3]), uniform(x[kTilesAt + 4])};
 #pragma unroll
@@ -736,7 +736,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 if (i + 1 < kt.n) next = row_of(i + 1);
                 for (uint32_t kv = 0; kv < 2; ++kv, ++issued) {
                     const uint32_t slot = issued % NS;
-                    if (!mbar_wait_warp(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1) || *s_abort) { give_up(15); ok = false; break; }
+                    if (!mbar_wait_warp(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1) || __any_sync(kFull, *s_abort)) { give_up(15); ok = false; break; }
                     const uint32_t to = bar(Sh::bFull + slot), dst = smem_s + Sh::oRing + slot * Sh::kTile;
                     if (lane == 0) mbar_expect_tx(to, Sh::kTile);
                     __syncwarp();
@@ -835,13 +835,10 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             if (lane == 0) mbar_arrive(bar(Sh::bFull + slot));
         };
         for (uint32_t k = 0;; ++k) {
-            const bool have = get_item(k);
-            if (have) {
-                kvh = head_of(k);
-                q_row = first_row_of(k);
-                leave_item(k);
-            }
-            if (!all_of<PW * 32>(have && ok)) break;            // all of these warps go on or none: they meet at a barrier in every tile
+            if (!all_of<PW * 32>(get_item(k))) break;           // all of these warps go on or none: they meet at a barrier in every tile
+            kvh = head_of(k);
+            q_row = first_row_of(k);
+            leave_item(k);
             v_exp = -1000;                                          // (no tile of V yet)
             Codes f0, f1;
             int32_t id = page_at(0), id_next = page_at(1);
