@@ -10,7 +10,8 @@ new tokens of a whole ragged batch, one behind the other:
                                     None: one new token per sequence (a decode step)
 
 All three live on the GPU and are read when the kernels run: nothing waits for them, and a captured call goes by what they
-hold when its graph is replayed.  Rows behind the last sequence are left as they were.  No counterpart in the reference,
+hold when its graph is replayed.  Rows behind the last sequence are left as they were (undefined in an output that the call
+makes itself: a padded batch whose later stages read them passes ``out``).  No counterpart in the reference,
 which leaves cache, attention and sampling to Hugging Face's ``generate`` (tests/test_rans_pytorch_runtime.py:89-118).
 
 Calls are queued on the current stream of the cache's device, whichever device is current.  A kernel whose internal wait ran
