@@ -297,7 +297,9 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         for (uint32_t k = 0; ok && get_item(k); ++k) {
             QueryTile q = qt[0];
             if (NT == 2 && t == 1) q = qt[NT - 1];
-            const int32_t pos = q.p0 + (int32_t)tok, last = min(pos, p.cap - 1);
+            // (the tile's rows behind the sequence's go along with its last one; no sum of a length and more passes 2^31 so)
+            const int32_t behind = q.p1 - q.p0, pos = q.p0 + max(min((int32_t)tok, behind), 0), last = min(pos, p.cap - 1);
+            const bool live = tok < a.tt && (int32_t)tok <= behind;
             const uint32_t s_addr = tmem + ((w * 32u) << 16) + t * kKt, o_addr = tmem + ((w * 32u) << 16) + Sh::cO + t * D;
             float m = -INFINITY;
             constexpr int kSums = BITS == 16 ? 4 : 2;
@@ -494,7 +496,6 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             ok = __all_sync(kFull, ok && !*s_abort);
             if (__all_sync(kFull, ok)) {
                 tc_fence_after();
-                const bool live = tok < a.tt && pos <= q.p1;
                 const float inv = m == -INFINITY ? 0.f : 1.f / l;     // (nothing seen: zeros)
                 const float up = BITS == 4 ? power_of_2(v_exp / 2) : 1.f, up2 = BITS == 4 ? power_of_2(v_exp - v_exp / 2) : 1.f;
                 volatile const int32_t *item = s_items + k % 2 * kItemWords;
@@ -656,7 +657,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
 #pragma unroll
             for (uint32_t t = 0; t < NT; ++t) {
                 const int32_t i0 = (int32_t)(((uint32_t)w0.y * NT + t) * a.tt), n = min(max(q_len - i0, 0), (int32_t)a.tt);
-                qt[t].p0 = kv_len - q_len + i0;
+                qt[t].p0 = kv_len - q_len + min(i0, q_len);
                 qt[t].p1 = qt[t].p0 + n - 1;
                 hi[t] = n ? max(min(qt[t].p1 + 1, p.cap), 0) : 0;
                 lo[t] = a.window ? min(max(qt[t].p0 - a.window + 1, 0), hi[t]) : 0;
