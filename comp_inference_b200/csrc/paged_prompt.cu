@@ -142,11 +142,18 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
+// The largest of three values, NaN where one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
 // 2^x of two values, x <= 2^6, in the fused multiply-add units: the integer next to x goes into the exponent field, 2^f for the rest
 // in [-1/2, 1/2] is a polynomial of degree 3 fitted for the smallest largest relative error, 7.5e-5, a fiftieth of what rounding to
 // bf16 loses.  The special-function unit makes four results per cycle and scheduler; a quarter of the weights comes from here
 // (4096 tokens, 32 heads of 128 over 8: 160.6 us when it was tried, none of them 167.6, half 181.8).  For x of
-// -126 and less it gives 2^-126, not 0: not for tiles with hidden scores.
+// -126 and less it gives 2^-126, not 0, and for a NaN too: not for tiles with hidden scores, nor where a row's largest is not finite.
 constexpr float kExp0 = 0.99992812f, kExp1 = 0.69326097f, kExp2 = 0.24261075f, kExp3 = 0.05517141f;
 __device__ __forceinline__ void ex2_poly(uint64_t x, float &r0, float &r1) {
     float x0, x1;
@@ -394,7 +401,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     for (int j = 0; j < 32; j += 8)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            mx4[e] = fmaxf(fmaxf(mx4[e], __uint_as_float(v[j + e])), __uint_as_float(v[j + 4 + e]));
+                            mx4[e] = max3_nan(mx4[e], __uint_as_float(v[j + e]), __uint_as_float(v[j + 4 + e]));
                 };
                 auto load = [&](int first) {                        // kHeld groups of 32 scores
 #pragma unroll
@@ -411,9 +418,13 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
 #pragma unroll
                     for (int c = 0; c < Sh::kHeld; ++c) largest(x[c]);
                 }
-                float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;
-                const bool grow = mx > m + kLazy;
-                if (__any_sync(kFull, grow || v_down != 1.f)) {
+                const float mx = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * scale;
+                const bool grow = mx > m + kLazy;               // (not for a NaN: its weight is one whatever it refers to)
+                // A score that is not finite (rows behind the sequence hold anything): its weight is 0 or NaN, which ex2_poly has not.
+                const bool odd = BITS == 16 && !edge && live && !(fabsf(mx) < INFINITY);
+                bool exact = edge;
+                if (__any_sync(kFull, grow || odd || v_down != 1.f)) {
+                    exact |= BITS == 16 && __any_sync(kFull, odd);
                     float c = grow ? ex2f(m - mx) : 1.f;
                     if (grow) m = mx;
 #pragma unroll
@@ -450,7 +461,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 }
                 const float ref = m == -INFINITY ? 0.f : -m;
                 const uint64_t ref2 = pair(ref, ref);
-                auto weights = [&](auto whole) {                    // whole: no score of the tile is hidden
+                auto weights = [&](auto whole) {                    // whole: no score of the tile is hidden, none infinite or NaN
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         if (c && c % Sh::kHeld == 0) load(c);
@@ -479,7 +490,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                         }
                     }
                 };
-                if (edge) weights(std::false_type());
+                if (exact) weights(std::false_type());
                 else weights(std::true_type());
                 done = true;
                 ++turn;

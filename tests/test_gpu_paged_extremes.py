@@ -1,10 +1,38 @@
-"""GPU: the operators over a paged cache with extreme lengths."""
+"""GPU: the operators over a paged cache at extremes: lengths next to the largest, scores that are not finite.
+
+What a query sees decides: a NaN or +infinity among its scores makes its row NaN, a score of -infinity has the weight 0, and a row with
+nothing but those is NaN (0 / 0)."""
 import pytest
 import torch
 
-from test_gpu_paged import DEV, ci, gen, i32, make_cache, rnd, rope_tables, starts_of
+import paged_reference as ref
+from test_gpu_paged import DEV, ci, gen, i32, make_cache, make_table, rnd, rope_tables, starts_of
 
 pytestmark = pytest.mark.gpu
+
+NAN, INF = float("nan"), float("inf")
+
+
+def spoil(cache, table, b, j, value):
+    """A value of key j of sequence b (4 bits: its first group, which holds no infinity: a NaN)."""
+    i = ref.page(cache, table, b, j)
+    if cache.bits == 16:
+        cache.k[i, :, j % cache.page_size, 0] = value
+    else:
+        cache.k_scale[i, :, j % cache.page_size, 0] = value
+
+
+def compare(q, cache, table, kv, new=None, **args):
+    """NaN where the definition gives it and nowhere else, the rest within the bound of its roundings."""
+    starts = starts_of(new) if new else None
+    got = ci().paged_attention(q, cache, table.to(DEV), i32(kv), starts, **args)
+    args.pop("max_q_len", None)
+    want, bound = ref.attention(q, cache, table, kv, starts, **args)
+    got = got.double().view_as(want)
+    nan = want.isnan()
+    assert torch.equal(got.isnan(), nan), (got.isnan() != nan).nonzero()[:8].tolist()
+    assert bool(((got - want).abs() <= bound)[~nan].all())
+    return nan
 
 
 @pytest.mark.parametrize("bits", [16, 4])
@@ -39,3 +67,49 @@ def test_lengths_next_to_the_largest(group, bits):
     assert bool((gk == 0).all()) and bool((gv == 0).all())
     one = ci().paged_attention(q[:2], cache, table, i32([2 ** 31 - 1, 96]))
     assert torch.equal(one, ci().paged_attention(q[:2], cache, table, i32([96, 96])))
+
+
+PROMPTS = [  # d, group, n_kv, page, new, tokens: in one piece, in several
+    (128, 2, 1, 32, [300], [600]),
+    (64, 3, 2, 64, [200], [500]),
+    (256, 2, 1, 16, [140], [400]),
+    (128, 4, 1, 64, [40], [5000]),
+]
+
+
+@pytest.mark.parametrize("d,group,n_kv,page,new,kv", PROMPTS)
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+def test_prompts_with_a_key_that_is_not_finite(d, group, n_kv, page, new, kv, value):
+    """At each position modulo 8 of a tile that every row sees all of."""
+    g = gen(d)
+    pages = sum(-(-n // page) for n in kv) + 1
+    cache, table = make_cache(g, pages, page, n_kv, d, 16), make_table(g, kv, page, pages)
+    q = rnd(g, sum(new), group * n_kv, d).to(torch.bfloat16).to(DEV)
+    q[..., 0] = 1.0
+    for j in range(136, 144):
+        i = ref.page(cache, table, 0, j)
+        keep = cache.k[i, :, j % page, 0].clone()
+        spoil(cache, table, 0, j, value)
+        got = ci().paged_attention(q, cache, table.to(DEV), i32(kv), starts_of(new))
+        if value == -INF:
+            if j == 137 or j == 142:
+                assert not bool(compare(q, cache, table, kv, new).any())
+        else:
+            assert bool(got.isnan().all()), (j, int(got.isnan().sum()), got.numel())
+        cache.k[i, :, j % page, 0] = keep
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_rows_behind_a_sequence_do_not_change_the_others(bits):
+    """NaN in the queries of padding and of the next sequence, which lie in the same tile of query rows."""
+    g = gen(23)
+    new, kv, d, group = [100, 30], [130, 400], 128, 6
+    cache, table = make_cache(g, 60, 16, 1, d, bits), make_table(g, kv, 16, 60)
+    q = rnd(g, 180, group, d).to(torch.bfloat16).to(DEV)
+    args = (cache, table.to(DEV), i32(kv), starts_of(new))
+    want = ci().paged_attention(q, *args)[:100].clone()
+    q[100:] = NAN
+    junk = rnd(g, 200, group, d).to(torch.bfloat16).to(DEV)
+    for _ in range(3):
+        ci().paged_attention(junk.fill_(NAN), cache, table.to(DEV), i32([400, 400]), i32([0, 120, 200]))       # NaN left in shared memory
+        assert torch.equal(ci().paged_attention(q, *args)[:100], want)
