@@ -23,7 +23,9 @@
 namespace ci {
 
 constexpr uint32_t kPaWarps = 4, kPaThreads = kPaWarps * 32;
-constexpr float kNone = -INFINITY;
+// The maximum of a row that has seen nothing, and the least one of a row that has seen scores, though all of them be -infinity or NaN:
+// its sum is then 0 or NaN, and the row NaN, as the definition has it.
+constexpr float kNone = -INFINITY, kLeast = -3.402823466e38f;
 
 struct PagedAttnArgs {
     PagedBatch p;
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
         float m[NR][2], l[NR][2], o[NR][NB][4][4], corr[NR][BITS == 4 ? G : 1][2];
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
-            m[nr][0] = m[nr][1] = kNone;
+            m[nr][0] = m[nr][1] = kLeast;
             l[nr][0] = l[nr][1] = 0.f;
 #pragma unroll
             for (int gr = 0; gr < (BITS == 4 ? G : 1); ++gr) corr[nr][gr][0] = corr[nr][gr][1] = 0.f;
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
                 for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const float c = mx[nr][j] == kNone ? 1.f : ex2(m[nr][j] - mx[nr][j]);
+                        const float c = ex2(m[nr][j] - mx[nr][j]);
                         m[nr][j] = mx[nr][j];
                         l[nr][j] *= c;
 #pragma unroll
@@ -416,11 +418,6 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
                     }
             }
             // ---- weights and values ------------------------------------------------------------------------------
-            float ref[NR][2];
-#pragma unroll
-            for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) ref[nr][j] = !kAll && m[nr][j] == kNone ? 0.f : m[nr][j];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float pr[NR][4];
@@ -428,7 +425,7 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
                 for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        pr[nr][e] = ex2(sc[u][nr][e] - ref[nr][e & 1]);
+                        pr[nr][e] = ex2(sc[u][nr][e] - m[nr][e & 1]);
                         l[nr][e & 1] += pr[nr][e];
                     }
                 if constexpr (BITS == 16) {
@@ -546,23 +543,31 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
                             make_float2(o[nr][x][mm][j], o[nr][x][mm][2 + j]);
             }
         __syncthreads();
+        // Whether a row sees a position of these tiles: asked where it has no weight.
+        auto sees = [&](uint32_t row) {
+            const int32_t at = s.kv_len - s.q_len + (int32_t)(row / a.group);
+            for (int32_t i = i0; i < n_tiles; ++i)
+                for (int32_t j0 = sp.first(i), k = 0; k < TILE / 16; ++k, j0 += 16)
+                    if (j0 <= at && j0 < sp.hi && (!a.window || min(j0 + 15, at) > at - a.window || j0 < a.sinks) && page_of(p, b, j0) >= 0) return true;
+            return false;
+        };
         const bool whole = u0 == 0 && u1 == units;
         const uint32_t slot = blockIdx.x * 2 + (u0 == 0 ? 1 : 0);   // the part that begins an item, or one that goes on with it
         for (uint32_t x = threadIdx.x; x < RT * D / 4; x += kPaThreads) {
             const uint32_t r = x / (D / 4), c = x % (D / 4) * 4, row = rt * RT + r;
-            float M = kNone, L = 0.f;
+            float M = kLeast, L = 0.f;
 #pragma unroll
             for (uint32_t w4 = 0; w4 < kPaWarps; ++w4) M = fmaxf(M, s_m[w4][r]);
-            const float safe = M == kNone ? 0.f : M;
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (uint32_t w4 = 0; w4 < kPaWarps; ++w4) {
-                if (s_m[w4][r] == kNone) continue;
-                const float e = ex2(s_m[w4][r] - safe);
+                if (s_l[w4][r] == 0.f) continue;                // (values that the row does not see may have left a NaN)
+                const float e = ex2(s_m[w4][r] - M);
                 const float4 z = *reinterpret_cast<const float4 *>(&s_o[w4][r][c]);
                 L += e * s_l[w4][r];
                 y.x += e * z.x; y.y += e * z.y; y.z += e * z.z; y.w += e * z.w;
             }
+            if (L == 0.f && !(row < rows && sees(row))) M = kNone;
             if (whole) {
                 if (row < rows) {
                     const float inv = M == kNone ? 0.f : 1.f / L;

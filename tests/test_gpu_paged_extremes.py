@@ -69,6 +69,66 @@ def test_lengths_next_to_the_largest(group, bits):
     assert torch.equal(one, ci().paged_attention(q[:2], cache, table, i32([96, 96])))
 
 
+STEPS = [  # d, group, n_kv, page, tokens of each sequence: alone (parts of them in many blocks), and in a batch that leaves them whole
+    (128, 4, 2, 64, [1, 3, 700, 64]),
+    (64, 7, 1, 16, [2, 33, 400, 5]),
+    (256, 2, 1, 32, [1, 130, 257, 40]),
+    (128, 16, 1, 32, [1, 90, 333, 17]),
+    (64, 1, 2, 64, [(7 * i) % 60 + 1 for i in range(900)]),
+]
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("d,group,n_kv,page,kv", STEPS)
+def test_steps_with_a_nan(d, group, n_kv, page, kv, bits):
+    g = gen(d + group)
+    pages = sum(-(-n // page) for n in kv) + 1
+    cache, table = make_cache(g, pages, page, n_kv, d, bits), make_table(g, kv, page, pages)
+    q = rnd(g, len(kv), group * n_kv, d).to(torch.bfloat16).to(DEV)
+    q[0, 0, 3] = NAN                                    # all scores of one head
+    spoil(cache, table, 1, kv[1] - 1, NAN)              # one key among several
+    spoil(cache, table, len(kv) - 1, 0, NAN)
+    nan = compare(q, cache, table, kv)
+    assert bool(nan[0, 0].all()) and not bool(nan[0, 1:].any()) and bool(nan[1].all()) and not bool(nan[2].any())
+
+
+@pytest.mark.parametrize("kv", [[1, 1, 40], [1, 700, 40], [1 + i % 50 for i in range(900)]])
+def test_steps_with_infinite_scores(kv):
+    g = gen(len(kv))
+    d, page = 128, 32
+    pages = sum(-(-n // page) for n in kv) + 1
+    q = rnd(g, len(kv), 4, d).to(torch.bfloat16).to(DEV)
+    q[..., 0] = 1.0
+    for b, value, where in ((1, -INF, "all"), (1, INF, "all"), (2, INF, "one"), (2, -INF, "one"), (2, -INF, "first 17"), (1, -INF, "but one"), (2, -INF, "last")):
+        cache, table = make_cache(gen(3), pages, page, 2, d, 16), make_table(gen(4), kv, page, pages)
+        n = kv[b]
+        for j in {"all": range(n), "one": [n // 2], "first 17": range(min(n - 1, 17)), "but one": [j for j in range(n) if j != n // 2],
+                  "last": [n - 1] if n > 1 else []}[where]:
+            spoil(cache, table, b, j, value)
+        nan = compare(q, cache, table, kv)
+        other = [i for i in range(len(kv)) if i != b]
+        assert not bool(nan[other].any())
+        if where == "all" or value == INF:
+            assert bool(nan[b].all())
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("new", [[3, 2], [12, 1]])
+def test_few_new_tokens_with_a_nan(new, bits):
+    """The tokens in front of a key do not see it."""
+    g = gen(7)
+    kv, d = [300, 20], 128
+    cache, table = make_cache(g, 30, 16, 1, d, bits), make_table(g, kv, 16, 30)
+    q = rnd(g, sum(new), 4, d).to(torch.bfloat16).to(DEV)
+    spoil(cache, table, 0, kv[0] - 2, NAN)
+    nan = compare(q, cache, table, kv, new)
+    assert not bool(nan[:new[0] - 2].any()) and bool(nan[new[0] - 2:new[0]].all()) and not bool(nan[new[0]:].any())
+    q[new[0] - 3] = NAN
+    nan = compare(q, cache, table, kv, new)
+    assert bool(nan[new[0] - 3].all())
+    compare(q, cache, table, kv, new, window=1)
+
+
 PROMPTS = [  # d, group, n_kv, page, new, tokens: in one piece, in several
     (128, 2, 1, 32, [300], [600]),
     (64, 3, 2, 64, [200], [500]),
