@@ -23,9 +23,6 @@
 namespace ci {
 
 constexpr uint32_t kPaWarps = 4, kPaThreads = kPaWarps * 32;
-// The maximum of a row that has seen nothing, and the least one of a row that has seen scores, though all of them be -infinity or NaN:
-// its sum is then 0 or NaN, and the row NaN, as the definition has it.
-constexpr float kNone = -INFINITY, kLeast = -3.402823466e38f;
 
 struct PagedAttnArgs {
     PagedBatch p;

@@ -308,7 +308,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             const int32_t behind = q.p1 - q.p0, pos = q.p0 + max(min((int32_t)tok, behind), 0), last = min(pos, p.cap - 1);
             const bool live = tok < a.tt && (int32_t)tok <= behind;
             const uint32_t s_addr = tmem + ((w * 32u) << 16) + t * kKt, o_addr = tmem + ((w * 32u) << 16) + Sh::cO + t * D;
-            float m = -INFINITY;
+            float m = kNone;
             constexpr int kSums = BITS == 16 ? 4 : 2;
             uint64_t l2[kSums] = {};                                // sums of weights, two in each
             bool done = false;                                      // a product of this piece has been
@@ -383,6 +383,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 }
                 const uint64_t scale2 = pair(scale, scale);
                 uint32_t x[Sh::kHeld][32];
+                uint32_t any = edge ? 0u : 1u;                      // not 0: the row sees some of the tile
                 auto hide = [&](uint32_t (&v)[32], int32_t c) {     // scores of positions that the row does not see
                     const int32_t f32 = f + c * 32;
                     uint32_t seen = low_bits(last + 1 - f32);
@@ -391,6 +392,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
 #pragma unroll
                         for (int j = 0; j < 32; j += 16)
                             if (gone >> ((uint32_t)(c * 32 + j) >> p.page_shift) & 1) seen &= ~(0xFFFFu << j);
+                    any |= seen;
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
                         if (!(seen & (1u << j))) v[j] = 0xFF800000u;
@@ -419,6 +421,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     for (int c = 0; c < Sh::kHeld; ++c) largest(x[c]);
                 }
                 const float mx = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * scale;
+                if (any) m = fmaxf(m, kLeast);
                 const bool grow = mx > m + kLazy;               // (not for a NaN: its weight is one whatever it refers to)
                 // A score that is not finite (rows behind the sequence hold anything): its weight is 0 or NaN, which ex2_poly has not.
                 const bool odd = BITS == 16 && !edge && live && !(fabsf(mx) < INFINITY);
@@ -459,7 +462,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     }
                     fence_async_proxy();
                 }
-                const float ref = m == -INFINITY ? 0.f : -m;
+                const float ref = m == kNone ? 0.f : -m;
                 const uint64_t ref2 = pair(ref, ref);
                 auto weights = [&](auto whole) {                    // whole: no score of the tile is hidden, none infinite or NaN
 #pragma unroll
@@ -507,7 +510,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             ok = __all_sync(kFull, ok && !*s_abort);
             if (__all_sync(kFull, ok)) {
                 tc_fence_after();
-                const float inv = m == -INFINITY ? 0.f : 1.f / l;     // (nothing seen: zeros)
+                const bool none = m == kNone;                         // nothing seen: zeros, whatever values have left in O
+                const float inv = none ? 0.f : 1.f / l;
                 const float up = BITS == 4 ? power_of_2(v_exp / 2) : 1.f, up2 = BITS == 4 ? power_of_2(v_exp - v_exp / 2) : 1.f;
                 volatile const int32_t *item = s_items + k % 2 * kItemWords;
                 const uint32_t pieces = (uint32_t)item[kPieces], kvh = head_of(k);
@@ -518,8 +522,11 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
 #pragma unroll 1
                 for (uint32_t j = 0; j < D / 32; ++j) {
                     uint32_t o[32];
-                    if (done) {
+                    if (done) {                             // (zeros in both branches: one behind them takes registers from the loop over tiles)
                         tmem_ld32(o_addr + j * 32, o);
+                        if (none)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = 0;
                     } else {
 #pragma unroll
                         for (int e = 0; e < 32; ++e) o[e] = 0;
@@ -910,7 +917,7 @@ __global__ void __launch_bounds__(256) k_prompt_join(const __grid_constant__ Pro
         const uint32_t at = (item * NT + t) * a.tt + tok;     // the row's token
         if (tok >= a.tt || at >= q_len) continue;
         auto part = [&](uint32_t i) { return ((size_t)(slot + i) * a.p.n_kv + kvh) * (NT * 128) + r; };
-        float M = -INFINITY, L = 0.f;
+        float M = kNone, L = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
         for (uint32_t i0 = 0; i0 < pieces; i0 += 8) {
@@ -918,7 +925,7 @@ __global__ void __launch_bounds__(256) k_prompt_join(const __grid_constant__ Pro
             float4 z[8];
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
-                ml[i] = make_float2(-INFINITY, 0.f);
+                ml[i] = make_float2(kNone, 0.f);
                 z[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (i0 + i < pieces) {
                     ml[i] = __ldcg(reinterpret_cast<const float2 *>(a.ml + part(i0 + i) * 2));
@@ -928,19 +935,19 @@ __global__ void __launch_bounds__(256) k_prompt_join(const __grid_constant__ Pro
             float most = M;
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) most = fmaxf(most, ml[i].x);
-            if (most == -INFINITY) continue;
-            const float down = M == -INFINITY ? 0.f : ex2f(M - most);
+            if (most == kNone) continue;
+            const float down = M == kNone ? 0.f : ex2f(M - most);
             M = most;
             L *= down;
             y.x *= down; y.y *= down; y.z *= down; y.w *= down;
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
-                const float e = ml[i].x == -INFINITY ? 0.f : ex2f(ml[i].x - M);
+                const float e = ml[i].x == kNone ? 0.f : ex2f(ml[i].x - M);
                 L += e * ml[i].y;
                 y.x += e * z[i].x; y.y += e * z[i].y; y.z += e * z[i].z; y.w += e * z[i].w;
             }
         }
-        const float inv = M == -INFINITY ? 0.f : 1.f / L;
+        const float inv = M == kNone ? 0.f : 1.f / L;
         *reinterpret_cast<uint2 *>(a.out + (int64_t)(q0 + (int32_t)at) * a.ldo + (size_t)(kvh * a.group + r % 128 % a.group) * D + c) =
             make_uint2(pack_bf16(y.x * inv, y.y * inv), pack_bf16(y.z * inv, y.w * inv));
     }

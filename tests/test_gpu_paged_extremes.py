@@ -160,6 +160,43 @@ def test_prompts_with_a_key_that_is_not_finite(d, group, n_kv, page, new, kv, va
 
 
 @pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("d,group,n_kv,page,new,kv", PROMPTS)
+def test_prompts_with_a_nan(d, group, n_kv, page, new, kv, bits):
+    g = gen(d + 1)
+    pages = sum(-(-n // page) for n in kv) + 1
+    cache, table = make_cache(g, pages, page, n_kv, d, bits), make_table(g, kv, page, pages)
+    q = rnd(g, sum(new), group * n_kv, d).to(torch.bfloat16).to(DEV)
+    q[5, 1, 7] = NAN                                    # all scores of one row, whatever its tiles
+    nan = compare(q, cache, table, kv, new)
+    assert bool(nan[5, 1].all()) and int(nan.sum()) == d
+    first = kv[0] - new[0]
+    spoil(cache, table, 0, first + 20, NAN)             # a key that the first twenty do not see
+    nan = compare(q, cache, table, kv, new)
+    assert not bool(nan[:5].any()) and not bool(nan[6:20].any()) and bool(nan[20:].all())
+    nan = compare(q, cache, table, kv, new, window=1)   # one token sees nothing else, the others not at all
+    assert bool(nan[20].all()) and not bool(nan[21:].any()) and not bool(nan[6:20].any())
+
+
+@pytest.mark.parametrize("d,group,n_kv,page,new,kv", PROMPTS)
+def test_prompts_of_nothing_but_infinite_scores(d, group, n_kv, page, new, kv):
+    """-infinity as a whole tile, where others follow, and everywhere."""
+    g = gen(d + 2)
+    pages = sum(-(-n // page) for n in kv) + 1
+    cache, table = make_cache(g, pages, page, n_kv, d, 16), make_table(g, kv, page, pages)
+    q = rnd(g, sum(new), group * n_kv, d).to(torch.bfloat16).to(DEV)
+    q[..., 0] = 1.0
+    for j in range(128):
+        spoil(cache, table, 0, j, -INF)
+    assert not bool(compare(q, cache, table, kv, new).any())
+    for j in range(128, kv[0]):
+        spoil(cache, table, 0, j, -INF)
+    assert bool(compare(q, cache, table, kv, new).all())
+    for j in range(3):
+        spoil(cache, table, 0, kv[0] - new[0] - j, 0.5)
+    assert not bool(compare(q, cache, table, kv, new).any())
+
+
+@pytest.mark.parametrize("bits", [16, 4])
 def test_rows_behind_a_sequence_do_not_change_the_others(bits):
     """NaN in the queries of padding and of the next sequence, which lie in the same tile of query rows."""
     g = gen(23)
@@ -173,3 +210,21 @@ def test_rows_behind_a_sequence_do_not_change_the_others(bits):
     for _ in range(3):
         ci().paged_attention(junk.fill_(NAN), cache, table.to(DEV), i32([400, 400]), i32([0, 120, 200]))       # NaN left in shared memory
         assert torch.equal(ci().paged_attention(q, *args)[:100], want)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_row_that_sees_nothing_beside_rows_that_see_a_nan(bits):
+    """Its page is not there; the tokens behind it have a page, and a NaN among its values."""
+    g = gen(29)
+    cache = make_cache(g, 12, 32, 1, 64, bits)
+    table = torch.tensor([[-1, -1, -1, 0, 1, 2, 3]], dtype=torch.int32)
+    if bits == 16:
+        cache.v[0, 0, 3, 5] = NAN
+    else:
+        cache.v_scale[0, 0, 3, 0] = NAN
+    for new, kv in (([224], [224]), ([100], [130])):
+        q = rnd(g, sum(new), 2, 64).to(torch.bfloat16).to(DEV)
+        got = ci().paged_attention(q, cache, table.to(DEV), i32(kv), starts_of(new))
+        blind = 96 - (kv[0] - new[0])
+        assert bool((got[:blind] == 0).all())
+        assert bool(got[blind + 4:, 5].isnan().all())
