@@ -135,6 +135,7 @@ SIGNATURES = {
     "ci_paged_attention": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedBatch), _V, C.c_int64, C.c_uint32, C.c_uint32,
                                      C.c_uint32, C.c_uint32, C.c_float, _V, C.c_size_t, _V, C.c_int64, _S]),
     "ci_paged_status": (C.c_int, [u32p, C.c_int, _S]),
+    "ci_paged_set_wait_limit": (None, [C.c_uint32, C.c_uint32]),
     "ci_adjust_logits": (C.c_int, [C.POINTER(LogitAdjust), _S]),
     "ci_allreduce_buffer_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32]),
     "ci_allreduce_counter_bytes": (C.c_size_t, []),

@@ -50,6 +50,7 @@ struct PromptArgs {
     const int4 *plan, *cuts;                 // see PromptPlan
     int32_t *next;                           // the first piece that no block has yet
     uint32_t count;                          // pieces and places for them, each for every head
+    uint32_t polls, at_once;                 // of a wait before it gives up; the code whose waits give up at once
     float *ml, *partial;                     // of pieces: [slots][NT 128][2], [slots][NT 128][D]
 };
 
@@ -205,7 +206,9 @@ __device__ __forceinline__ int32_t exponent_of(float x) {
 }
 __device__ __forceinline__ float power_of_2(int32_t n) { return __uint_as_float((uint32_t)(min(max(n, -126), 127) + 127) << 23); }
 
-template <int D, int BITS>
+// SHORT: with the limits of ci_paged_set_wait_limit; reading them at each wait costs 1 to 2 % (4 x 2000 tokens, heads of 64 in 4 bits:
+// 109.0 us instead of 107.1), so the kernel that serves calls has a constant.
+template <int D, int BITS, bool SHORT>
 __global__ void __launch_bounds__(PromptShape<D, BITS>::kThreads, 1)
 k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                const __grid_constant__ CUtensorMap v_map) {
@@ -257,8 +260,11 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     tc_fence_after();
     const uint32_t tmem = uniform(*s_tmem);
     auto give_up = [&](uint32_t code) {
-        if (lane == 0) { atomicExch(&g_prompt_status, code); *s_abort = 1; }
+        if (lane == 0) { atomicCAS(&g_prompt_status, 0u, code); *s_abort = 1; }     // the first one's stays
     };
+    // Waits of the roles on each other.  Those for what this block has in flight itself (14, and behind the last piece) go by the
+    // usual limit whatever these have.
+    auto polls = [&](uint32_t code) { return !SHORT ? kWaitPolls : code == a.at_once ? 0u : a.polls; };
 
     // ---- pieces, one after the other: the roles run ahead of each other across their borders ------------------------
     QueryTile qt[NT];
@@ -266,7 +272,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     uint32_t b = 0;
     uint32_t ring0 = 0, q_count = 0;                            // tiles of K and V, and of Q, before this piece
     auto get_item = [&](uint32_t k) {                           // false: there is none (or the wait ran out)
-        if (!__all_sync(kFull, mbar_wait(bar(Sh::bItem + k % 2), k / 2 & 1))) {
+        if (!__all_sync(kFull, mbar_wait(bar(Sh::bItem + k % 2), k / 2 & 1, polls(20)))) {
             give_up(20);
             return false;
         }
@@ -322,7 +328,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             volatile const int32_t *s_scale = reinterpret_cast<volatile const int32_t *>(smem + Sh::oBar + Sh::oScale);
             int32_t v_exp = 0;                                      // O stands for O 2^v_exp
             if (BITS == 4 && kt.n > 0) {                            // this row of Q to fp16, its largest value below 2^15
-                ok = __all_sync(kFull, mbar_wait(bar(Sh::bQ), q_count & 1));
+                ok = __all_sync(kFull, mbar_wait(bar(Sh::bQ), q_count & 1, polls(18)));
                 if (!ok) give_up(18);
                 const uint32_t q_s = smem_s + Sh::oQ + t * Sh::kTile + row * 128;
                 auto chunk = [&](uint32_t c) { return q_s + (c / 8) * Sh::kBlock + ((c % 8 ^ (row & 7)) << 4); };
@@ -360,7 +366,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 const int32_t f = kt.first(i);
                 const bool edge = gone || f + (int32_t)kKt - 1 > min(q.p0, p.cap - 1) ||
                                   (a.window && f <= q.p1 - a.window && f + (int32_t)kKt > a.sinks);
-                if (!__all_sync(kFull, mbar_wait(bar(Sh::bS + t), turn & 1))) {
+                if (!__all_sync(kFull, mbar_wait(bar(Sh::bS + t), turn & 1, polls(11)))) {
                     give_up(11);
                     ok = false;
                     break;
@@ -371,7 +377,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     // The tile of V cannot be replaced before this row's weights are out, so its barrier can be waited on here; the
                     // exponents of the tile were written before it.
                     const uint32_t c = ring0 + 2 * (uint32_t)i + 1, at = c / 2 % 8;
-                    if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1))) {
+                    if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1, polls(19)))) {
                         give_up(19);
                         ok = false;
                         break;
@@ -449,7 +455,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 // tile: a prompt of 16001 under a window of 4096 1225 us instead of 780 then.)
                 if (BITS == 16 && (f + (int32_t)kKt > kt.hi || (a.window && f < kt.lo && f + (int32_t)kKt > a.sinks))) {
                     const uint32_t c = ring0 + 2 * (uint32_t)i + 1;
-                    if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1))) {
+                    if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1, polls(16)))) {
                         give_up(16);
                         ok = false;
                         break;
@@ -506,7 +512,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 l += l0 + l1;
             }
             // ---- the row's result ----------------------------------------------------------------------------------
-            if (ok && !mbar_wait(bar(Sh::bO + t), k & 1)) { give_up(12); ok = false; }
+            if (ok && !mbar_wait(bar(Sh::bO + t), k & 1, polls(12))) { give_up(12); ok = false; }
             ok = __all_sync(kFull, ok && !*s_abort);
             if (__all_sync(kFull, ok)) {
                 tc_fence_after();
@@ -549,6 +555,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     }
                 }
             }
+            if (!ok) tmem_st_wait();                                // (nothing under way into tensor memory that is given back)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(Sh::bRead + t));         // O may be written again
@@ -569,7 +576,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         const uint64_t q_desc = umma_desc_sw128(smem_s + Sh::oQ + t * Sh::kTile), k_desc = umma_desc_sw128(smem_s + Sh::oRing);
         const uint64_t v_desc = umma_desc_sw128_mn(smem_s + Sh::oRing, Sh::kBlock);
         const uint32_t s_col = tmem + t * kKt, o_col = tmem + Sh::cO + t * D;
-        auto full = [&](uint32_t c) { return mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1); };
+        auto full = [&](uint32_t c) { return mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1, polls(13)); };
         auto scores = [&](int32_t i) {
             tc_fence_after();
             const uint64_t kd = k_desc + ((ring0 + 2 * i) % NS) * (Sh::kTile >> 4);
@@ -597,7 +604,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             if (NT == 2 && t == 1) q = qt[NT - 1];
             bool first = true;                                      // no product with V yet: O is written, not added to
             if (kt.n > 0) {
-                ok = __all_sync(kFull, mbar_wait(bar(BITS == 16 ? Sh::bQ : Sh::bQh), q_count & 1) && full(ring0));
+                ok = __all_sync(kFull, mbar_wait(bar(BITS == 16 ? Sh::bQ : Sh::bQh), q_count & 1, polls(13)) && full(ring0));
                 if (!ok) break;
                 if (kt.seen_by(q, 0)) scores(0);
                 release(ring0);
@@ -605,7 +612,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             }
             for (int32_t i = 0; i < kt.n && ok; ++i) {
                 if (NT == 2 && (t == 1 || round > 0)) {
-                    ok = __all_sync(kFull, mbar_wait(bar(Sh::bTurn + t), (t == 1 ? round : round - 1) & 1));
+                    ok = __all_sync(kFull, mbar_wait(bar(Sh::bTurn + t), (t == 1 ? round : round - 1) & 1, polls(13)));
                     if (!ok) break;
                 }
                 ++round;
@@ -614,7 +621,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     ok = __all_sync(kFull, full(ring0 + 2 * i + 1));
 #pragma unroll
                     for (uint32_t h = 0; h < 2; ++h) {              // the weights come in two halves
-                        ok = ok && __all_sync(kFull, mbar_wait(bar(Sh::bP + 2 * t + h), made & 1));
+                        ok = ok && __all_sync(kFull, mbar_wait(bar(Sh::bP + 2 * t + h), made & 1, polls(13)));
                         if (!ok) break;
                         tc_fence_after();
                         if (elect_one()) {
@@ -643,7 +650,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             }
             if (!ok) break;
             // (not before the rows' threads have waited for the piece before: a phase that nobody has seen would be lost)
-            if (k > 0 && !__all_sync(kFull, mbar_wait(bar(Sh::bRead + t), (k - 1) & 1))) {
+            if (k > 0 && !__all_sync(kFull, mbar_wait(bar(Sh::bRead + t), (k - 1) & 1, polls(13)))) {
                 ok = false;
                 break;
             }
@@ -658,7 +665,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
     } else if (warp == Sh::kSched) {
         // =========================== which piece next ===============================================================
         for (uint32_t k = 0;; ++k) {
-            if (!mbar_wait_warp(bar(Sh::bTaken + k % 2), (k / 2 & 1) ^ 1)) { give_up(21); break; }
+            if (!mbar_wait_warp(bar(Sh::bTaken + k % 2), (k / 2 & 1) ^ 1, polls(21))) { give_up(21); break; }
             uint32_t v = 0;
             if (lane == 0) v = (uint32_t)atomicAdd(a.next, 1);
             v = __shfl_sync(kFull, v, 0);
@@ -727,7 +734,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         int32_t q_row = 0;                                      // and first token
         bool ok = true;
         auto load_q = [&]() {
-            if (q_count && !mbar_wait_warp(bar(Sh::bQfree), (q_count - 1) & 1)) return false;
+            if (q_count && !mbar_wait_warp(bar(Sh::bQfree), (q_count - 1) & 1, polls(22))) return false;
             if (lane == 0) {
                 const uint32_t bytes = a.tt * a.group * 128;    // of a block of 64 channels
                 mbar_expect_tx(bar(Sh::bQ), NT * NB * bytes);
@@ -755,7 +762,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 if (i + 1 < kt.n) next = row_of(i + 1);
                 for (uint32_t kv = 0; kv < 2; ++kv, ++issued) {
                     const uint32_t slot = issued % NS;
-                    if (!mbar_wait_warp(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1) || __any_sync(kFull, *s_abort)) { give_up(15); ok = false; break; }
+                    if (!mbar_wait_warp(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1, polls(15)) || __any_sync(kFull, *s_abort)) { give_up(15); ok = false; break; }
                     const uint32_t to = bar(Sh::bFull + slot), dst = smem_s + Sh::oRing + slot * Sh::kTile;
                     if (lane == 0) mbar_expect_tx(to, Sh::kTile);
                     __syncwarp();
@@ -769,9 +776,9 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             }
             end_item();
         }
-        if (!ok)                                                // copies under way end before the block does
-            for (uint32_t c = issued > NS ? issued - NS : 0; c < issued; ++c) (void)mbar_wait_warp(bar(Sh::bFull + c % NS), (c / NS) & 1);
-        if (!ok && queries) (void)mbar_wait_warp(bar(Sh::bQ), (queries - 1) & 1);
+        // Copies under way end before the block does: others may have given up on them, and this warp have left for that.
+        for (uint32_t c = issued > NS ? issued - NS : 0; c < issued; ++c) (void)mbar_wait_warp(bar(Sh::bFull + c % NS), (c / NS) & 1);
+        if (queries) (void)mbar_wait_warp(bar(Sh::bQ), (queries - 1) & 1);
     } else {
         // =========================== codes to fp16: a thread, or two, per position ==========================================
         constexpr uint32_t G = D / 64;
@@ -824,7 +831,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             else e = v_exp;
             const float down = power_of_2(-e / 2), down2 = power_of_2(-e - -e / 2);
             const uint32_t slot = issued % NS, dst = smem_s + Sh::oRing + slot * Sh::kTile + y * 128;
-            if (ok && !__all_sync(kFull, mbar_wait(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1))) {
+            if (ok && !__all_sync(kFull, mbar_wait(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1, polls(17)))) {
                 give_up(17);
                 ok = false;
             }
@@ -864,7 +871,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             if (kt.n > 0) {
                 fetch(f0, id, 0, 0);
                 if (warp == Sh::kProd) {
-                    if (q_count) ok = mbar_wait_warp(bar(Sh::bQfree), (q_count - 1) & 1);
+                    if (q_count) ok = mbar_wait_warp(bar(Sh::bQfree), (q_count - 1) & 1, polls(22));
                     if (!ok) give_up(22);
                     if (ok && lane == 0) {
                         const uint32_t bytes = a.tt * a.group * 128;
@@ -891,7 +898,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             }
             end_item();
         }
-        if (!ok && queries) (void)mbar_wait_warp(bar(Sh::bQ), (queries - 1) & 1);
+        if (queries) (void)mbar_wait_warp(bar(Sh::bQ), (queries - 1) & 1);
     }
     tc_fence_before();
     __syncthreads();
@@ -953,6 +960,9 @@ __global__ void __launch_bounds__(256) k_prompt_join(const __grid_constant__ Pro
     }
 }
 
+// (of the process; ci_paged_set_wait_limit)
+static uint32_t g_prompt_polls = kWaitPolls, g_prompt_at_once = 0;
+
 static size_t prompt_slot_rows(uint32_t head_dim) { return 2 * (size_t)sm_count() * (head_dim == 256 ? 128 : 256); }     // of all slots
 
 PromptPlan prompt_plan(uint32_t head_dim, uint32_t page_size, uint32_t n_kv, const ci_paged_batch *b, uint32_t group, int32_t window,
@@ -975,11 +985,11 @@ size_t prompt_workspace_bytes(uint32_t head_dim, const PromptPlan &l) {
     return (((size_t)l.sms + 2 + l.count) * 2) * sizeof(int4) + prompt_slot_rows(head_dim) * (2 + (size_t)head_dim) * sizeof(float);
 }
 
-template <int D, int BITS>
+template <int D, int BITS, bool SHORT>
 static int launch_prompt(const PromptArgs &a, const PromptPlan &l, const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t s) {
     using Sh = PromptShape<D, BITS>;
     static SmemLimit lim = {};
-    if (int rc = ensure_smem_limit(lim, (const void *)k_paged_prompt<D, BITS>, Sh::kSmem)) return rc;
+    if (int rc = ensure_smem_limit(lim, (const void *)k_paged_prompt<D, BITS, SHORT>, Sh::kSmem)) return rc;
     const uint64_t blocks = (uint64_t)l.count * a.p.n_kv;
     CI_REQUIRE(blocks <= 0x7FFFFFFFu, "too many blocks");
     cudaLaunchConfig_t cfg = {};
@@ -992,7 +1002,7 @@ static int launch_prompt(const PromptArgs &a, const PromptPlan &l, const CUtenso
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    CI_CUDA(cudaLaunchKernelEx(&cfg, k_paged_prompt<D, BITS>, a, qm, km, vm));
+    CI_CUDA(cudaLaunchKernelEx(&cfg, k_paged_prompt<D, BITS, SHORT>, a, qm, km, vm));
     if (!l.may_cut) return CI_OK;
     cfg.gridDim = dim3(l.sms + 1, Sh::NT * 128 / kJoinRows);    // (two pieces at least to a cut item)
     cfg.blockDim = dim3(256);
@@ -1033,6 +1043,8 @@ int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const Prom
     a.cuts = l.cuts;
     a.next = &l.cuts->y;
     a.count = l.count * p.n_kv;
+    a.polls = g_prompt_polls;
+    a.at_once = g_prompt_at_once;
     a.ml = (float *)(l.pieces + (size_t)l.count * 2);
     a.partial = a.ml + prompt_slot_rows(c->head_dim) * 2;
     CUtensorMap qm, km, vm;
@@ -1051,11 +1063,16 @@ int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const Prom
     if (c->bits == 16) {
         if (int rc = pool_map(&km, c, c->k)) return rc;
         if (int rc = pool_map(&vm, c, c->v)) return rc;
-        return c->head_dim == 64 ? launch_prompt<64, 16>(a, l, qm, km, vm, s) : c->head_dim == 128 ? launch_prompt<128, 16>(a, l, qm, km, vm, s)
-                                                                                             : launch_prompt<256, 16>(a, l, qm, km, vm, s);
     }
-    return c->head_dim == 64 ? launch_prompt<64, 4>(a, l, qm, km, vm, s) : c->head_dim == 128 ? launch_prompt<128, 4>(a, l, qm, km, vm, s)
-                                                                                         : launch_prompt<256, 4>(a, l, qm, km, vm, s);
+    const bool usual = a.polls == kWaitPolls && a.at_once == 0;
+    auto launch = [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        return c->bits == 16 ? (usual ? launch_prompt<D, 16, false>(a, l, qm, km, vm, s) : launch_prompt<D, 16, true>(a, l, qm, km, vm, s))
+                             : (usual ? launch_prompt<D, 4, false>(a, l, qm, km, vm, s) : launch_prompt<D, 4, true>(a, l, qm, km, vm, s));
+    };
+    return c->head_dim == 64    ? launch(std::integral_constant<int, 64>())
+           : c->head_dim == 128 ? launch(std::integral_constant<int, 128>())
+                                : launch(std::integral_constant<int, 256>());
 }
 
 }  // namespace ci
@@ -1066,4 +1083,9 @@ extern "C" int ci_paged_status(uint32_t *code, int clear, ci_stream_t stream) {
     void *word = nullptr;
     CI_CUDA(cudaGetSymbolAddress(&word, g_prompt_status));
     return ci_status((uint32_t *)word, code, clear, stream);
+}
+
+extern "C" void ci_paged_set_wait_limit(uint32_t polls, uint32_t code) {
+    g_prompt_polls = polls ? polls : kWaitPolls;
+    g_prompt_at_once = code;
 }

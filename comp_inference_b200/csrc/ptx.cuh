@@ -5,7 +5,7 @@
 
 namespace ci {
 
-constexpr uint32_t kWaitPolls = 1u << 22;   // mbarrier polls before a wait gives up
+constexpr uint32_t kWaitPolls = 1u << 22;   // mbarrier polls before a wait gives up, each of up to 4 us
 constexpr uint32_t kLutBytes = kProbScale * 4;
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -286,9 +286,9 @@ __device__ __forceinline__ void sts_v4(uint32_t addr, uint32_t a, uint32_t b, ui
 }
 
 // Every lane polls an mbarrier phase itself, bounded.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t polls = kWaitPolls) {
     uint32_t ok = 0;
-    for (uint32_t it = 0; it < kWaitPolls && !ok; ++it) ok = mbar_try_wait(bar, parity);
+    for (uint32_t it = 0; it < polls && !ok; ++it) ok = mbar_try_wait(bar, parity);
     return ok != 0;
 }
 
@@ -337,10 +337,10 @@ inline double run_cost(uint32_t units, uint32_t w, double extra) {
 }
 
 // Lane 0 polls an mbarrier phase, bounded; the verdict is broadcast to the warp.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, uint32_t polls = kWaitPolls) {
     uint32_t ok = 0;
     if (lane_id() == 0)
-        for (uint32_t it = 0; it < kWaitPolls && !ok; ++it) ok = mbar_try_wait(bar, parity);
+        for (uint32_t it = 0; it < polls && !ok; ++it) ok = mbar_try_wait(bar, parity);
     return __shfl_sync(kFull, ok, 0) != 0;
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {

@@ -450,6 +450,9 @@ int ci_paged_attention(const ci_paged_cache *cache, const ci_paged_batch *batch,
 /* ci_status for the waits inside ci_paged_attention on the current device: a wait that runs out ends the call with wrong
  * outputs and leaves its code here.  Waits for `stream`; the first call on a device outside any stream capture. */
 int ci_paged_status(uint32_t *code, int clear, ci_stream_t stream);
+/* How often those waits poll before they give up (process-wide; 0 restores the default of several seconds), and the code of waits
+ * that give up without a poll (0: none).  For tests of the give-up path and for hosts with their own watchdog. */
+void ci_paged_set_wait_limit(uint32_t polls, uint32_t code);
 
 /* Logits [B, V] (bf16, rows ld_in / ld_out apart; d_out may be d_in) as a sampler adjusts them, in fp32 with one rounding:
  *   x / r (x > 0) or x * r, r = d_repetition[b], for tokens of the history d_tokens[b][0 .. d_lens[b]);
