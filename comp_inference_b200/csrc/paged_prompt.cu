@@ -96,11 +96,12 @@ __device__ __forceinline__ float ex2f(float x) {
 struct QueryTile {
     int32_t p0, p1, from, to;
 };
-// The key tiles that a block visits: tile i of n starts at first(i).
+// The key tiles that a block visits: tile i of n starts at first(i).  The first n_sink lie in front of the windows; n_first, these and
+// what one query tile still has in its window, hold first tokens.
 struct KeyTiles {
-    int32_t lo, hi, t_lo, n_sink, n;
+    int32_t lo, hi, t_lo, n_sink, n, n_first;
     __device__ __forceinline__ int32_t first(int32_t i) const { return (i < n_sink ? i : t_lo + i - n_sink) * (int32_t)kKt; }
-    __device__ __forceinline__ bool seen_by(const QueryTile &q, int32_t i) const { return i < q.to && (i < n_sink || i >= q.from); }
+    __device__ __forceinline__ bool seen_by(const QueryTile &q, int32_t i) const { return i < q.to && (i >= q.from || i < n_first); }
     // Of these tiles only those of one piece of several.  The first tokens of a window go with the first one.
     __device__ __forceinline__ void take(uint32_t piece, uint32_t pieces) {
         auto begin = [&](uint32_t k) {
@@ -117,7 +118,7 @@ struct KeyTiles {
 };
 
 // A piece as the scheduling warp hands it to the others; sequence < 0: there is no more.
-enum PieceWords : uint32_t { kSequence, kHead, kFirstRow, kPieces, kSlot, kTilesAt, kQueriesAt = kTilesAt + 5 };
+enum PieceWords : uint32_t { kSequence, kHead, kFirstRow, kPieces, kSlot, kTilesAt, kQueriesAt = kTilesAt + 6 };
 static_assert(kQueriesAt + 8 <= kItemWords, "room for two query tiles");
 
 // The same in every lane: said to the compiler, which then forms what depends on it in uniform registers.
@@ -279,7 +280,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         volatile const int32_t *x = s_items + k % 2 * kItemWords;
         if (__any_sync(kFull, x[kSequence] < 0 || *s_abort)) return false;
         b = (uint32_t)uniform(x[kSequence]);
-        kt = {uniform(x[kTilesAt]), uniform(x[kTilesAt + 1]), uniform(x[kTilesAt + 2]), uniform(x[kTilesAt + 3]), uniform(x[kTilesAt + 4])};
+        kt = {uniform(x[kTilesAt]), uniform(x[kTilesAt + 1]), uniform(x[kTilesAt + 2]), uniform(x[kTilesAt + 3]), uniform(x[kTilesAt + 4]), uniform(x[kTilesAt + 5])};
 #pragma unroll
         for (uint32_t t = 0; t < NT; ++t)
             qt[t] = {uniform(x[kQueriesAt + 4 * t]), uniform(x[kQueriesAt + 4 * t + 1]), uniform(x[kQueriesAt + 4 * t + 2]), uniform(x[kQueriesAt + 4 * t + 3])};
@@ -696,6 +697,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             kt.n_sink = a.window ? min((min(a.sinks, kt.hi) + (int32_t)kKt - 1) / (int32_t)kKt, kt.t_lo) : 0;
             kt.n = kt.n_sink + (kt.hi + (int32_t)kKt - 1) / (int32_t)kKt - kt.t_lo;
             if (w0.w > 1) kt.take((uint32_t)w0.z, (uint32_t)w0.w);
+            kt.n_first = a.window ? kt.n_sink + max((min(a.sinks, kt.hi) + (int32_t)kKt - 1) / (int32_t)kKt - kt.t_lo, 0) : 0;
 #pragma unroll
             for (uint32_t t = 0; t < NT; ++t) {
                 qt[t].from = lo[t] / (int32_t)kKt - kt.t_lo + kt.n_sink;
@@ -713,6 +715,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 x[kTilesAt + 2] = kt.t_lo;
                 x[kTilesAt + 3] = kt.n_sink;
                 x[kTilesAt + 4] = kt.n;
+                x[kTilesAt + 5] = kt.n_first;
 #pragma unroll
                 for (uint32_t t = 0; t < NT; ++t) {
                     x[kQueriesAt + 4 * t] = qt[t].p0;
