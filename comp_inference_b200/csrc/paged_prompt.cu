@@ -21,7 +21,9 @@
 // A cache of 4 bits is turned into fp16 on its way into shared memory by four or eight warps, so that what codes stand for, and the
 // weights, are rounded by 2^-12 and not 2^-9 (error of a prompt's outputs against 64 bits 0.0017 instead of 0.0034; bf16's own
 // rounding of the result is 0.0016).  fp16 has no range for that by itself: every key tile is scaled by the power of two that
-// its largest value asks for, the values by one that only grows, O following it, and a query row by its own.
+// its largest value asks for, the values by one that changes when a tile leaves its range, O following it, and a query row by its own.
+// A value tile's largest lies between 2^8 and 2^15 of its scale, so steps and lowest values down to 2^-25 of that are held exactly.  The
+// scale stays above 2^-92 of the largest value of the piece so far: O of the rows that have seen that one must not overflow.
 //
 // What bounds it: in bf16 the chain from a tile's scores over its exponentials to its product, with two tiles in turn (tensor
 // pipe 61 % active, issue slots 47 %, special functions 47 %; 16001 tokens under a window of 4096: 772 us, 1214 TFLOP/s, 0.73 of the
@@ -79,8 +81,9 @@ struct PromptShape {
     static constexpr uint32_t bQ = 0, bFull = 1, bEmpty = bFull + NS, bS = bEmpty + NS, bP = bS + NT, bO = bP + 2 * NT, bRead = bO + NT, bTurn = bRead + NT,
                               bQh = bTurn + 2, bQfree = bQh + 1, bItem = bQfree + 1, bTaken = bItem + 2, bEnd = bTaken + 2;
     static constexpr uint32_t oTmem = (bEnd + 1) * 8, oAbort = oTmem + 4, oItem = oTmem + 8;
-    static constexpr uint32_t oScale = oItem + 2 * kItemWords * 4, oLargest = oScale + 64;   // 4 bits: exponents of eight tiles' K and V; of warps
-    static_assert(oLargest + 64 <= kMisc, "barrier region");
+    static constexpr uint32_t oScale = oItem + 2 * kItemWords * 4, oLargest = oScale + 64;   // 4 bits: exponents of eight tiles' K and V; of warps;
+    static constexpr uint32_t oTop = oLargest + 64;                          // and no tile's values of the piece had a larger one
+    static_assert(oTop + 4 <= kMisc, "barrier region");
     static constexpr int kHeld = BITS == 16 ? 4 : 2;                         // groups of 32 scores that a row's thread holds
     static constexpr uint32_t cO = NT * kKt;                                 // first column of O
 };
@@ -373,7 +376,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     break;
                 }
                 tc_fence_after();
-                float v_down = 1.f;                                 // what O is to be multiplied by for the scale of this tile's V
+                int32_t v_move = 0;                                 // O is to be multiplied by 2^v_move for the scale of this tile's V
                 if (BITS == 4) {
                     // The tile of V cannot be replaced before this row's weights are out, so its barrier can be waited on here; the
                     // exponents of the tile were written before it.
@@ -385,7 +388,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     }
                     const int32_t ke = s_scale[at], ve = s_scale[8 + at];
                     scale = fmaxf(row_scale * power_of_2(ke / 2) * power_of_2(ke - ke / 2), 1.2e-38f);
-                    v_down = done ? power_of_2(v_exp - ve) : 1.f;
+                    v_move = done ? v_exp - ve : 0;
                     v_exp = ve;
                 }
                 const uint64_t scale2 = pair(scale, scale);
@@ -433,13 +436,13 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 // A score that is not finite (rows behind the sequence hold anything): its weight is 0 or NaN, which ex2_poly has not.
                 const bool odd = BITS == 16 && !edge && live && !(fabsf(mx) < INFINITY);
                 bool exact = edge;
-                if (__any_sync(kFull, grow || odd || v_down != 1.f)) {
+                if (__any_sync(kFull, grow || odd || v_move != 0)) {
                     exact |= BITS == 16 && __any_sync(kFull, odd);
                     float c = grow ? ex2f(m - mx) : 1.f;
                     if (grow) m = mx;
 #pragma unroll
                     for (int e = 0; e < kSums; ++e) l2[e] = fma2(l2[e], pair(c, c), 0);
-                    c *= v_down;
+                    if (BITS == 4) c *= power_of_2(v_move / 2) * power_of_2(v_move - v_move / 2);
                     if (done) {
 #pragma unroll 1
                         for (uint32_t j = 0; j < D / 32; ++j) {
@@ -790,6 +793,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
         const bool first_thread = threadIdx.x == Sh::kProd * 32;
         volatile int32_t *s_scale = reinterpret_cast<volatile int32_t *>(smem + Sh::oBar + Sh::oScale);
         volatile uint32_t *s_largest = reinterpret_cast<volatile uint32_t *>(smem + Sh::oBar + Sh::oLargest);
+        volatile int32_t *s_top = reinterpret_cast<volatile int32_t *>(smem + Sh::oBar + Sh::oTop);    // (no register for it in the loop)
         uint32_t issued = 0, queries = 0, kvh = 0;
         int32_t q_row = 0, v_exp;
         bool ok = true;
@@ -830,8 +834,15 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             for (uint32_t w = 0; w < PW; ++w) e = max(e, (int32_t)s_largest[(issued & 1) * 8 + w]);
             e -= 200;
             if (kv == 0) e -= 14;                           // below 2^14
-            else if (e - v_exp > 15) e = v_exp = e - 12;    // below 2^15; where it has to grow, below 2^12 again
-            else e = v_exp;
+            else {
+                // from 2^8 to 2^15; where it has to change, below 2^12 again (a tile of zeros changes nothing)
+                if (e - v_exp > 15 || (e - v_exp <= 8 && e > -126)) {
+                    const int32_t top = max(*s_top, max(e, v_exp + 15));    // no tile so far had more
+                    *s_top = top;                               // (the same from every thread, whichever was here before)
+                    if (e - v_exp > 15 || top - 80 < v_exp) v_exp = max(e - 12, top - 80);
+                }
+                e = v_exp;
+            }
             const float down = power_of_2(-e / 2), down2 = power_of_2(-e - -e / 2);
             const uint32_t slot = issued % NS, dst = smem_s + Sh::oRing + slot * Sh::kTile + y * 128;
             if (ok && !__all_sync(kFull, mbar_wait(bar(Sh::bEmpty + slot), ((issued / NS) & 1) ^ 1, polls(17)))) {
@@ -869,6 +880,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
             q_row = first_row_of(k);
             leave_item(k);
             v_exp = -1000;                                          // (no tile of V yet)
+            *s_top = -126;
             Codes f0, f1;
             int32_t id = page_at(0), id_next = page_at(1);
             if (kt.n > 0) {

@@ -97,8 +97,11 @@ def paged_attention(q, cache, block_table, kv_lens, q_starts=None, max_q_len=0, 
     known; it chooses between kernels, and a longer sequence is served all the same.  ``scale``: head_dim ** -0.5 if not given.
     ``out``: rows that do not overlap q, 16-byte aligned (columns of a wider matrix included).
 
-    Where several new tokens of one sequence stand in one call, an infinity or a NaN in a value that a later one sees may
-    reach the earlier ones; what lies behind a sequence's end, outside everyone's window or on no page reaches nobody."""
+    A NaN or +infinity among a token's scores makes its row NaN, -infinity is a weight of 0, nothing but -infinity NaN (0 / 0).
+    Where several new tokens of one sequence stand in one call, an infinity or a NaN in a value that one of them sees may reach the
+    others, the earlier ones and, under a window, the later ones too; what lies behind a sequence's end, outside everyone's
+    window or on no page reaches nobody.  In a cache of 4 bits the values of 128 neighbouring positions then share a power of two: steps
+    below 2^-25 of the largest value among them, or 2^-90 of the largest so far, lose bits."""
     return cache._handle.attention(q, block_table, kv_lens, q_starts, max_q_len, window, sinks, scale, out)
 
 

@@ -228,3 +228,20 @@ def test_a_row_that_sees_nothing_beside_rows_that_see_a_nan(bits):
         blind = 96 - (kv[0] - new[0])
         assert bool((got[:blind] == 0).all())
         assert bool(got[blind + 4:, 5].isnan().all())
+
+
+@pytest.mark.parametrize("d,group,new,kv,window", [(128, 2, 600, 600, 20), (64, 1, 600, 600, 5), (256, 1, 600, 600, 150), (128, 1, 700, 1000, 64)])
+def test_values_that_shrink_under_a_window(d, group, new, kv, window):
+    """Values of 4 bits that shrink along the sequence by 2^60 (12.8 binary places in a tile of 128 positions), and in the last case tiles
+    of 1e20 and of 1 in turn: rows that see the small ones alone, beside rows that see the large ones."""
+    g = gen(d + kv)
+    table = make_table(g, [kv], 32, kv // 32 + 2)
+    pos = torch.arange(kv, dtype=torch.float64)
+    grow = 2.0 ** (30.0 - pos / 10.0) if kv == 600 else torch.where(pos % 256 < 128, 1e20, 1.0)
+    one, none = torch.ones(kv, d, dtype=torch.bfloat16, device=DEV), torch.zeros(kv, d, dtype=torch.bfloat16, device=DEV)
+    cache = ci().PagedKVCache(kv // 32 + 2, 32, 1, d, 4, DEV)
+    k, v = rnd(g, kv, d).to(torch.bfloat16).to(DEV), (grow[:, None] * rnd(g, kv, d)).to(torch.bfloat16).to(DEV)
+    ci().rope_paged_append(k, k, v, one, none, cache, table.to(DEV), i32([kv]), i32([0, kv]))
+    q = rnd(g, new, group, d).to(torch.bfloat16).to(DEV)
+    for sinks in (0, 3):
+        compare(q, cache, table, [kv], [new], window=window, sinks=sinks)
