@@ -619,12 +619,19 @@ ci_paged_batch paged_batch(const PagedCache &cache, const Tensor &table, const T
     return b;
 }
 
-// [T, heads, d] or [T, heads * d] with the heads side by side, as rows `ld` apart; copied where `align` asks for 16-byte rows
-// that it does not have.
+// [T, heads, d] or [T, heads * d] with the heads side by side, as rows `ld` apart; to be copied (ready) where it is laid out otherwise,
+// or `align` asks for 16-byte rows that it does not have.
 struct HeadRows {
     Tensor keep;
-    const uint16_t *ptr;
+    const uint16_t *ptr;                         // null until ready() where it has to be copied
     int64_t T, heads, ld;
+    // Behind the last check of a call: until then nothing is queued.
+    void ready() {
+        if (ptr != nullptr) return;
+        keep = keep.contiguous();
+        if (!aligned16(keep)) keep = keep.clone();
+        ptr = (const uint16_t *)keep.data_ptr();
+    }
 };
 HeadRows head_rows(const Tensor &x, int64_t d, const char *name, bool align) {
     want(x, at::kBFloat16, name);
@@ -638,17 +645,16 @@ HeadRows head_rows(const Tensor &x, int64_t d, const char *name, bool align) {
     // rows that overlap (an expanded tensor) are copied too
     const bool rows = r.T <= 1 || x.stride(0) >= r.heads * d;
     const bool ok = side_by_side && rows && (!align || (aligned16(x) && (r.T <= 1 || x.stride(0) % 8 == 0)));
-    r.keep = ok ? x : x.contiguous();
-    if (align && !aligned16(r.keep)) r.keep = r.keep.clone();
-    r.ld = r.T > 1 ? r.keep.stride(0) : r.heads * d;
-    r.ptr = (const uint16_t *)r.keep.data_ptr();
+    r.keep = x;
+    r.ld = ok && r.T > 1 ? x.stride(0) : r.heads * d;
+    r.ptr = ok ? (const uint16_t *)x.data_ptr() : nullptr;
     return r;
 }
 
 Tensor paged_append(PagedCache &cache, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &cos, const Tensor &sin,
                     const Tensor &table, const Tensor &kv_lens, const OptTensor &q_starts, const OptTensor &out) {
     const int64_t d = cache.c.head_dim, n_kv = cache.c.n_kv;
-    const HeadRows rq = head_rows(q, d, "q", false), rk = head_rows(k, d, "k", false), rv = head_rows(v, d, "v", false);
+    HeadRows rq = head_rows(q, d, "q", false), rk = head_rows(k, d, "k", false), rv = head_rows(v, d, "v", false);
     REFUSE(rk.T != rq.T || rv.T != rq.T, "q, k and v have " + std::to_string(rq.T) + ", " + std::to_string(rk.T) + " and " + std::to_string(rv.T) + " tokens");
     REFUSE(rk.heads != n_kv || rv.heads != n_kv, "k and v have " + std::to_string(rk.heads) + " and " + std::to_string(rv.heads) + " heads, the cache " + std::to_string(n_kv));
     want(cos, at::kBFloat16, "cos");
@@ -668,9 +674,13 @@ Tensor paged_append(PagedCache &cache, const Tensor &q, const Tensor &k, const T
     else y = at::empty({rq.T, rq.heads, d}, q.options());
     if (rq.T == 0 || b.B == 0) return y;
     const int64_t w = rq.heads * d, wk = rk.heads * d;
-    REFUSE((y.data_ptr() != (const void *)rq.ptr || (rq.T > 1 && rq.ld != w)) && overlap(y.data_ptr(), rq.T, w, w, rq.ptr, rq.T, w, rq.ld), "out overlaps q; it may be all of q, or none");
-    REFUSE(overlap(y.data_ptr(), rq.T, w, w, rk.ptr, rq.T, wk, rk.ld) || overlap(y.data_ptr(), rq.T, w, w, rv.ptr, rq.T, wk, rv.ld), "out overlaps k or v");
-    check(ci_rope_paged_append(cache.now(), &b, rq.ptr, rq.ld, rk.ptr, rk.ld, rv.ptr, rv.ld, (uint32_t)rq.heads, (const uint16_t *)cos.data_ptr(),
+    // (what is copied overlaps nothing)
+    auto over = [&](const HeadRows &r, int64_t cols) { return r.ptr != nullptr && overlap(y.data_ptr(), rq.T, w, w, r.ptr, rq.T, cols, r.ld); };
+    REFUSE((y.data_ptr() != (const void *)rq.ptr || (rq.T > 1 && rq.ld != w)) && over(rq, w), "out overlaps q; it may be all of q, or none");
+    REFUSE(over(rk, wk) || over(rv, wk), "out overlaps k or v");
+    const ci_paged_cache *c = cache.now();
+    for (HeadRows *r : {&rq, &rk, &rv}) r->ready();
+    check(ci_rope_paged_append(c, &b, rq.ptr, rq.ld, rk.ptr, rk.ld, rv.ptr, rv.ld, (uint32_t)rq.heads, (const uint16_t *)cos.data_ptr(),
                                (const uint16_t *)sin.data_ptr(), (uint32_t)cos.size(0), (uint16_t *)y.data_ptr(), stream()));
     return y;
 }
@@ -688,7 +698,7 @@ py::tuple paged_gather(PagedCache &cache, const Tensor &table, const Tensor &kv_
 Tensor paged_attention(PagedCache &cache, const Tensor &q, const Tensor &table, const Tensor &kv_lens, const OptTensor &q_starts,
                        int64_t max_q_len, int64_t window, int64_t sinks, std::optional<double> scale, const OptTensor &out) {
     const int64_t d = cache.c.head_dim;
-    const HeadRows r = head_rows(q, d, "q", true);
+    HeadRows r = head_rows(q, d, "q", true);
     REFUSE(r.heads % cache.c.n_kv != 0, std::to_string(r.heads) + " query heads over " + std::to_string(cache.c.n_kv) + " key/value heads");
     REFUSE(window < 0 || sinks < 0 || max_q_len < 0, "window, sinks and max_q_len must not be negative");
     constexpr int64_t most = 0x7FFFFFFF;
@@ -706,9 +716,10 @@ Tensor paged_attention(PagedCache &cache, const Tensor &q, const Tensor &table, 
     if (out.has_value()) same_device(y, cache.k, "out");
     else y = at::empty({r.T, r.heads * d}, q.options());
     if (r.T == 0 || b.B == 0) return y;
-    REFUSE(overlap(y.data_ptr(), r.T, r.heads * d, r.T > 1 ? y.stride(0) : r.heads * d, r.ptr, r.T, r.heads * d, r.ld), "out overlaps q");
-    // of this call: from the allocator's pool of the stream, or of the graph that is being captured
+    REFUSE(r.ptr != nullptr && overlap(y.data_ptr(), r.T, r.heads * d, r.T > 1 ? y.stride(0) : r.heads * d, r.ptr, r.T, r.heads * d, r.ld), "out overlaps q");
     const ci_paged_cache *c = cache.now();
+    r.ready();
+    // of this call: from the allocator's pool of the stream, or of the graph that is being captured
     const uint32_t longest = (uint32_t)std::min(max_q_len, most);
     const Tensor ws = at::empty({(int64_t)ci_paged_attention_workspace_bytes(c, &b, (uint32_t)r.heads, longest)}, q.options().dtype(at::kByte));
     check(ci_paged_attention(c, &b, r.ptr, r.ld, (uint32_t)r.heads, longest, (uint32_t)std::min(window, most),

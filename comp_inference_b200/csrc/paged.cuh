@@ -175,6 +175,7 @@ int check_paged(const ci_paged_cache *c, const ci_paged_batch *b, PagedBatch &ou
 PromptPlan prompt_plan(uint32_t head_dim, uint32_t page_size, uint32_t n_kv, const ci_paged_batch *b, uint32_t group, int32_t window,
                        int32_t sinks, uint32_t min_rows, void *workspace);
 size_t prompt_workspace_bytes(uint32_t head_dim, const PromptPlan &l);
+int check_paged_prompt(const ci_paged_cache *c, const PromptPlan &l);
 int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const PromptPlan &l, const uint16_t *q, int64_t ldq, uint32_t n_q,
                         float scale_log2, uint16_t *out, int64_t ldo, cudaStream_t s);
 

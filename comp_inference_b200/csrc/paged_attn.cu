@@ -808,7 +808,7 @@ int ci_paged_attention(const ci_paged_cache *c, const ci_paged_batch *batch, con
     PromptPlan plan = {};
     if (prompts) {
         plan = prompt_plan(c->head_dim, c->page_size, c->n_kv, batch, a.group, a.window, a.sinks, kPaRows, (uint8_t *)d_workspace + few_bytes(c->head_dim));
-        CI_REQUIRE((uint64_t)plan.count * c->n_kv <= 0x7FFFFFFFu, "too many blocks");
+        if (int rc = check_paged_prompt(c, plan)) return rc;
     }
     const bool wide = longest_of(batch, max_q_len) * a.group > 8;
     cudaStream_t s = (cudaStream_t)stream;

@@ -1006,7 +1006,6 @@ static int launch_prompt(const PromptArgs &a, const PromptPlan &l, const CUtenso
     static SmemLimit lim = {};
     if (int rc = ensure_smem_limit(lim, (const void *)k_paged_prompt<D, BITS, SHORT>, Sh::kSmem)) return rc;
     const uint64_t blocks = (uint64_t)l.count * a.p.n_kv;
-    CI_REQUIRE(blocks <= 0x7FFFFFFFu, "too many blocks");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(blocks < l.sms ? blocks : l.sms));
     cfg.blockDim = dim3(Sh::kThreads);
@@ -1039,11 +1038,17 @@ static int pool_map(CUtensorMap *m, const ci_paged_cache *c, void *base) {
     return CI_OK;
 }
 
+// What launch_paged_prompt asks for, asked before the first kernel of a call is queued.
+int check_paged_prompt(const ci_paged_cache *c, const PromptPlan &l) {
+    CI_REQUIRE(c->bits == 4 || (uint64_t)c->num_pages * c->n_kv * c->page_size <= 0x7FFFFFFFu, "a pool of more than 2^31 rows");
+    CI_REQUIRE((uint64_t)l.count * c->n_kv <= 0x7FFFFFFFu, "too many blocks");
+    CI_REQUIRE(encode_tiled_fn() != nullptr, "the driver has no cuTensorMapEncodeTiled");
+    return CI_OK;
+}
+
 // The pieces of a plan that is there when the kernel runs.  Needs group <= 128.
 int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const PromptPlan &l, const uint16_t *q, int64_t ldq, uint32_t n_q,
                         float scale_log2, uint16_t *out, int64_t ldo, cudaStream_t s) {
-    CI_REQUIRE(encode_tiled_fn() != nullptr, "the driver has no cuTensorMapEncodeTiled");
-    CI_REQUIRE(c->bits == 4 || (uint64_t)c->num_pages * c->n_kv * c->page_size <= 0x7FFFFFFFu, "a pool of more than 2^31 rows");
     PromptArgs a;
     a.p = p;
     a.k = (const uint8_t *)c->k; a.v = (const uint8_t *)c->v; a.ks = c->k_scale; a.vs = c->v_scale;
