@@ -701,6 +701,8 @@ Tensor paged_attention(PagedCache &cache, const Tensor &q, const Tensor &table, 
     HeadRows r = head_rows(q, d, "q", true);
     REFUSE(r.heads % cache.c.n_kv != 0, std::to_string(r.heads) + " query heads over " + std::to_string(cache.c.n_kv) + " key/value heads");
     REFUSE(window < 0 || sinks < 0 || max_q_len < 0, "window, sinks and max_q_len must not be negative");
+    const float factor = (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)d));
+    REFUSE(!std::isfinite(factor * 1.4427f), "a scale of " + std::to_string(*scale));
     constexpr int64_t most = 0x7FFFFFFF;
     REFUSE(r.T * r.heads > most, std::to_string(r.T) + " tokens of " + std::to_string(r.heads) + " heads");
     Tensor y;
@@ -723,7 +725,7 @@ Tensor paged_attention(PagedCache &cache, const Tensor &q, const Tensor &table, 
     const uint32_t longest = (uint32_t)std::min(max_q_len, most);
     const Tensor ws = at::empty({(int64_t)ci_paged_attention_workspace_bytes(c, &b, (uint32_t)r.heads, longest)}, q.options().dtype(at::kByte));
     check(ci_paged_attention(c, &b, r.ptr, r.ld, (uint32_t)r.heads, longest, (uint32_t)std::min(window, most),
-                             (uint32_t)std::min(sinks, most), (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)d)), ws.data_ptr(),
+                             (uint32_t)std::min(sinks, most), factor, ws.data_ptr(),
                              ws.nbytes(), (uint16_t *)y.data_ptr(), r.T > 1 ? y.stride(0) : r.heads * d, stream()));
     return y;
 }

@@ -781,6 +781,7 @@ int ci_paged_attention(const ci_paged_cache *c, const ci_paged_batch *batch, con
     CI_REQUIRE(((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out)) & 15u) == 0 && ldq % 8 == 0 && ldo % 8 == 0,
                "queries and output must be 16-byte aligned");
     CI_REQUIRE((uint64_t)a.p.T * n_q <= 0x7FFFFFFFu, "%u tokens of %u query heads", a.p.T, n_q);
+    CI_REQUIRE(isfinite(scale * 1.4427f), "a scale of %g", scale);
     if (a.p.T == 0 || a.p.B == 0) return CI_OK;
     CI_REQUIRE(d_workspace != nullptr && (reinterpret_cast<uintptr_t>(d_workspace) & 15u) == 0, "attention needs an aligned workspace");
     const size_t need = ci_paged_attention_workspace_bytes(c, batch, n_q, max_q_len);

@@ -94,7 +94,7 @@ def paged_attention(q, cache, block_table, kv_lens, q_starts=None, max_q_len=0, 
 
     ``window`` > 0: a token at position i sees positions j with i - j < window, and those with j < ``sinks``.  A token that
     sees nothing (no tokens, no pages) gets zeros.  ``max_q_len``: no sequence has more new tokens than that, 0 if it is not
-    known; it chooses between kernels, and a longer sequence is served all the same.  ``scale``: head_dim ** -0.5 if not given.
+    known; it chooses between kernels, and a longer sequence is served all the same.  ``scale``: a finite number, head_dim ** -0.5 if not given.
     ``out``: rows that do not overlap q, 16-byte aligned (columns of a wider matrix included).
 
     A NaN or +infinity among a token's scores makes its row NaN, -infinity is a weight of 0, nothing but -infinity NaN (0 / 0).

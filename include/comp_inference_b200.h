@@ -440,7 +440,7 @@ int ci_paged_gather(const ci_paged_cache *cache, const ci_paged_batch *batch, ui
  * j <= i of the token's sequence (i: the token's own position) with i - j < window or j < sinks; window = 0: all j <= i.  A
  * token that sees nothing gets zeros.  q rows ldq elements apart, heads head_dim apart, both 16-byte aligned, and out alike
  * with ldo.  max_q_len: no sequence has more new tokens (0: not known; it chooses kernels, and longer ones are served all
- * the same).  d_workspace: ci_paged_attention_workspace_bytes of the same arguments, 16-byte aligned, its contents do not matter; calls that
+ * the same).  scale: finite.  d_workspace: ci_paged_attention_workspace_bytes of the same arguments, 16-byte aligned, its contents do not matter; calls that
  * overlap on the GPU must not share one. */
 size_t ci_paged_attention_workspace_bytes(const ci_paged_cache *cache, const ci_paged_batch *batch, uint32_t n_q,
                                           uint32_t max_q_len);

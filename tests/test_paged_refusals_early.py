@@ -49,6 +49,16 @@ def test_nothing_is_copied_for_a_refused_call(call):
     assert not any("clone" in n or "copy" in n or "contiguous" in n for n in calls.names), calls.names
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39, 3e38])
+def test_a_scale_that_is_not_finite(scale):
+    """3e38 is not in the exponentials' base.  (A NaN made prompts the mean of their values.)"""
+    with pytest.raises(ValueError, match="scale"):
+        ci.paged_attention(bf(3, 4, 128), cache(), i32(3, 2), i32(3), scale=scale)
+    c, b = (C.byref(x) for x in descriptors())
+    assert _lib.load().ci_paged_attention(c, b, 4096, 512, 4, 0, 0, 0, scale, 4096, 1 << 40, 4096, 512, None) == -1
+    assert b"scale" in _lib.load().ci_last_error()
+
+
 def test_a_pool_that_the_prompts_kernel_cannot_index():
     """Refused for that, not for what its first kernel met."""
     lib = _lib.load()
