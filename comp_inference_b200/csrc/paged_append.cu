@@ -15,7 +15,7 @@ int check_paged(const ci_paged_cache *c, const ci_paged_batch *b, PagedBatch &o)
     CI_REQUIRE((uint64_t)c->num_pages * c->n_kv * c->page_size <= 0xFFFFFF00u, "a pool of more than 2^32 rows");
     CI_REQUIRE(((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | reinterpret_cast<uintptr_t>(c->k_scale) |
                  reinterpret_cast<uintptr_t>(c->v_scale)) & 15u) == 0, "pages must be 16-byte aligned");
-    CI_REQUIRE(b->B == 0 || (b->block_table && b->kv_lens), "null block table or lengths");
+    CI_REQUIRE(b->B == 0 || ((b->block_table || b->max_pages == 0) && b->kv_lens), "null block table or lengths");
     CI_REQUIRE(b->B <= (1u << 20) && b->T <= (1u << 30), "%u sequences with %u new tokens", b->B, b->T);
     CI_REQUIRE((uint64_t)b->max_pages * c->page_size <= (1u << 30), "a block table of %u pages of %u tokens", b->max_pages, c->page_size);
     CI_REQUIRE(b->table_stride >= b->max_pages, "block table rows of %u pages %u apart", b->max_pages, b->table_stride);

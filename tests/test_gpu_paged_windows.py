@@ -22,3 +22,21 @@ def test_first_tokens_stay_seen_where_the_window_leaves_them(d, group, new, kv, 
         want, bound = ref.attention(q, cache, table, kv, starts_of(new), window, sinks)
         over = (got.double().view_as(want) - want).abs() > bound
         assert not bool(over.any()), (window, sinks, over.flatten(1).any(1).nonzero().flatten().tolist()[:10])
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_table_without_pages(bits):
+    """No token has a page: attention and gather give zeros, an append rotates and writes nothing."""
+    g = gen(bits)
+    cache = make_cache(g, 3, 16, 1, 64, bits)
+    before = [x.clone() for x in (cache.k, cache.v)]
+    table = torch.empty(2, 0, dtype=torch.int32, device=DEV)
+    one, none = torch.ones(200, 64, dtype=torch.bfloat16, device=DEV), torch.zeros(200, 64, dtype=torch.bfloat16, device=DEV)
+    for new, kv in ((None, [5, 0]), ([100, 3], [150, 3])):
+        starts = starts_of(new) if new else None
+        T = sum(new) if new else 2
+        q, k = rnd(g, T, 2, 64).to(torch.bfloat16).to(DEV), rnd(g, T, 1, 64).to(torch.bfloat16).to(DEV)
+        assert bool((ci().paged_attention(q, cache, table, i32(kv), starts) == 0).all())
+        rotated = ci().rope_paged_append(q, k, k, one, none, cache, table, i32(kv), starts)
+        assert torch.equal(rotated[0], q[0]) and all(torch.equal(x, y) for x, y in zip((cache.k, cache.v), before))
+        assert all(bool((x == 0).all()) for x in ci().paged_gather(cache, table, i32(kv), starts, T))

@@ -65,3 +65,12 @@ def test_a_pool_that_the_prompts_kernel_cannot_index():
     c, b = (C.byref(x) for x in descriptors(num_pages=(1 << 24) + 1, page_size=128, n_kv=1, q_starts=4096, T=500))
     assert lib.ci_paged_attention(c, b, 4096, 512, 4, 0, 0, 0, 1.0, 4096, 1 << 40, 4096, 512, None) == -1
     assert b"2^31" in lib.ci_last_error()
+
+
+def test_a_table_without_pages_is_no_argument_error():
+    """(Its pointer is null; what is refused is its device.)"""
+    for call in (lambda: ci.paged_attention(bf(3, 4, 128), cache(), i32(3, 0), i32(3)), lambda: ci.paged_gather(cache(), i32(3, 0), i32(3))):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            call()
+    c, b = (C.byref(x) for x in descriptors(block_table=None, max_pages=0, table_stride=0, T=(1 << 30) + 1))
+    assert _lib.load().ci_paged_gather(c, b, 4096, 4096, None) == -1 and b"null" not in _lib.load().ci_last_error()
