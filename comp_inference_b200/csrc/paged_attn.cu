@@ -459,11 +459,12 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
                                 if (kAll) {
                                     corr[nr][gr][0] += x0 * middle;
                                     corr[nr][gr][1] += x1 * middle;
-                                } else {                        // steps that nobody wrote: 0 times them need not be 0
-                                    if (x0 == 0.f) y &= 0xFFFF0000u;
-                                    if (x1 == 0.f) y &= 0x0000FFFFu;
-                                    corr[nr][gr][0] += x0 == 0.f ? 0.f : x0 * middle;
-                                    corr[nr][gr][1] += x1 == 0.f ? 0.f : x1 * middle;
+                                } else {                        // steps that the row does not see: 0 times them need not be 0
+                                    const bool no0 = sc[u][nr][2 * j] == kNone, no1 = sc[u][nr][2 * j + 1] == kNone;
+                                    if (no0) y &= 0xFFFF0000u;
+                                    if (no1) y &= 0x0000FFFFu;
+                                    corr[nr][gr][0] += no0 ? 0.f : x0 * middle;
+                                    corr[nr][gr][1] += no1 ? 0.f : x1 * middle;
                                 }
                                 pb[nr][j] = transpose8x8(y);
                             }

@@ -245,3 +245,24 @@ def test_values_that_shrink_under_a_window(d, group, new, kv, window):
     q = rnd(g, new, group, d).to(torch.bfloat16).to(DEV)
     for sinks in (0, 3):
         compare(q, cache, table, [kv], [new], window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("new", [None, [3], [80]])
+def test_a_nan_among_values_of_the_smallest_weight(new, bits):
+    """A weight that is 0 in 32 bits is not 0: a NaN that a token sees makes its channels NaN, wherever in the tiles it lies."""
+    g = gen(31)
+    d, kv = 128, [300]
+    for j in (5, 130, 290 if new != [80] else 219):
+        cache, table = make_cache(g, 10, 32, 1, d, bits), make_table(g, kv, 32, 10)
+        i = ref.page(cache, table, 0, j)
+        if bits == 16:
+            cache.k[i, 0, j % 32] = -2.0
+            cache.v[i, 0, j % 32, :64] = NAN
+        else:
+            cache.k_scale[i, 0, j % 32, :, 0] = 0.0
+            cache.k_scale[i, 0, j % 32, :, 1] = -2.0
+            cache.v_scale[i, 0, j % 32, 0] = NAN
+        q = torch.ones(new[0] if new else 1, 4, d, dtype=torch.bfloat16, device=DEV)
+        got = ci().paged_attention(q, cache, table.to(DEV), i32(kv), starts_of(new) if new else None, scale=1.0).view(-1, 4, d)
+        assert bool(got[..., :64].isnan().all()) and not bool(got[..., 64:].isnan().any())
