@@ -161,6 +161,11 @@ __device__ __forceinline__ void plan_prompts(const PagedBatch &p, const PromptPl
 // its sum is then 0 or NaN, and the row NaN, as the definition has it.
 constexpr float kNone = -INFINITY, kLeast = -3.402823466e38f;
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ float lo_bf16(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_bf16(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {

@@ -30,7 +30,7 @@ struct PagedAttnArgs {
     const uint32_t *ks, *vs;
     const uint16_t *q;
     int64_t ldq;                                 // elements between tokens; heads lie D apart
-    uint32_t n_q, group;
+    uint32_t group;
     int32_t window, sinks;                       // window 0: none
     float scale_log2;
     uint32_t max_rows;                           // sequences with more rows (queries x heads of a group) are not this kernel's
@@ -40,11 +40,6 @@ struct PagedAttnArgs {
     float *ml, *partial;                         // [blocks][2][rows][2], [blocks][2][rows][D]
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -793,7 +788,6 @@ int ci_paged_attention(const ci_paged_cache *c, const ci_paged_batch *batch, con
     a.k = (const uint8_t *)c->k; a.v = (const uint8_t *)c->v; a.ks = c->k_scale; a.vs = c->v_scale;
     a.q = d_q;
     a.ldq = ldq;
-    a.n_q = n_q;
     a.group = n_q / c->n_kv;
     constexpr uint32_t kFar = 1u << 30;                         // further than any position lies
     a.window = (int32_t)(window >= kFar ? 0 : window);

@@ -44,7 +44,7 @@ struct PromptArgs {
     PagedBatch p;
     const uint8_t *k, *v;                    // 4 bits only
     const uint32_t *ks, *vs;
-    uint32_t n_q, group, tt, negate;
+    uint32_t group, tt, negate;
     int32_t window, sinks;
     float scale_log2;                        // not negative
     uint16_t *out;
@@ -87,12 +87,6 @@ struct PromptShape {
     static constexpr int kHeld = BITS == 16 ? 4 : 2;                         // groups of 32 scores that a row's thread holds
     static constexpr uint32_t cO = NT * kKt;                                 // first column of O
 };
-
-__device__ __forceinline__ float ex2f(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // A query tile: positions of its first and last token (p1 < p0: it has none), and which of the block's key tiles they see: the
 // first tokens' and [from, to).
@@ -438,7 +432,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                 bool exact = edge;
                 if (__any_sync(kFull, grow || odd || v_move != 0)) {
                     exact |= BITS == 16 && __any_sync(kFull, odd);
-                    float c = grow ? ex2f(m - mx) : 1.f;
+                    float c = grow ? ex2(m - mx) : 1.f;
                     if (grow) m = mx;
 #pragma unroll
                     for (int e = 0; e < kSums; ++e) l2[e] = fma2(l2[e], pair(c, c), 0);
@@ -488,8 +482,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                                 ex2_poly(y, e0, e1);
                             } else {
                                 split(y, e0, e1);
-                                e0 = ex2f(e0);
-                                e1 = ex2f(e1);
+                                e0 = ex2(e0);
+                                e1 = ex2(e1);
                             }
                             l2[j % kSums] = add2(l2[j % kSums], pair(e0, e1));
                             pk[j] = BITS == 16 ? pack_bf16(e0, e1) : pack_f16(e0, e1);
@@ -958,13 +952,13 @@ __global__ void __launch_bounds__(256) k_prompt_join(const __grid_constant__ Pro
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) most = fmaxf(most, ml[i].x);
             if (most == kNone) continue;
-            const float down = M == kNone ? 0.f : ex2f(M - most);
+            const float down = M == kNone ? 0.f : ex2(M - most);
             M = most;
             L *= down;
             y.x *= down; y.y *= down; y.z *= down; y.w *= down;
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
-                const float e = ml[i].x == kNone ? 0.f : ex2f(ml[i].x - M);
+                const float e = ml[i].x == kNone ? 0.f : ex2(ml[i].x - M);
                 L += e * ml[i].y;
                 y.x += e * z[i].x; y.y += e * z[i].y; y.z += e * z[i].z; y.w += e * z[i].w;
             }
@@ -1052,7 +1046,6 @@ int launch_paged_prompt(const ci_paged_cache *c, const PagedBatch &p, const Prom
     PromptArgs a;
     a.p = p;
     a.k = (const uint8_t *)c->k; a.v = (const uint8_t *)c->v; a.ks = c->k_scale; a.vs = c->v_scale;
-    a.n_q = n_q;
     a.group = n_q / c->n_kv;
     a.tt = 128 / a.group;
     a.negate = scale_log2 < 0.f;
