@@ -24,10 +24,11 @@ struct PagedBatch {
 // How the prompts' kernel (paged_prompt.cu) shares its work, made on the device by k_paged_join, which runs before it.  An item is
 // per_item tokens of a sequence for one key/value head.  Items with many more key tiles than others are cut into pieces: no shorter
 // than a multiprocessor's share of all tiles where there are no more items than multiprocessors, so that the pieces are not
-// more either and run at once (pieces no longer than the share would be up to one more for every item, a second round: 16
-// sequences of 32 new tokens and 2048 in all 67 us instead of 42); half of that where a multiprocessor has several items anyway.
+// more either and run at once (of half a share: 16 sequences of 32 new tokens and 2048 in all 58 us instead of 43, uncut 39; 8 of 32
+// over 8000 80 instead of 74, uncut 102); half of that where a multiprocessor has several items anyway (12 sequences of 200 new
+// tokens and 300 to 30000 in all, 32 heads of 128 over 8: 454 us, whole shares 621, uncut 618).
 // Not shorter than kFewest either: a piece begins with queries and first keys one after the other and ends with k_prompt_join.
-// 32 tokens behind 8000 others, eight sequences of it: 79 us, uncut 108; 64 tokens behind 32000: 87 us, uncut 402.
+// 64 tokens of a sequence of 32000: 59 us, uncut 397.
 constexpr uint32_t kKt = 128;                // positions per key tile
 constexpr uint32_t kFewest = 4;
 struct PromptPlan {

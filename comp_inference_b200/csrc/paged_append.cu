@@ -110,8 +110,9 @@ struct TokenPart {
 // A warp has a token, or a share of its heads: its sequence, place, page and angles are looked up once for all of them.  A head takes
 // D / 16 lanes: a lane has eight channels of its lower half and the eight that are rotated with them.  Groups of 64 channels
 // lie in eight lanes (four of them, both halves, for D = 64).  Two rounds of heads are in flight.  7100 tokens of 32 + 8 + 8
-// heads of 128: 35 us, 5.1 TB/s: memory.  Into 4 bits, 8500 tokens: 55 us, the codes' arithmetic and its registers (three blocks on a
-// multiprocessor; two take 60).
+// heads of 128: 35 us, 5.1 TB/s: memory.  Into 4 bits, 8500 tokens: 53 us, 2.8 TB/s, neither memory nor a pipe (integers 40 %, issue slots
+// 57 %): latency, with three blocks of 80 registers on a multiprocessor (two take 58).  The angles are 32 of those registers in fp32; all
+// variants spill 28 to 44 bytes a thread.
 template <int D, int BITS>
 __global__ void __launch_bounds__(256, BITS == 16 ? 4 : 3) k_rope_append(const __grid_constant__ AppendArgs a) {
     constexpr uint32_t LANES = D / 16, G = D / kGroup, PER = 32 / LANES, FLIGHT = 2;
@@ -234,8 +235,9 @@ struct GatherArgs {
     uint32_t parts;
 };
 
-// Rows of a cache as bf16 (23 thousand tokens of 8 heads of 128 out of 4 bits: 29 us, 4.4 TB/s), a token, or a share of its heads, per warp: a row takes D / 8 lanes, 16 bytes to each; positions without
-// a page give zeros.
+// Rows of a cache as bf16, a token, or a share of its heads, per warp: a row takes D / 8 lanes, 16 bytes to each; positions without a page
+// give zeros.  23 thousand tokens of 8 heads of 128 out of 4 bits, 123 MB: 33 us, 3.8 TB/s (integers 54 %, issue slots 57 %, loads
+// under way); 8 thousand out of bf16, 69 MB that stay in L2: 9 us.
 template <int D, int BITS>
 __global__ void __launch_bounds__(256) k_paged_gather(const __grid_constant__ GatherArgs a) {
     constexpr uint32_t LANES = D / 8, G = D / kGroup, PER = 32 / LANES;

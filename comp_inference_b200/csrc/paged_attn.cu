@@ -13,10 +13,12 @@
 // one long sequence among short ones, or a single sequence, fills the machine; what a block boundary cuts is joined by
 // k_paged_join from (max, sum, output) of the parts.  Lengths are read on the device: a captured call serves any.
 //
-// What bounds it: in bf16 memory (32 sequences of 1 to 16000 tokens, 251 MB: 50 us, 5.0 TB/s, 45 of them this kernel); heads of 64
-// and small pages latency (67 MB of a window: 18 us); 4 bits the instructions that turn codes into operands, 7 for eight keys and 11
-// for eight values beside the permutes (417 MB: 142 us, 2.9 TB/s, integer pipe 59 % and issue slots 54 % of the time; four or five
-// blocks of fewer registers on a multiprocessor 151 to 191 us); a short step the launches (513 tokens of 32 heads: 10.9 us).
+// What bounds it: in bf16 memory (32 sequences of 1 to 16000 tokens, 251 MB: 49 us, 45 of them this kernel, 5.4 TB/s; it spills in heads
+// of 256 alone); heads of 64 and small pages the bytes in flight (67 MB of a window: 18 us of inputs that stay in L2, 22 of others; values
+// are asked for where they are used, only keys a tile ahead); 4 bits the instructions that turn codes into operands, 7 for eight keys and
+// 11 for eight values beside the permutes, and the latency that 12 warps leave between them (417 MB: 139 us, 3.0 TB/s, integer pipe 60 %
+// and issue slots 55 % of the time; four blocks on a multiprocessor 186 us, with one tile at a time 150); a short step its two
+// launches and the chain of latencies in each (513 tokens of 32 heads: 10.4 us).
 #include "paged.cuh"
 #include "ptx.cuh"
 
@@ -67,7 +69,7 @@ struct Span {
 
 // What starting on a group of rows and putting its result together costs, in tiles: lengths, queries, page ids, first keys, one
 // after the other.  Without it the blocks that get the short sequences of a batch end last (32 sequences of 1 to 16000 tokens, 251 MB:
-// 81.6 us with 0, 57.1 with 1, 51.5 with 3, 52.2 with 6).
+// 79.2 us with 0, 54.7 with 1, 48.9 with 3, 49.7 with 6).
 constexpr uint32_t kItemCost = 3;
 
 // Units of work of a sequence's groups of rows, and the number of those groups.  One group: its own tiles; several: no
@@ -421,7 +423,9 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
                         l[nr][e & 1] += pr[nr][e];
                     }
                 if constexpr (BITS == 16) {
-                    uint32_t pb[NR][2];                         // the weights in bf16, as the tensor instructions take them
+                    // The weights in bf16, the type of the values, which the tensor instructions want alike: half a step of 2^-8
+                    // of each, the sums in fp32 (outputs 0.0016 to 0.0021 from 64 bits in the mean, 0.0016 of it their own rounding).
+                    uint32_t pb[NR][2];
 #pragma unroll
                     for (int nr = 0; nr < NR; ++nr) {
                         pb[nr][0] = transpose8x8(pack_bf16(pr[nr][0], pr[nr][1]));
@@ -442,7 +446,7 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
 #pragma unroll
                     for (int gr = 0; gr < G; ++gr) {
                         // v = low + step c = middle + step (c - 8): the step goes with the weight, and what its product loses by
-                        // rounding counts c - 8 times
+                        // rounding to bf16 counts c - 8 times (outputs 0.0023 from 64 bits in the mean)
                         uint32_t pb[NR][2];
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
@@ -588,7 +592,8 @@ __global__ void __launch_bounds__(kPaThreads, D == 64 ? 4 / NR : D == 128 && NR 
 
 // Joins the parts of an item that several blocks had: block c has the item that block c of the attention began, all rows at once, if
 // that has few parts.  Items of many parts are few, and the blocks share their rows: a block per row, its threads over the
-// parts (5 items of 59 parts, heads of 256: the join's 55 us became 13).  Everything in a fixed order: the same sum every time.
+// parts (a step of 5 sequences of 20000 tokens, eight heads of 256 over one, 59 parts each: 36.4 us, 42.2 without).  Everything in a
+// fixed order: the same sum every time.
 constexpr int32_t kFewParts = 16, kAtOnce = 8;
 
 template <int D, int RT>
@@ -697,8 +702,8 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Page
 }
 
 constexpr uint32_t kPaMaxRows = 16;              // widest group of query rows of any variant
-// Query rows of a sequence and key head up to which this kernel has them.  48 drawn batches with sequences around it: up to 32 rows
-// 5 % slower in the mean, 16 10 %, 8 17 % (batches of 60 to 230 rows gain up to 40 %, those that need no other kernel lose up to half).
+// Query rows of a sequence and key head up to which this kernel has them.  24 drawn batches of 6 to 120 rows over 250 to 12000
+// tokens: up to 32 rows 8 % slower in the mean, 16 21 %, 8 31 %; 128 13 % faster (0.44 to 1.01 of the time).
 constexpr uint32_t kPaRows = 64;
 constexpr uint32_t kPaMaxResident = 4;           // blocks of a multiprocessor that the workspace has room for
 
@@ -712,8 +717,8 @@ static int resident_blocks(const void *kernel, uint32_t &blocks) {
 
 template <int D, int BITS, int NR>
 static int launch_attention(const PagedAttnArgs &a, const PromptPlan &plan, cudaStream_t s) {
-    // 4 bits: two tiles of 16 tokens at once; heads of 256 have no registers for that (contexts of hundreds of tokens 31 -> 24 us
-    // with one, of 38000 99 -> 105).  bf16 heads of 64: 25 us with two where one takes 21.
+    // 4 bits: two tiles of 16 tokens at once; heads of 256 have no registers for that (32 sequences of 100 to 700 tokens 22.4 us with
+    // two, 17.8 with one; four of 38000 86.5 and 87.5).  bf16 heads of 64: 23.4 us with two where one takes 18.1.
     constexpr int U = BITS == 4 && D < 256 ? 2 : 1;
     static uint32_t resident = 0;
     if (resident == 0)

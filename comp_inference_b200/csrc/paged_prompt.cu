@@ -14,20 +14,22 @@
 // Blocks stay, one on each multiprocessor, and take piece after piece of the plan that k_paged_join has made (PromptPlan): one warp
 // fetches the next piece and says what it sees, one issues the TMA copies, one per query tile the products, and each goes on to the
 // next piece when its own part is done, so that queries, first keys and first scores of the next are there when the rows of
-// this one are written (4096 tokens, 32 heads of 128 over 8: a block for each piece 135 us, 127 so; six prompts of 1024, 64 heads of
-// 64 over 16, under a window of 256: 123 and 89).  mbarriers connect the roles.  All waits are bounded: on expiry a role sets the
-// status word and the abort flag, and everyone leaves.
+// this one are written (4096 tokens, 32 heads of 128 over 8: a block for each piece 134 us, 122 so; six prompts of 1024, 64 heads of
+// 64 over 16, under a window of 256: 155 and 106; 16 of 256: 49 and 40).  mbarriers connect the roles.  All waits are bounded: on
+// expiry a role sets the status word and the abort flag, and everyone leaves when its copies and products under way are there.
 //
 // A cache of 4 bits is turned into fp16 on its way into shared memory by four or eight warps, so that what codes stand for, and the
-// weights, are rounded by 2^-12 and not 2^-9 (error of a prompt's outputs against 64 bits 0.0017 instead of 0.0034; bf16's own
+// weights, are off by 2^-11 of themselves at most and not 2^-8 (mean error of a prompt's outputs against 64 bits 0.0017; bf16's own
 // rounding of the result is 0.0016).  fp16 has no range for that by itself: every key tile is scaled by the power of two that
 // its largest value asks for, the values by one that changes when a tile leaves its range, O following it, and a query row by its own.
 // A value tile's largest lies between 2^8 and 2^15 of its scale, so steps and lowest values down to 2^-25 of that are held exactly.  The
 // scale stays above 2^-92 of the largest value of the piece so far: O of the rows that have seen that one must not overflow.
 //
-// What bounds it: in bf16 the chain from a tile's scores over its exponentials to its product, with two tiles in turn (tensor
-// pipe 61 % active, issue slots 47 %, special functions 47 %; 16001 tokens under a window of 4096: 772 us, 1214 TFLOP/s, 0.73 of the
-// measured rate); in 4 bits the arithmetic of turning codes (4096 tokens 197 us, without it 158; tensor pipe 35 %, issue slots 53 %).
+// What bounds it: in bf16 the chain from a tile's scores over its exponentials to its product, with two tiles in turn (4096 tokens
+// 122 us, 1126 TFLOP/s, tensor pipe 61 % active, issue slots 47 %; 16001 tokens under a window of 4096: 860 to 900 us under the power
+// cap, 1040 to 1090 TFLOP/s, 0.75 to 0.78 of the measured sustained rate); in 4 bits the arithmetic of turning codes, which every block
+// does for itself (4096 tokens 194 us, integer pipe 42 %, issue slots 55 %), scores read twice from tensor memory, and the
+// producers' meeting in every tile.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -151,7 +153,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // 2^x of two values, x <= 2^6, in the fused multiply-add units: the integer next to x goes into the exponent field, 2^f for the rest
 // in [-1/2, 1/2] is a polynomial of degree 3 fitted for the smallest largest relative error, 7.5e-5, a fiftieth of what rounding to
 // bf16 loses.  The special-function unit makes four results per cycle and scheduler; a quarter of the weights comes from here
-// (4096 tokens, 32 heads of 128 over 8: 160.6 us when it was tried, none of them 167.6, half 181.8).  For x of
+// (4096 tokens, 32 heads of 128 over 8: 121.7 us, none of them 124.0, half 140.0).  For x of
 // -126 and less it gives 2^-126, not 0, and for a NaN too: not for tiles with hidden scores, nor where a row's largest is not finite.
 constexpr float kExp0 = 0.99992812f, kExp1 = 0.69326097f, kExp2 = 0.24261075f, kExp3 = 0.05517141f;
 __device__ __forceinline__ void ex2_poly(uint64_t x, float &r0, float &r1) {
@@ -449,8 +451,7 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                     }
                 }
                 // Rows of V that no query of the block sees become zeros: 0 times what lies there need not be 0.  A thread has the row of
-                // its number; both query tiles write them, as neither waits for the other.  (The copying warp alone took 15 us over a
-                // tile: a prompt of 16001 under a window of 4096 1225 us instead of 780 then.)
+                // its number; both query tiles write them, as neither waits for the other.
                 if (BITS == 16 && (f + (int32_t)kKt > kt.hi || (a.window && f < kt.lo && f + (int32_t)kKt > a.sinks))) {
                     const uint32_t c = ring0 + 2 * (uint32_t)i + 1;
                     if (!__all_sync(kFull, mbar_wait(bar(Sh::bFull + c % NS), (c / NS) & 1, polls(16)))) {
@@ -485,6 +486,8 @@ k_paged_prompt(const __grid_constant__ PromptArgs a, const __grid_constant__ CUt
                                 e0 = ex2(e0);
                                 e1 = ex2(e1);
                             }
+                            // (in the values' type, as the tensor instructions want: half a step of bf16 is 2^-8 of a weight, of fp16
+                            // 2^-11; sums in fp32.  Outputs in bf16 0.0020 from 64 bits in the mean, 0.0016 of it their own rounding.)
                             l2[j % kSums] = add2(l2[j % kSums], pair(e0, e1));
                             pk[j] = BITS == 16 ? pack_bf16(e0, e1) : pack_f16(e0, e1);
                         }
